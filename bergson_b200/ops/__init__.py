@@ -12,20 +12,26 @@ from .functional import (
     rotary_tables,
     swiglu,
     token_cross_entropy,
+    token_distillation,
     use_fused,
 )
+from .packed import PackedSequences, packed_causal_attention, packed_rotary
 
 __all__ = [
     "Linear",
+    "PackedSequences",
     "linear",
     "causal_attention",
     "composable",
     "gelu",
     "layer_norm",
+    "packed_causal_attention",
+    "packed_rotary",
     "rms_norm",
     "rotary",
     "rotary_tables",
     "swiglu",
     "token_cross_entropy",
+    "token_distillation",
     "use_fused",
 ]

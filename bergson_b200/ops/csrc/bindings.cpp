@@ -10,6 +10,7 @@
 #include <map>
 #include <mutex>
 
+#include "bindings.h"
 #include "kernels.h"
 #include "kernels_cov.h"
 #include "kernels_peer.h"
@@ -76,6 +77,8 @@ static int64_t partial_blocks(int64_t d) { return d <= 1024 ? 148 * 8 : (d <= 20
 int* status_ptr_current() { return status_tensor(at::cuda::current_device()).data_ptr<int>(); }
 
 }  // namespace
+
+int* bgn_status_word(const at::Tensor& like) { return status_ptr(like); }
 
 std::vector<at::Tensor> rmsnorm_fwd(at::Tensor x, at::Tensor w, double eps) {
   CHECK_CUDA_CONTIG(x); CHECK_CUDA_CONTIG(w);
@@ -786,4 +789,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("proj_token_rows", &proj_token_rows);
   m.def("wait_probe", &wait_probe);
   m.def("kernel_status", &kernel_status);
+  bgn_register_packed(m);
 }

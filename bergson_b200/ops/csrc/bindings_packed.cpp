@@ -1,0 +1,236 @@
+// Python bindings of the operators on packed documents and of the distillation loss: checks,
+// allocation of outputs, current-stream lookup.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include "bindings.h"
+#include "kernels_distill.h"
+#include "kernels_packed.h"
+
+namespace {
+
+int type_of(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kHalf: return 0;
+    case at::kBFloat16: return 1;
+    case at::kFloat: return 2;
+    default: TORCH_CHECK(false, "bergson_b200: unsupported dtype ", t.scalar_type());
+  }
+}
+
+void ran(int err, const char* what) {
+  TORCH_CHECK(err == 0, "bergson_b200: ", what, " failed: ", cudaGetErrorString(static_cast<cudaError_t>(err)));
+}
+
+cudaStream_t current() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+// [tokens, heads, dim] as the kernels read it: contiguous features, heads and tokens on 16-byte
+// boundaries, the token stride a multiple of the head stride.  Anything else is copied.
+at::Tensor readable(const at::Tensor& x) {
+  const int64_t packet = 16 / x.element_size();
+  const int64_t st = x.stride(0), sh = x.stride(1);
+  const bool heads_ok = x.size(1) == 1 || (sh >= x.size(2) && sh % packet == 0);
+  const int64_t head = x.size(1) == 1 ? x.size(2) : sh;
+  const bool tokens_ok = !heads_ok || x.size(0) == 1 || (st >= head * x.size(1) && st % packet == 0 && st % head == 0);
+  const bool aligned = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  return (x.stride(2) == 1 || x.size(2) == 1) && heads_ok && tokens_ok && aligned ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+// Strides of a readable tensor; those of a single head or token are never used but must be sound.
+std::pair<long, long> strides_of(const at::Tensor& x) {
+  const long head = x.size(1) == 1 ? x.size(2) : x.stride(1);
+  const long tok = x.size(0) == 1 ? head * x.size(1) : x.stride(0);
+  return {tok, head};
+}
+
+void check_packed(const at::Tensor& q, const at::Tensor& k) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 3 && q.size(0) == k.size(0) && q.size(2) == k.size(2) &&
+                  q.scalar_type() == k.scalar_type() && k.device() == q.device(),
+              "bergson_b200: q [T, H, D] and k [T, H_kv, D] of one dtype and device expected");
+}
+
+void check_index(const at::Tensor& x, int64_t n, const at::Tensor& like) {
+  TORCH_CHECK(x.scalar_type() == at::kInt && x.is_contiguous() && x.device() == like.device() && x.numel() == n,
+              "bergson_b200: the packing does not fit the tensors");
+}
+
+BgnPackedAttention packed_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& first_key,
+                               const at::Tensor& end_query, const at::Tensor& query_order, const at::Tensor& key_order,
+                               int64_t valid, double scale) {
+  const int64_t rows = q.size(0), tiles = (rows + 127) / 128;
+  check_packed(q, k);
+  TORCH_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device(),
+              "bergson_b200: k and v must be alike");
+  TORCH_CHECK(rows < (int64_t(1) << 30) && valid >= 0 && valid <= rows, "bergson_b200: row count out of range");
+  TORCH_CHECK(2 * tiles * q.size(1) < (int64_t(1) << 31), "bergson_b200: too many tiles for one launch");
+  check_index(first_key, rows, q);
+  check_index(end_query, rows, q);
+  check_index(query_order, tiles, q);
+  check_index(key_order, tiles, q);
+  BgnPackedAttention a = {};
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  std::tie(a.q_tok, a.q_head) = strides_of(q);
+  std::tie(a.k_tok, a.k_head) = strides_of(k);
+  std::tie(a.v_tok, a.v_head) = strides_of(v);
+  a.first_key = first_key.data_ptr<int>();
+  a.end_query = end_query.data_ptr<int>();
+  a.query_order = query_order.data_ptr<int>();
+  a.key_order = key_order.data_ptr<int>();
+  a.rows = int(rows);
+  a.valid = int(valid);
+  a.heads = int(q.size(1));
+  a.kv_heads = int(k.size(1));
+  a.dim = int(q.size(2));
+  a.type = type_of(q);
+  a.scale = float(scale);
+  return a;
+}
+
+std::vector<at::Tensor> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor first_key,
+                                             at::Tensor end_query, at::Tensor query_order, at::Tensor key_order,
+                                             int64_t valid, double scale) {
+  c10::cuda::CUDAGuard guard(q.device());
+  check_packed(q, k);
+  q = readable(q);
+  k = readable(k);
+  v = readable(v);
+  const auto a = packed_args(q, k, v, first_key, end_query, query_order, key_order, valid, scale);
+  auto o = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  auto lse2 = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  ran(bgn_packed_attention_fwd(&a, o.data_ptr(), lse2.data_ptr<float>(), bgn_status_word(q), current()),
+      "packed_attention_fwd");
+  return {o, lse2};
+}
+
+std::vector<at::Tensor> packed_attention_bwd(at::Tensor d_o, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
+                                             at::Tensor lse2, at::Tensor first_key, at::Tensor end_query,
+                                             at::Tensor query_order, at::Tensor key_order, int64_t valid, double scale) {
+  c10::cuda::CUDAGuard guard(q.device());
+  check_packed(q, k);
+  q = readable(q);
+  k = readable(k);
+  v = readable(v);
+  TORCH_CHECK(d_o.sizes() == q.sizes() && d_o.scalar_type() == q.scalar_type() && d_o.device() == q.device() &&
+                  o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.is_contiguous() &&
+                  lse2.scalar_type() == at::kFloat && lse2.is_contiguous() && lse2.numel() == q.size(0) * q.size(1),
+              "bergson_b200: the output's gradient does not fit the operands");
+  d_o = readable(d_o);
+  const auto a = packed_args(q, k, v, first_key, end_query, query_order, key_order, valid, scale);
+  auto delta = at::empty_like(lse2);
+  auto dq = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  auto dk = at::empty({k.size(0), k.size(1), k.size(2)}, k.options());
+  auto dv = at::empty_like(dk);
+  const auto [tok, head] = strides_of(d_o);
+  ran(bgn_packed_attention_bwd(&a, o.data_ptr(), lse2.data_ptr<float>(), d_o.data_ptr(), tok, head,
+                               delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                               bgn_status_word(q), current()),
+      "packed_attention_bwd");
+  return {dq, dk, dv};
+}
+
+std::vector<at::Tensor> packed_rotary(at::Tensor q, at::Tensor k, at::Tensor cos, at::Tensor sin, at::Tensor position,
+                                      int64_t rot, bool inverse) {
+  c10::cuda::CUDAGuard guard(q.device());
+  check_packed(q, k);
+  check_index(position, q.size(0), q);
+  TORCH_CHECK(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat && cos.is_contiguous() &&
+                  sin.is_contiguous() && cos.sizes() == sin.sizes() && cos.dim() == 2 && cos.size(1) == rot / 2 &&
+                  cos.device() == q.device() && sin.device() == q.device(),
+              "bergson_b200: rotary tables [positions, rot / 2] in fp32 expected");
+  const auto inner = [](const at::Tensor& x) {
+    return x.size(2) == 1 || x.stride(2) == 1 ? x : x.clone(at::MemoryFormat::Contiguous);
+  };
+  q = inner(q);
+  k = inner(k);
+  BgnPackedRotary a = {};
+  auto qo = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  auto ko = at::empty({k.size(0), k.size(1), k.size(2)}, k.options());
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.q_tok = q.stride(0);
+  a.q_head = q.stride(1);
+  a.k_tok = k.stride(0);
+  a.k_head = k.stride(1);
+  a.position = position.data_ptr<int>();
+  a.cos = cos.data_ptr<float>();
+  a.sin = sin.data_ptr<float>();
+  a.q_out = qo.data_ptr();
+  a.k_out = ko.data_ptr();
+  a.rows = int(q.size(0));
+  a.heads = int(q.size(1));
+  a.kv_heads = int(k.size(1));
+  a.dim = int(q.size(2));
+  a.rot = int(rot);
+  a.type = type_of(q);
+  a.sign = inverse ? -1.f : 1.f;
+  ran(bgn_packed_rotary(&a, current()), "packed_rotary");
+  return {qo, ko};
+}
+
+BgnDistill distill_args(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher, double temperature) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1 && logits.stride(0) >= logits.size(1),
+              "bergson_b200: logits [T, V] with contiguous rows expected");
+  TORCH_CHECK(ids.dim() == 2 && ids.sizes() == teacher.sizes() && ids.size(0) == logits.size(0) && ids.is_contiguous() &&
+                  teacher.is_contiguous() && ids.device() == logits.device() && teacher.device() == logits.device() &&
+                  (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt),
+              "bergson_b200: teacher ids and logits [T, K] expected");
+  TORCH_CHECK(logits.size(1) < (int64_t(1) << 30), "bergson_b200: vocabulary out of range");
+  BgnDistill a = {};
+  a.logits = logits.data_ptr();
+  a.ids = ids.data_ptr();
+  a.teacher = teacher.data_ptr();
+  a.pitch = logits.stride(0);
+  a.tokens = logits.size(0);
+  a.vocab = int(logits.size(1));
+  a.top = int(ids.size(1));
+  a.type = type_of(logits);
+  a.teacher_type = type_of(teacher);
+  a.ids_64 = ids.scalar_type() == at::kLong;
+  a.temperature = float(temperature);
+  return a;
+}
+
+// Rows the kernels can walk; a single row's pitch is of no account.
+at::Tensor rows_of(const at::Tensor& x) {
+  return x.stride(1) == 1 && x.stride(0) >= x.size(1) ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+std::vector<at::Tensor> distill_fwd(at::Tensor logits, at::Tensor ids, at::Tensor teacher, double temperature) {
+  c10::cuda::CUDAGuard guard(logits.device());
+  logits = rows_of(logits);
+  const auto a = distill_args(logits, ids, teacher, temperature);
+  auto loss = at::empty({logits.size(0)}, logits.options().dtype(at::kFloat));
+  auto stats = at::empty({logits.size(0), 2}, loss.options());
+  ran(bgn_distill_fwd(&a, loss.data_ptr<float>(), stats.data_ptr<float>(), current()), "distill_fwd");
+  return {loss, stats};
+}
+
+at::Tensor distill_bwd(at::Tensor logits, at::Tensor ids, at::Tensor teacher, at::Tensor stats, at::Tensor dloss,
+                       double temperature) {
+  c10::cuda::CUDAGuard guard(logits.device());
+  logits = rows_of(logits);
+  const auto a = distill_args(logits, ids, teacher, temperature);
+  TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 2 * logits.size(0) &&
+                  dloss.scalar_type() == at::kFloat && dloss.is_contiguous() && dloss.numel() == logits.size(0) &&
+                  stats.device() == logits.device() && dloss.device() == logits.device(),
+              "bergson_b200: distill_bwd: stats [T, 2] and dloss [T] in fp32 expected");
+  // The gradient has the logits' row pitch, so that both have the same alignment.
+  auto wide = at::empty({logits.size(0), logits.stride(0)}, logits.options());
+  auto dlogits = wide.narrow(1, 0, logits.size(1));
+  ran(bgn_distill_bwd(&a, stats.data_ptr<float>(), dloss.data_ptr<float>(), dlogits.data_ptr(), wide.size(1), current()),
+      "distill_bwd");
+  return dlogits;
+}
+
+}  // namespace
+
+void bgn_register_packed(pybind11::module& m) {
+  m.def("packed_attention_fwd", &packed_attention_fwd);
+  m.def("packed_attention_bwd", &packed_attention_bwd);
+  m.def("packed_rotary", &packed_rotary);
+  m.def("distill_fwd", &distill_fwd);
+  m.def("distill_bwd", &distill_bwd);
+}

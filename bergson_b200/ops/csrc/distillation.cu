@@ -1,0 +1,318 @@
+// Distillation from a teacher's top logits: loss and gradient over [tokens, vocab] student logits.
+//
+//   p = softmax(t / tau) over the row's entries,  q = softmax(z / tau) over the vocabulary
+//   loss = tau^2 sum_k p_k (log p_k - log q[id_k]),   dz_v = g tau (q_v - sum_{k: id_k = v} p_k)
+//
+// With w_k = e^{(t_k - t_max) / tau}, W = sum w, m the maximum and s the sum of e^{(z - m) / tau}:
+//   loss = tau^2 ( sum_k w_k ((t_k - t_max) - (z[id_k] - m)) / tau / W - log W + log s ),
+// so one sweep over the row with a running maximum and sum is enough, and the large parts cancel
+// before anything is rounded.  Exponents are taken to base 2.  HBM bounds both directions: the
+// forward reads the logits once, the backward reads them once and writes the gradient once.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+#include "kernels_distill.h"
+
+namespace bgn {
+
+namespace cg = cooperative_groups;
+
+constexpr int kDistillThreads = 512;
+constexpr int kDistillWarps = kDistillThreads / 32;
+constexpr float kDistillLog2e = 1.4426950408889634f;
+constexpr float kDistillLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float load_code(const void* p, long i, int type) {
+  if (type == 2) return static_cast<const float*>(p)[i];
+  if (type == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+
+// Entry i of the teacher: its id, and -1 where there is none (an id outside the vocabulary, or a
+// logit of -inf, which has no probability).
+__device__ __forceinline__ int load_entry(const BgnDistill& a, long i, float* t) {
+  const long id = a.ids_64 ? static_cast<const long*>(a.ids)[i] : long(static_cast<const int*>(a.ids)[i]);
+  *t = load_code(a.teacher, i, a.teacher_type);
+  return id >= 0 && id < a.vocab && *t != -INFINITY ? int(id) : -1;
+}
+
+// Reductions over the block, in the order of the warps; every thread gets the result.
+template <int N, bool MAX>
+__device__ __forceinline__ void block_reduce(float (&v)[N], float* red) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    v[n] = MAX ? warp_max(v[n]) : warp_sum(v[n]);
+    if (lane == 0) red[n * kDistillWarps + warp] = v[n];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    float r = red[n * kDistillWarps];
+#pragma unroll
+    for (int w = 1; w < kDistillWarps; ++w) r = MAX ? fmaxf(r, red[n * kDistillWarps + w]) : r + red[n * kDistillWarps + w];
+    v[n] = r;
+  }
+  __syncthreads();
+}
+
+template <typename T>
+struct alignas(16) DistillPacket {
+  static constexpr int N = 16 / int(sizeof(T));
+  T v[N];
+};
+
+// Elements in front of the first 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ int lead_of(const T* p, int n) {
+  const int lead = int(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T));
+  return lead < n ? lead : n;
+}
+
+// A cluster of blocks shares one row: block r of it sweeps the r-th part of the columns, the first
+// block joins the parts in rank order.
+template <typename T>
+__global__ void __launch_bounds__(kDistillThreads) distill_fwd_kernel(BgnDistill a, float* loss, float* stats) {
+  constexpr int V = DistillPacket<T>::N;
+  __shared__ float red[3 * kDistillWarps];
+  __shared__ float part[2];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int parts = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+  const long row = blockIdx.x / parts;
+  const T* z = static_cast<const T*>(a.logits) + row * a.pitch;
+  const float c = kDistillLog2e / a.temperature;
+
+  const int per = ((a.vocab + parts - 1) / parts + V - 1) / V * V;
+  const int begin = min(rank * per, a.vocab), n = min(begin + per, a.vocab) - begin;
+  const T* x = z + begin;
+  float m = -INFINITY, s = 0.f;
+  // The difference to the maximum is taken before the factor, which could overflow a type's lowest value.
+  const auto one = [&](float v) {
+    if (v > m) {
+      s *= exp2f((m - v) * c);
+      m = v;
+    }
+    // an entry of -inf adds nothing, and there may be no finite maximum yet
+    if (v != -INFINITY) s += exp2f((v - m) * c);
+  };
+  const int lead = lead_of(x, n), packets = (n - lead) / V;
+  if (int(threadIdx.x) < lead) one(to_float<T>(x[threadIdx.x]));
+  const DistillPacket<T>* xp = reinterpret_cast<const DistillPacket<T>*>(x + lead);
+  constexpr int U = 4;  // packets in flight for a thread
+  for (int i = threadIdx.x; i < packets; i += kDistillThreads * U) {
+    DistillPacket<T> p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * kDistillThreads < packets) p[u] = xp[i + u * kDistillThreads];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u * kDistillThreads >= packets) break;
+      float f[V], mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        f[e] = to_float<T>(p[u].v[e]);
+        mx = fmaxf(mx, f[e]);
+      }
+      if (mx > m) {
+        s *= exp2f((m - mx) * c);
+        m = mx;
+      }
+      if (mx != -INFINITY) {
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum += exp2f((f[e] - m) * c);
+        s += sum;
+      }
+    }
+  }
+  for (int i = lead + packets * V + threadIdx.x; i < n; i += kDistillThreads) one(to_float<T>(x[i]));
+
+  // Teacher entries of the row: only the first block needs them.
+  const long k0 = row * a.top;
+  float t_max = -INFINITY;
+  if (rank == 0)
+    for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
+      float t;
+      if (load_entry(a, k0 + k, &t) >= 0) t_max = fmaxf(t_max, t);
+    }
+  float mx[2] = {m, t_max};
+  block_reduce<2, true>(mx, red);
+  float sums[1] = {m == -INFINITY ? s : s * exp2f((m - mx[0]) * c)};
+  block_reduce<1, false>(sums, red);
+  float row_m = mx[0], row_s = sums[0];
+  if (parts > 1) {
+    if (threadIdx.x == 0) {
+      part[0] = row_m;
+      part[1] = row_s;
+    }
+    cluster.sync();
+    if (rank == 0) {
+      for (int r = 1; r < parts; ++r) row_m = fmaxf(row_m, *cluster.map_shared_rank(&part[0], r));
+      row_s = 0.f;
+      for (int r = 0; r < parts; ++r) {
+        const float pm = *cluster.map_shared_rank(&part[0], r), ps = *cluster.map_shared_rank(&part[1], r);
+        row_s += pm == -INFINITY ? ps : ps * exp2f((pm - row_m) * c);
+      }
+    }
+    cluster.sync();  // the parts stay until they are read
+    if (rank != 0) return;
+  }
+  float w_sum[2] = {0.f, 0.f};  // W, sum of w (log2 w - log2 of the student's unnormalised value)
+  int any = 0;
+  for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
+    float t;
+    const int id = load_entry(a, k0 + k, &t);
+    if (id < 0) continue;
+    any = 1;
+    t = (t - mx[1]) * c;
+    const float w = exp2f(t);
+    w_sum[0] += w;
+    if (w != 0.f) w_sum[1] += w * (t - (to_float<T>(z[id]) - row_m) * c);
+  }
+  any = __syncthreads_or(any);
+  block_reduce<2, false>(w_sum, red);
+  if (threadIdx.x == 0) {
+    const float l2 = log2f(row_s);
+    stats[2 * row] = row_m;
+    stats[2 * row + 1] = l2;
+    loss[row] = any ? a.temperature * a.temperature * kDistillLn2 * (w_sum[1] / w_sum[0] - log2f(w_sum[0]) + l2) : 0.f;
+  }
+}
+
+// grid (parts, tokens): a block rewrites one part of a row's columns and puts its teacher entries right
+// afterwards, each from the logit itself, so that every value is rounded once.
+template <typename T>
+__global__ void __launch_bounds__(kDistillThreads)
+distill_bwd_kernel(BgnDistill a, const float* stats, const float* dloss, T* dlogits, long d_pitch, int parts) {
+  constexpr int V = DistillPacket<T>::N;
+  __shared__ float red[kDistillWarps];
+  __shared__ float p_of[kDistillMaxTop];
+  __shared__ int id_of[kDistillMaxTop];
+  const long row = blockIdx.x / parts;
+  const int rank = int(blockIdx.x % parts);
+  const float c = kDistillLog2e / a.temperature;
+  const long k0 = row * a.top;
+
+  float t_max[1] = {-INFINITY};
+  int any = 0;
+  for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
+    id_of[k] = load_entry(a, k0 + k, &p_of[k]);
+    if (id_of[k] >= 0) {
+      any = 1;
+      t_max[0] = fmaxf(t_max[0], p_of[k]);
+    }
+  }
+  any = __syncthreads_or(any);
+  block_reduce<1, true>(t_max, red);
+  float w_sum[1] = {0.f};
+  for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
+    p_of[k] = id_of[k] >= 0 ? exp2f((p_of[k] - t_max[0]) * c) : 0.f;
+    w_sum[0] += p_of[k];
+  }
+  block_reduce<1, false>(w_sum, red);
+  const float inv_w = any ? 1.f / w_sum[0] : 0.f;
+  const float g = any ? dloss[row] * a.temperature : 0.f;
+  const float m = stats[2 * row], l2 = stats[2 * row + 1];
+  const T* z = static_cast<const T*>(a.logits) + row * a.pitch;
+  T* dz = dlogits + row * d_pitch;
+
+  const int per = ((a.vocab + parts - 1) / parts + V - 1) / V * V;
+  const int begin = min(rank * per, a.vocab), n = min(begin + per, a.vocab) - begin;
+  const T* x = z + begin;
+  T* y = dz + begin;
+  const auto value = [&](float v) { return g == 0.f ? 0.f : g * exp2f((v - m) * c - l2); };
+  const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0;
+  const int lead = same ? lead_of(x, n) : n, packets = (n - lead) / V;
+  for (int i = threadIdx.x; i < lead; i += kDistillThreads) y[i] = from_float<T>(value(to_float<T>(x[i])));
+  const DistillPacket<T>* xp = reinterpret_cast<const DistillPacket<T>*>(x + lead);
+  DistillPacket<T>* yp = reinterpret_cast<DistillPacket<T>*>(y + lead);
+  constexpr int U = 4;
+  for (int i = threadIdx.x; i < packets; i += kDistillThreads * U) {
+    DistillPacket<T> p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * kDistillThreads < packets) p[u] = xp[i + u * kDistillThreads];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u * kDistillThreads >= packets) break;
+#pragma unroll
+      for (int e = 0; e < V; ++e) p[u].v[e] = from_float<T>(value(to_float<T>(p[u].v[e])));
+      yp[i + u * kDistillThreads] = p[u];
+    }
+  }
+  for (int i = lead + packets * V + threadIdx.x; i < n; i += kDistillThreads) y[i] = from_float<T>(value(to_float<T>(x[i])));
+  __syncthreads();
+  // The teacher's entries: the first of equal ids takes the sum of all of them, in their order.
+  for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
+    const int id = id_of[k];
+    if (id < begin || id >= begin + n) continue;
+    bool first = true;
+    float p = 0.f;
+    for (int j = 0; j < a.top; ++j) {
+      if (id_of[j] != id) continue;
+      if (j < k) {
+        first = false;
+        break;
+      }
+      p += p_of[j];
+    }
+    if (first) dz[id] = from_float<T>(g == 0.f ? 0.f : g * (exp2f((to_float<T>(z[id]) - m) * c - l2) - p * inv_w));
+  }
+}
+
+template <typename T>
+static cudaError_t launch_distill_fwd(const BgnDistill& a, float* loss, float* stats, int parts, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(a.tokens) * unsigned(parts));
+  cfg.blockDim = dim3(kDistillThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = unsigned(parts);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, distill_fwd_kernel<T>, a, loss, stats);
+}
+
+// Blocks to a row: with few rows a row is shared, so that some two blocks per SM are at work, as
+// long as each has at least four packets a thread.
+static int row_parts(const BgnDistill& a, int most) {
+  const int per_block = kDistillThreads * 4 * (a.type == 2 ? 4 : 8);
+  int parts = 1;
+  while (parts < most && a.tokens * parts < 2 * 148 && a.vocab / (2 * parts) >= per_block) parts *= 2;
+  return parts;
+}
+
+static bool distill_sound(const BgnDistill* a) {
+  return a->tokens > 0 && a->tokens < (1l << 27) && a->vocab > 0 && a->top > 0 && a->top <= kDistillMaxTop &&
+         a->pitch >= a->vocab && a->temperature > 0.f && a->type >= 0 && a->type <= 2 && a->teacher_type >= 0 &&
+         a->teacher_type <= 2;
+}
+
+}  // namespace bgn
+
+using namespace bgn;
+
+extern "C" int bgn_distill_fwd(const BgnDistill* a, float* loss, float* stats, cudaStream_t stream) {
+  if (!distill_sound(a)) return int(cudaErrorInvalidValue);
+  const int parts = row_parts(*a, 8);
+  if (a->type == 2) return int(launch_distill_fwd<float>(*a, loss, stats, parts, stream));
+  if (a->type == 1) return int(launch_distill_fwd<__nv_bfloat16>(*a, loss, stats, parts, stream));
+  return int(launch_distill_fwd<__half>(*a, loss, stats, parts, stream));
+}
+
+extern "C" int bgn_distill_bwd(const BgnDistill* a, const float* stats, const float* dloss, void* dlogits, long d_pitch,
+                               cudaStream_t stream) {
+  if (!distill_sound(a) || d_pitch < a->vocab) return int(cudaErrorInvalidValue);
+  const int parts = row_parts(*a, 16);
+  const unsigned grid = unsigned(a->tokens) * unsigned(parts);
+  if (a->type == 2)
+    distill_bwd_kernel<float><<<grid, kDistillThreads, 0, stream>>>(*a, stats, dloss, static_cast<float*>(dlogits), d_pitch, parts);
+  else if (a->type == 1)
+    distill_bwd_kernel<__nv_bfloat16><<<grid, kDistillThreads, 0, stream>>>(
+        *a, stats, dloss, static_cast<__nv_bfloat16*>(dlogits), d_pitch, parts);
+  else
+    distill_bwd_kernel<__half><<<grid, kDistillThreads, 0, stream>>>(*a, stats, dloss, static_cast<__half*>(dlogits), d_pitch, parts);
+  return int(cudaGetLastError());
+}

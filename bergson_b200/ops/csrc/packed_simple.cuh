@@ -1,0 +1,348 @@
+// Causal attention over packed documents on the FMA units: forward and backward for every type.
+//
+// Token t attends the keys first_key[t] .. t.  Tiles are cut from the packed token axis without
+// regard to documents: a tile of 64 queries visits the keys from its first row's first key to its
+// last row, and a per-row range masks the rest, so short documents share tiles.
+//
+//   S = scale q k^T, P = softmax(S), O = P v                         (one pass, running max and sum)
+//   delta_t = do_t . o_t,  dS = P (do v^T - delta)
+//   dQ = scale dS k,  dK = scale dS^T q (summed over the heads of a group),  dV = P^T do
+//
+// The scaled score is rounded on its own in both directions, so that a row with one key has P = 1 exactly.
+// dQ and dK/dV are two kernels that recompute P from the stored log-sum-exp: sums stay in one block
+// and one order, so results do not depend on scheduling.
+#pragma once
+
+#include "common.cuh"
+#include "kernels_packed.h"
+
+namespace bgn {
+
+constexpr int kSimpleTile = 64;              // queries and keys of a tile
+constexpr int kSimplePitch = kSimpleTile + 4;  // floats between the rows of a tile in shared memory
+constexpr int kSimpleThreads = 256;          // 16 x 16 threads, 4 x 4 scores each
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Tile of `kSimpleTile` tokens in shared memory as [feature][token]; rows at or past `limit` and
+// features at or past `dim` are zero.
+template <typename T, int DP>
+__device__ __forceinline__ void simple_load(float* dst, const T* src, long tok_stride, int t0, int limit, int dim) {
+  constexpr int V = 16 / int(sizeof(T));
+  // One packet per step; neighbouring threads take neighbouring tokens, so the transposed stores
+  // fall into different banks.
+  for (int i = threadIdx.x; i < kSimpleTile * (DP / V); i += kSimpleThreads) {
+    const int tok = i % kSimpleTile, d = (i / kSimpleTile) * V;
+    union { uint4 u; T h[V]; } p;
+    p.u = make_uint4(0, 0, 0, 0);
+    if (t0 + tok < limit && d < dim) p.u = *reinterpret_cast<const uint4*>(src + long(t0 + tok) * tok_stride + d);
+#pragma unroll
+    for (int e = 0; e < V; ++e) dst[(d + e) * kSimplePitch + tok] = to_float<T>(p.h[e]);
+  }
+}
+
+// acc[i][j] += sum_d a[d][4 ty + i] b[d][4 tx + j]
+template <int DP>
+__device__ __forceinline__ void simple_scores(float (&acc)[4][4], const float* a, const float* b, int ty, int tx) {
+#pragma unroll 8
+  for (int d = 0; d < DP; ++d) {
+    const float4 x = *reinterpret_cast<const float4*>(a + d * kSimplePitch + 4 * ty);
+    const float4 y = *reinterpret_cast<const float4*>(b + d * kSimplePitch + 4 * tx);
+    const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[i], ys[j], acc[i][j]);
+  }
+}
+
+// out[i][c] += sum_j p[4 ty + i][j] x[tx + 16 c][j].  In a tile with masked scores (exact zeros of p) a
+// zero takes no part at all: what stands in a masked row may be infinite or NaN.
+template <int DP>
+__device__ __forceinline__ void simple_product(float (&out)[4][DP / 16], const float* p, const float* x, int ty, int tx,
+                                               bool masked) {
+  if (!masked) {
+#pragma unroll 4
+    for (int j = 0; j < kSimpleTile; j += 4) {
+      float4 a[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(p + (4 * ty + i) * kSimplePitch + j);
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) {
+        const float4 b = *reinterpret_cast<const float4*>(x + (tx + 16 * c) * kSimplePitch + j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          out[i][c] = fmaf(a[i].x, b.x, fmaf(a[i].y, b.y, fmaf(a[i].z, b.z, fmaf(a[i].w, b.w, out[i][c]))));
+      }
+    }
+  } else {
+    for (int j = 0; j < kSimpleTile; ++j) {
+      float a[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = p[(4 * ty + i) * kSimplePitch + j];
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) {
+        const float b = x[(tx + 16 * c) * kSimplePitch + j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (a[i] != 0.f) out[i][c] = fmaf(a[i], b, out[i][c]);
+      }
+    }
+  }
+}
+
+// Sum / maximum over the 16 threads that share a row group (half a warp).
+__device__ __forceinline__ float half_warp_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float half_warp_max(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPackedAttention a, T* o, float* lse2) {
+  extern __shared__ float smem[];
+  float* qs = smem;
+  float* ks = qs + DP * kSimplePitch;
+  float* vs = ks + DP * kSimplePitch;
+  float* ps = vs + DP * kSimplePitch;  // [query][key]
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  const int head = blockIdx.x % a.heads, slot = blockIdx.x / a.heads;
+  const int kv_head = head / (a.heads / a.kv_heads);
+  const int q0 = (a.query_order[slot / 2] * 2 + (slot & 1)) * kSimpleTile;
+  if (q0 >= a.rows) return;
+  const float c = a.scale * kLog2e;
+
+  simple_load<T, DP>(qs, static_cast<const T*>(a.q) + long(head) * a.q_head, a.q_tok, q0, a.valid, a.dim);
+  int first[4];
+  float m[4], l[4], out[4][DP / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = q0 + 4 * ty + i;
+    first[i] = row < a.valid ? a.first_key[row] : 0x7fffffff;
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) out[i][d] = 0.f;
+  }
+  const int q1 = min(q0 + kSimpleTile, a.valid);
+  const int last_first = q1 > q0 ? a.first_key[q1 - 1] : 0;
+  for (int k0 = q1 > q0 ? a.first_key[q0] : q1; k0 < q1; k0 += kSimpleTile) {
+    const bool masked = k0 + kSimpleTile - 1 > q0 || k0 < last_first;
+    __syncthreads();
+    simple_load<T, DP>(ks, static_cast<const T*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
+    simple_load<T, DP>(vs, static_cast<const T*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
+    __syncthreads();
+    float s[4][4] = {};
+    simple_scores<DP>(s, qs, ks, ty, tx);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = q0 + 4 * ty + i;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = k0 + 4 * tx + j;
+        s[i][j] = (key >= first[i] && key <= row) ? s[i][j] * c : -INFINITY;
+        mx = fmaxf(mx, s[i][j]);
+      }
+      mx = fmaxf(half_warp_max(mx), m[i]);
+      const float base = mx == -INFINITY ? 0.f : mx;  // nothing attended yet
+      const float old = exp2f(m[i] - base);
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p = exp2f(s[i][j] - base);
+        ps[(4 * ty + i) * kSimplePitch + 4 * tx + j] = p;
+        sum += p;
+      }
+      l[i] = l[i] * old + half_warp_sum(sum);
+      m[i] = mx;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) out[i][d] *= old;
+    }
+    __syncthreads();
+    simple_product<DP>(out, ps, vs, ty, tx, masked);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = q0 + 4 * ty + i;
+    if (row >= a.rows) continue;
+    const bool some = row < a.valid && first[i] <= row;
+    const float inv = some ? 1.f / l[i] : 0.f;
+    if (tx == 0) lse2[long(head) * a.rows + row] = some ? m[i] + log2f(l[i]) : INFINITY;
+    T* dst = o + (long(row) * a.heads + head) * a.dim;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+      if (tx + 16 * d < a.dim) dst[tx + 16 * d] = from_float<T>(some ? out[i][d] * inv : 0.f);
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kSimpleThreads)
+packed_dq_simple_kernel(BgnPackedAttention a, const T* o, const float* lse2, const T* d_o, long do_tok, long do_head,
+                        float* delta, T* dq) {
+  extern __shared__ float smem[];
+  float* qs = smem;
+  float* gs = qs + DP * kSimplePitch;
+  float* ks = gs + DP * kSimplePitch;
+  float* vs = ks + DP * kSimplePitch;
+  float* ds = vs + DP * kSimplePitch;  // [query][key]
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  const int head = blockIdx.x % a.heads, slot = blockIdx.x / a.heads;
+  const int kv_head = head / (a.heads / a.kv_heads);
+  const int q0 = (a.query_order[slot / 2] * 2 + (slot & 1)) * kSimpleTile;
+  if (q0 >= a.rows) return;
+  const float c = a.scale * kLog2e;
+
+  simple_load<T, DP>(qs, static_cast<const T*>(a.q) + long(head) * a.q_head, a.q_tok, q0, a.valid, a.dim);
+  simple_load<T, DP>(gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
+  __syncthreads();
+  int first[4];
+  float lse[4], dl[4], out[4][DP / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = q0 + 4 * ty + i;
+    const bool in = row < a.valid;
+    first[i] = in ? a.first_key[row] : 0x7fffffff;
+    lse[i] = in ? lse2[long(head) * a.rows + row] : INFINITY;
+    float sum = 0.f;
+    if (in) {
+      const T* orow = o + (long(row) * a.heads + head) * a.dim;
+      for (int d = tx; d < a.dim; d += 16) sum = fmaf(to_float<T>(orow[d]), gs[d * kSimplePitch + 4 * ty + i], sum);
+    }
+    dl[i] = half_warp_sum(sum);
+    if (tx == 0 && row < a.rows) delta[long(head) * a.rows + row] = dl[i];
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) out[i][d] = 0.f;
+  }
+  const int q1 = min(q0 + kSimpleTile, a.valid);
+  const int last_first = q1 > q0 ? a.first_key[q1 - 1] : 0;
+  for (int k0 = q1 > q0 ? a.first_key[q0] : q1; k0 < q1; k0 += kSimpleTile) {
+    const bool masked = k0 + kSimpleTile - 1 > q0 || k0 < last_first;
+    __syncthreads();
+    simple_load<T, DP>(ks, static_cast<const T*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
+    simple_load<T, DP>(vs, static_cast<const T*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
+    __syncthreads();
+    float s[4][4] = {}, dp[4][4] = {};
+    simple_scores<DP>(s, qs, ks, ty, tx);
+    simple_scores<DP>(dp, gs, vs, ty, tx);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = q0 + 4 * ty + i;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = k0 + 4 * tx + j;
+        // A row with one key has P = 1 and no gradient through the softmax: exactly zero.
+        const bool in = key >= first[i] && key <= row && first[i] < row;
+        ds[(4 * ty + i) * kSimplePitch + 4 * tx + j] = in ? exp2f(__fmul_rn(s[i][j], c) - lse[i]) * (dp[i][j] - dl[i]) : 0.f;
+      }
+    }
+    __syncthreads();
+    simple_product<DP>(out, ds, ks, ty, tx, masked);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = q0 + 4 * ty + i;
+    if (row >= a.rows) continue;
+    T* dst = dq + (long(row) * a.heads + head) * a.dim;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+      if (tx + 16 * d < a.dim) dst[tx + 16 * d] = from_float<T>(out[i][d] * a.scale);
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kSimpleThreads)
+packed_dkv_simple_kernel(BgnPackedAttention a, const float* lse2, const T* d_o, long do_tok, long do_head,
+                         const float* delta, T* dk, T* dv) {
+  extern __shared__ float smem[];
+  float* ks = smem;
+  float* vs = ks + DP * kSimplePitch;
+  float* qs = vs + DP * kSimplePitch;
+  float* gs = qs + DP * kSimplePitch;
+  float* ps = gs + DP * kSimplePitch;  // [key][query]
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  const int kv_head = blockIdx.x % a.kv_heads, slot = blockIdx.x / a.kv_heads;
+  const int group = a.heads / a.kv_heads;
+  const int k0 = (a.key_order[slot / 2] * 2 + (slot & 1)) * kSimpleTile;
+  if (k0 >= a.rows) return;
+  const float c = a.scale * kLog2e;
+
+  simple_load<T, DP>(ks, static_cast<const T*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
+  simple_load<T, DP>(vs, static_cast<const T*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
+  int end[4], own_first[4];
+  float out_k[4][DP / 16], out_v[4][DP / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int key = k0 + 4 * ty + i;
+    end[i] = key < a.valid ? a.end_query[key] : 0;
+    own_first[i] = key < a.valid ? a.first_key[key] : 0;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) out_k[i][d] = out_v[i][d] = 0.f;
+  }
+  const int k1 = min(k0 + kSimpleTile, a.valid);
+  const int q_end = k1 > k0 ? min(a.end_query[k1 - 1], a.valid) : 0;
+  const int first_end = k1 > k0 ? a.end_query[k0] : 0;
+  for (int head = kv_head * group; head < (kv_head + 1) * group; ++head) {
+    for (int q0 = k0; q0 < q_end; q0 += kSimpleTile) {
+      const bool masked = q0 < k0 + kSimpleTile || q0 + kSimpleTile > first_end;
+      __syncthreads();
+      simple_load<T, DP>(qs, static_cast<const T*>(a.q) + long(head) * a.q_head, a.q_tok, q0, a.valid, a.dim);
+      simple_load<T, DP>(gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
+      __syncthreads();
+      float s[4][4] = {}, dp[4][4] = {};
+      simple_scores<DP>(s, ks, qs, ty, tx);
+      simple_scores<DP>(dp, vs, gs, ty, tx);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = q0 + 4 * tx + j;
+        const bool in_row = row < a.valid;
+        const float lse = in_row ? lse2[long(head) * a.rows + row] : INFINITY;
+        const float dl = in_row ? delta[long(head) * a.rows + row] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = k0 + 4 * ty + i;
+          const bool in = row >= key && row < end[i];
+          const float p = in ? exp2f(__fmul_rn(s[i][j], c) - lse) : 0.f;
+          s[i][j] = p;
+          dp[i][j] = in && own_first[i] < row ? p * (dp[i][j] - dl) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ps[(4 * ty + i) * kSimplePitch + 4 * tx + j] = s[i][j];
+      __syncthreads();
+      simple_product<DP>(out_v, ps, gs, ty, tx, masked);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ps[(4 * ty + i) * kSimplePitch + 4 * tx + j] = dp[i][j];
+      __syncthreads();
+      simple_product<DP>(out_k, ps, qs, ty, tx, masked);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int key = k0 + 4 * ty + i;
+    if (key >= a.rows) continue;
+    const long at = (long(key) * a.kv_heads + kv_head) * a.dim;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+      if (tx + 16 * d < a.dim) {
+        dk[at + tx + 16 * d] = from_float<T>(out_k[i][d] * a.scale);
+        dv[at + tx + 16 * d] = from_float<T>(out_v[i][d]);
+      }
+  }
+}
+
+template <int DP>
+constexpr int simple_smem(int tiles) {
+  return (tiles * DP + kSimpleTile) * kSimplePitch * int(sizeof(float));
+}
+
+}  // namespace bgn

@@ -214,9 +214,14 @@ def rotary_tables(seq_len: int, rot_dim: int, theta: float, device, dtype=torch.
 
 def rotary_ref(x: Tensor, cos: Tensor, sin: Tensor, rot_dim: int) -> Tensor:
     """x: [B, S, H, D]; rotate the first ``rot_dim`` features of each head."""
-    half = rot_dim // 2
     c = cos[None, : x.shape[1], None, :].to(x.dtype)
     s = sin[None, : x.shape[1], None, :].to(x.dtype)
+    return rotary_pairs(x, c, s, rot_dim)
+
+
+def rotary_pairs(x: Tensor, c: Tensor, s: Tensor, rot_dim: int) -> Tensor:
+    """Turn the pairs (i, i + rot_dim / 2) of the last dimension; ``c``, ``s`` broadcast against them."""
+    half = rot_dim // 2
     x1, x2, rest = x[..., :half], x[..., half:rot_dim], x[..., rot_dim:]
     return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s, rest], dim=-1)
 
@@ -412,24 +417,30 @@ def _causal_bias(S: int, dtype: torch.dtype, device) -> Tensor:
     return bias
 
 
+def causal_attention_ref(q: Tensor, k: Tensor, v: Tensor, scale: float) -> Tensor:
+    # Explicit softmax(QK^T)V: differentiable to any order on every backend.  Three passes
+    # over the [B, H, S, S] scores instead of six: the scale goes onto q, the causal mask
+    # is the additive input of the batched product, and the softmax reads and writes the
+    # tensors' own dtype (its arithmetic is fp32 inside the kernel for 16-bit inputs).
+    B, Hq, S, D = q.shape
+    Hkv = k.shape[1]
+    if Hkv != Hq:
+        rep = Hq // Hkv
+        k = k.repeat_interleave(rep, dim=1)
+        v = v.repeat_interleave(rep, dim=1)
+    bias = _causal_bias(S, q.dtype, q.device)
+    att = torch.baddbmm(bias, (q * scale).reshape(B * Hq, S, D), k.reshape(B * Hq, S, D).transpose(1, 2))
+    att = _softmax_last(att)
+    return torch.bmm(att, v.reshape(B * Hq, S, D)).view(B, Hq, S, D)
+
+
 def causal_attention(q: Tensor, k: Tensor, v: Tensor, scale: float | None = None) -> Tensor:
     """q: [B, Hq, S, D]; k, v: [B, Hkv, S, D] (Hq a multiple of Hkv). Causal."""
     B, Hq, S, D = q.shape
     Hkv = k.shape[1]
     scale = scale if scale is not None else 1.0 / math.sqrt(D)
     if _composable() or not q.is_cuda:
-        # Explicit softmax(QK^T)V: differentiable to any order on every backend.  Three passes
-        # over the [B, H, S, S] scores instead of six: the scale goes onto q, the causal mask
-        # is the additive input of the batched product, and the softmax reads and writes the
-        # tensors' own dtype (its arithmetic is fp32 inside the kernel for 16-bit inputs).
-        if Hkv != Hq:
-            rep = Hq // Hkv
-            k = k.repeat_interleave(rep, dim=1)
-            v = v.repeat_interleave(rep, dim=1)
-        bias = _causal_bias(S, q.dtype, q.device)
-        att = torch.baddbmm(bias, (q * scale).reshape(B * Hq, S, D), k.reshape(B * Hq, S, D).transpose(1, 2))
-        att = _softmax_last(att)
-        return torch.bmm(att, v.reshape(B * Hq, S, D)).view(B, Hq, S, D)
+        return causal_attention_ref(q, k, v, scale)
     return F.scaled_dot_product_attention(
         q, k, v, is_causal=True, scale=scale, enable_gqa=(Hkv != Hq)
     )
@@ -507,3 +518,83 @@ def token_cross_entropy(
     ):
         return _TokenCEFn.apply(logits, targets, ignore_index)
     return token_cross_entropy_ref(logits, targets, ignore_index, label_smoothing)
+
+
+# --------------------------------------------------------------------------- #
+# distillation from a teacher's top logits (per-token losses)
+# --------------------------------------------------------------------------- #
+
+_DISTILL_MAX_TOP = 1024
+
+
+def token_distillation_ref(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor, temperature: float) -> Tensor:
+    dtype = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    z = logits.to(dtype) / temperature
+    t = teacher_logits.to(dtype) / temperature
+    used = (teacher_ids >= 0) & (teacher_ids < logits.shape[1]) & (t != float("-inf"))
+    some = used.any(1, keepdim=True)
+    t = torch.where(used, t, float("-inf"))
+    log_p = torch.log_softmax(torch.where(some, t, torch.zeros_like(t)), dim=1)
+    p = log_p.exp()
+    log_q = torch.log_softmax(z, dim=1).gather(1, torch.where(used, teacher_ids, 0).long())
+    # Where an entry has no probability its term is zero whatever the student gives it.
+    term = torch.where(used & (p > 0), p * (log_p - log_q), torch.zeros_like(p))
+    return term.sum(1) * temperature**2
+
+
+class _TokenDistillationFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_ids, teacher_logits, temperature):
+        from . import native
+
+        teacher_ids, teacher_logits = teacher_ids.contiguous(), teacher_logits.contiguous()
+        loss, stats = native.distill_fwd(logits, teacher_ids, teacher_logits, temperature)
+        ctx.save_for_backward(logits, teacher_ids, teacher_logits, stats)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        from . import native
+
+        logits, ids, teacher, stats = ctx.saved_tensors
+        dloss = dloss.float().contiguous()
+        return native.distill_bwd(logits, ids, teacher, stats, dloss, ctx.temperature), None, None, None
+
+
+def token_distillation(
+    logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor, temperature: float = 1.0
+) -> Tensor:
+    """``[T, V]`` student logits and the teacher's ``[T, K]`` top logits with their ids -> ``[T]`` fp32
+    losses ``temperature^2 KL(p || q)``: p is the softmax of a row's teacher logits over its entries, q
+    the student's softmax over the vocabulary, both at ``temperature``.
+
+    An id outside ``[0, V)`` (by convention -1) or a teacher logit of -inf is no entry; a row without
+    entries gives 0 and a zero gradient; an id that occurs twice counts with both probabilities.  The
+    teacher gets no gradient.  fp64 logits and ``ops.composable()`` run on torch operations; the
+    kernels' backward cannot be differentiated again.
+    """
+    if logits.ndim != 2 or not logits.is_floating_point():
+        raise ValueError(f"token_distillation: logits [tokens, vocabulary] expected, got {tuple(logits.shape)}")
+    if teacher_ids.ndim != 2 or teacher_ids.shape != teacher_logits.shape or teacher_ids.shape[0] != logits.shape[0]:
+        raise ValueError(f"token_distillation: teacher ids {tuple(teacher_ids.shape)} and logits "
+                         f"{tuple(teacher_logits.shape)} for {logits.shape[0]} tokens")
+    if teacher_ids.dtype not in (torch.int64, torch.int32) or not teacher_logits.is_floating_point():
+        raise ValueError("token_distillation: teacher ids are int32 or int64, teacher logits floating point")
+    if not 1 <= teacher_ids.shape[1] <= _DISTILL_MAX_TOP:
+        raise ValueError(f"token_distillation: {teacher_ids.shape[1]} entries a token; 1 to {_DISTILL_MAX_TOP}")
+    if logits.shape[1] == 0:
+        raise ValueError("token_distillation: empty vocabulary")
+    if teacher_ids.device != logits.device or teacher_logits.device != logits.device:
+        raise ValueError("token_distillation: student and teacher on different devices")
+    if teacher_logits.requires_grad:
+        raise ValueError("token_distillation: the teacher gets no gradient; pass teacher_logits.detach()")
+    temperature = float(temperature)
+    if not (temperature > 0.0 and math.isfinite(temperature)):
+        raise ValueError(f"token_distillation: temperature must be positive, got {temperature}")
+    kernels = (torch.bfloat16, torch.float16, torch.float32)
+    if (logits.dtype in kernels and teacher_logits.dtype in kernels and logits.shape[0] > 0
+            and use_fused(logits, teacher_ids, teacher_logits)):
+        return _TokenDistillationFn.apply(logits, teacher_ids, teacher_logits, temperature)
+    return token_distillation_ref(logits, teacher_ids, teacher_logits, temperature)
