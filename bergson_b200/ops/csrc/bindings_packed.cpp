@@ -56,7 +56,8 @@ void check_index(const at::Tensor& x, int64_t n, const at::Tensor& like) {
 }
 
 BgnPackedAttention packed_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& first_key,
-                               const at::Tensor& end_query, const at::Tensor& query_order, const at::Tensor& key_order,
+                               const at::Tensor& end_query, const at::Tensor& query_order,
+                               const at::Tensor& query_pair_order, const at::Tensor& key_order,
                                int64_t valid, double scale) {
   const int64_t rows = q.size(0), tiles = (rows + 127) / 128;
   check_packed(q, k);
@@ -67,6 +68,7 @@ BgnPackedAttention packed_args(const at::Tensor& q, const at::Tensor& k, const a
   check_index(first_key, rows, q);
   check_index(end_query, rows, q);
   check_index(query_order, tiles, q);
+  check_index(query_pair_order, (rows + 255) / 256, q);
   check_index(key_order, tiles, q);
   BgnPackedAttention a = {};
   a.q = q.data_ptr();
@@ -78,6 +80,7 @@ BgnPackedAttention packed_args(const at::Tensor& q, const at::Tensor& k, const a
   a.first_key = first_key.data_ptr<int>();
   a.end_query = end_query.data_ptr<int>();
   a.query_order = query_order.data_ptr<int>();
+  a.query_pair_order = query_pair_order.data_ptr<int>();
   a.key_order = key_order.data_ptr<int>();
   a.rows = int(rows);
   a.valid = int(valid);
@@ -90,14 +93,14 @@ BgnPackedAttention packed_args(const at::Tensor& q, const at::Tensor& k, const a
 }
 
 std::vector<at::Tensor> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor first_key,
-                                             at::Tensor end_query, at::Tensor query_order, at::Tensor key_order,
+                                             at::Tensor end_query, at::Tensor query_order, at::Tensor query_pair_order, at::Tensor key_order,
                                              int64_t valid, double scale) {
   c10::cuda::CUDAGuard guard(q.device());
   check_packed(q, k);
   q = readable(q);
   k = readable(k);
   v = readable(v);
-  const auto a = packed_args(q, k, v, first_key, end_query, query_order, key_order, valid, scale);
+  const auto a = packed_args(q, k, v, first_key, end_query, query_order, query_pair_order, key_order, valid, scale);
   auto o = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
   auto lse2 = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
   ran(bgn_packed_attention_fwd(&a, o.data_ptr(), lse2.data_ptr<float>(), bgn_status_word(q), current()),
@@ -107,7 +110,7 @@ std::vector<at::Tensor> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Ten
 
 std::vector<at::Tensor> packed_attention_bwd(at::Tensor d_o, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
                                              at::Tensor lse2, at::Tensor first_key, at::Tensor end_query,
-                                             at::Tensor query_order, at::Tensor key_order, int64_t valid, double scale) {
+                                             at::Tensor query_order, at::Tensor query_pair_order, at::Tensor key_order, int64_t valid, double scale) {
   c10::cuda::CUDAGuard guard(q.device());
   check_packed(q, k);
   q = readable(q);
@@ -118,7 +121,7 @@ std::vector<at::Tensor> packed_attention_bwd(at::Tensor d_o, at::Tensor q, at::T
                   lse2.scalar_type() == at::kFloat && lse2.is_contiguous() && lse2.numel() == q.size(0) * q.size(1),
               "bergson_b200: the output's gradient does not fit the operands");
   d_o = readable(d_o);
-  const auto a = packed_args(q, k, v, first_key, end_query, query_order, key_order, valid, scale);
+  const auto a = packed_args(q, k, v, first_key, end_query, query_order, query_pair_order, key_order, valid, scale);
   auto delta = at::empty_like(lse2);
   auto dq = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
   auto dk = at::empty({k.size(0), k.size(1), k.size(2)}, k.options());

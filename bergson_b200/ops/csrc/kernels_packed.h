@@ -16,6 +16,7 @@ typedef struct {
   const int* first_key;    // [rows]: first key that row t attends (its document's first token); t + 1: none
   const int* end_query;    // [rows]: one past the last row that attends key j; j: none
   const int* query_order;  // [ceil(rows / 128)]: query tiles of 128 rows, most keys first
+  const int* query_pair_order;  // [ceil(rows / 256)]: pairs of neighbouring query tiles, most keys first
   const int* key_order;    // [ceil(rows / 128)]: key tiles of 128 rows, most queries first
   int rows;                // rows of the tensors
   int valid;               // rows that belong to documents; the ones behind give zeros

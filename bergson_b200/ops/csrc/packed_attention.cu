@@ -1,4 +1,7 @@
 // Host side of the attention over packed documents.
+#include <mutex>
+
+#include "packed_fwd.cuh"
 #include "packed_simple.cuh"
 
 using namespace bgn;
@@ -42,6 +45,78 @@ cudaError_t simple_bwd(const BgnPackedAttention& a, const void* o, const float* 
   return cudaGetLastError();
 }
 
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  });
+  return fn;
+}
+
+// [tokens, heads, dim] in boxes of 128 tokens x 64 features of one head.  Rows behind the last document
+// and features past dim are outside the map and read as zeros, whatever stands there.
+bool operand_map(CUtensorMap* map, const void* base, int fmt, int dim, int heads, int valid, long head, long tok) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc || (reinterpret_cast<uintptr_t>(base) & 15) || head % 8 || tok % 8) return false;
+  cuuint64_t dims[3] = {cuuint64_t(dim), cuuint64_t(heads), cuuint64_t(valid > 0 ? valid : 1)};
+  cuuint64_t strides[2] = {cuuint64_t(head) * 2, cuuint64_t(tok) * 2};
+  cuuint32_t box[3] = {64, 1, cuuint32_t(kTile)};
+  cuuint32_t one[3] = {1, 1, 1};
+  return enc(map, fmt == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+             const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int FMT, int DP>
+cudaError_t tensor_fwd(const BgnPackedAttention& a, void* o, float* lse2, int* status, cudaStream_t stream) {
+  ensure_context_bound();
+  CUtensorMap mq, mk, mv;
+  if (!operand_map(&mq, a.q, FMT, a.dim, a.heads, a.valid, a.q_head, a.q_tok) ||
+      !operand_map(&mk, a.k, FMT, a.dim, a.kv_heads, a.valid, a.k_head, a.k_tok) ||
+      !operand_map(&mv, a.v, FMT, a.dim, a.kv_heads, a.valid, a.v_head, a.v_tok))
+    return cudaErrorInvalidValue;
+  PackedFwdArgs p = {};
+  // Two heads of a group always see the same keys; two row tiles of a head do not.
+  p.head_pairs = (a.heads / a.kv_heads) % 2 == 0;
+  p.first_key = a.first_key;
+  p.order = p.head_pairs ? a.query_order : a.query_pair_order;
+  p.rows = a.rows;
+  p.valid = a.valid;
+  p.heads = a.heads;
+  p.kv_heads = a.kv_heads;
+  p.dim = a.dim;
+  p.scale = a.scale;
+  p.q = a.q;
+  p.k = a.k;
+  p.v = a.v;
+  p.q_tok = a.q_tok;
+  p.q_head = a.q_head;
+  p.k_tok = a.k_tok;
+  p.k_head = a.k_head;
+  p.v_tok = a.v_tok;
+  p.v_head = a.v_head;
+  p.o = o;
+  p.lse2 = lse2;
+  constexpr int smem = fwd_smem_bytes<DP>();
+  auto kern = packed_fwd_kernel<FMT, DP>;
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem);
+  if (e != cudaSuccess) return e;
+  const unsigned tiles = unsigned((a.rows + kTile - 1) / kTile);
+  const unsigned grid = p.head_pairs ? tiles * unsigned(a.heads / 2) : (tiles + 1) / 2 * unsigned(a.heads);
+  kern<<<grid, kFwdThreads, smem, stream>>>(mq, mk, mv, p, status);
+  return cudaGetLastError();
+}
+
 bool sound(const BgnPackedAttention* a) {
   return a->rows > 0 && a->valid >= 0 && a->valid <= a->rows && a->heads > 0 && a->kv_heads > 0 &&
          a->heads % a->kv_heads == 0 && a->dim >= 8 && a->dim <= 128 && a->dim % 8 == 0 && a->type >= 0 && a->type <= 2 &&
@@ -53,12 +128,11 @@ bool sound(const BgnPackedAttention* a) {
 extern "C" int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, float* lse2, int* status,
                                         cudaStream_t stream) {
   if (!sound(a)) return int(cudaErrorInvalidValue);
-  (void)status;
-  if (a->type == 2) return int(a->dim <= 64 ? simple_fwd<float, 64>(*a, o, lse2, stream) : simple_fwd<float, 128>(*a, o, lse2, stream));
+  const bool narrow = a->dim <= 64;
+  if (a->type == 2) return int(narrow ? simple_fwd<float, 64>(*a, o, lse2, stream) : simple_fwd<float, 128>(*a, o, lse2, stream));
   if (a->type == 1)
-    return int(a->dim <= 64 ? simple_fwd<__nv_bfloat16, 64>(*a, o, lse2, stream)
-                            : simple_fwd<__nv_bfloat16, 128>(*a, o, lse2, stream));
-  return int(a->dim <= 64 ? simple_fwd<__half, 64>(*a, o, lse2, stream) : simple_fwd<__half, 128>(*a, o, lse2, stream));
+    return int(narrow ? tensor_fwd<1, 64>(*a, o, lse2, status, stream) : tensor_fwd<1, 128>(*a, o, lse2, status, stream));
+  return int(narrow ? tensor_fwd<0, 64>(*a, o, lse2, status, stream) : tensor_fwd<0, 128>(*a, o, lse2, status, stream));
 }
 
 extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const float* lse2, const void* d_o,

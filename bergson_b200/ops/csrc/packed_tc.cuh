@@ -1,0 +1,179 @@
+// What the tensor-core kernels of the packed attention share: TMEM accesses, the MMA form that reads
+// its A operand from TMEM, operand maps, and the exact recomputation of a tile's rows.
+#pragma once
+
+#include "common.cuh"
+#include "kernels_packed.h"
+
+namespace bgn {
+
+constexpr int kTile = 128;                  // rows (queries or keys) of a tile
+constexpr float kPackedLog2e = 1.4426950408889634f;
+
+// Bytes of a [128 rows, DP features] operand tile: slabs of 64 features in the 128-byte swizzle.
+template <int DP>
+constexpr int tile_bytes() {
+  return kTile * DP * 2;
+}
+constexpr int kSlabBytes = kTile * 128;
+
+// D[tmem] (+)= A[tmem] * B[smem]: A has one row per lane, two 16-bit values of the reduction per column.
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}"
+      :
+      : "r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 32 lanes x 32 columns without waiting; tmem_ld_wait() makes the values of all loads before it usable.
+__device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Ties values to the place in the program: what reads them cannot be moved in front of it.
+__device__ __forceinline__ void pin_32(uint32_t (&r)[32]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+  asm volatile(""
+               : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+
+__device__ __forceinline__ void tmem_st_32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+      :
+      : "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two values rounded to the 16-bit type, the first in the low half.
+template <int FMT>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if (FMT == 1) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+template <int FMT>
+struct Type16;
+template <>
+struct Type16<0> { using T = __half; };
+template <>
+struct Type16<1> { using T = __nv_bfloat16; };
+
+// Whether one of two packed 16-bit values is infinite or NaN (all exponent bits set): adding the
+// exponent's lowest bit carries into the sign bit.
+template <int FMT>
+__device__ __forceinline__ bool not_finite2(uint32_t u) {
+  return FMT == 1 ? (((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0
+                  : (((u & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0;
+}
+
+// One warp's share of a look through `bytes` of an operand tile in shared memory.
+template <int FMT>
+__device__ __forceinline__ bool scan_not_finite(const uint8_t* tile, int bytes, int part, int parts, int lane) {
+  bool bad = false;
+  const uint4* p = reinterpret_cast<const uint4*>(tile);
+  for (int i = part * 32 + lane; i < bytes / 16; i += parts * 32) {
+    const uint4 u = p[i];
+    bad |= not_finite2<FMT>(u.x) || not_finite2<FMT>(u.y) || not_finite2<FMT>(u.z) || not_finite2<FMT>(u.w);
+  }
+  return bad;
+}
+
+// Features of a row that a lane holds when a warp works on whole rows.
+template <int FMT, int DP>
+__device__ __forceinline__ void load_row(float (&x)[DP / 32], const void* base, long offset, int dim, int lane) {
+  using T = typename Type16<FMT>::T;
+  const T* p = static_cast<const T*>(base) + offset;
+#pragma unroll
+  for (int e = 0; e < DP / 32; ++e) x[e] = lane + 32 * e < dim ? to_float<T>(p[lane + 32 * e]) : 0.f;
+}
+
+template <int N>
+__device__ __forceinline__ float warp_dot(const float (&x)[N], const float (&y)[N]) {
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) s = fmaf(x[e], y[e], s);
+  return warp_sum(s);
+}
+
+// Gives up after a wait that ran out: long enough for every copy in flight to land.
+__device__ __forceinline__ void drain_copies() {
+  const long long start = clock64();
+  while (clock64() - start < 400000) {
+  }
+}
+
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void store_v8(void* ptr, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(ptr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// A thread's row of an accumulator in TMEM, scaled, rounded and stored to `dst` (dim features,
+// 16-byte aligned).
+template <int FMT, int DP>
+__device__ __forceinline__ void store_row(uint32_t tmem, float scale, void* dst, int dim, bool write) {
+  const bool wide = (dim & 15) == 0;  // every row begins on a 32-byte boundary then
+#pragma unroll 1
+  for (int c = 0; c < DP; c += 32) {
+    if (c >= dim) break;
+    uint32_t r[32];
+    tmem_ld_32(tmem + c, r);
+    tmem_ld_wait();
+    pin_32(r);
+    if (write) {
+      uint32_t h[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        h[i] = pack16<FMT>(__uint_as_float(r[2 * i]) * scale, __uint_as_float(r[2 * i + 1]) * scale);
+      uint8_t* at = static_cast<uint8_t*>(dst) + c * 2;
+      if (wide) {
+        store_v8(at, h);
+        if (c + 16 < dim) store_v8(at + 32, h + 8);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (c + 8 * i < dim)
+            *reinterpret_cast<uint4*>(at + 16 * i) = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+      }
+    }
+    __syncwarp();
+  }
+}
+
+}  // namespace bgn

@@ -69,14 +69,20 @@ class PackedSequences:
         key_work = np.minimum(end_query[last], valid) - head if rows else head
         query_order = np.argsort(-query_work, kind="stable")
         key_order = np.argsort(-key_work, kind="stable")
-        parts = [first_key, end_query, position, query_order, key_order, np.concatenate([[0], ends])]
+        pair = np.maximum(np.append(query_work, -1)[1::2], query_work[::2])[: -(-len(head) // 2)]
+        query_pair_order = np.argsort(-pair, kind="stable")
+        parts = [first_key, end_query, position, query_order, query_pair_order, key_order, np.concatenate([[0], ends])]
         table = torch.from_numpy(np.concatenate(parts).astype(np.int32)).to(device)
         self.device = table.device
-        (self.first_key, self.end_query, self.position, self.query_order, self.key_order,
-         self.cu_seqlens) = table.split([len(p) for p in parts])
+        (self.first_key, self.end_query, self.position, self.query_order, self.query_pair_order,
+         self.key_order, self.cu_seqlens) = table.split([len(p) for p in parts])
 
     def __repr__(self) -> str:
         return f"PackedSequences({len(self.lengths)} documents, {self.num_tokens} tokens, {self.rows} rows)"
+
+    def tables(self):
+        """What the attention kernels read of the plan."""
+        return self.first_key, self.end_query, self.query_order, self.query_pair_order, self.key_order
 
     def spans(self):
         """(begin, end) of each document that has tokens."""
@@ -135,8 +141,7 @@ class _PackedAttentionFn(torch.autograd.Function):
         from . import native
 
         p = packing
-        o, lse2 = native.packed_attention_fwd(q, k, v, p.first_key, p.end_query, p.query_order, p.key_order,
-                                              p.num_tokens, scale)
+        o, lse2 = native.packed_attention_fwd(q, k, v, *p.tables(), p.num_tokens, scale)
         ctx.save_for_backward(q, k, v, o, lse2)
         ctx.packing, ctx.scale = packing, scale
         return o
@@ -148,8 +153,7 @@ class _PackedAttentionFn(torch.autograd.Function):
 
         q, k, v, o, lse2 = ctx.saved_tensors
         p = ctx.packing
-        dq, dk, dv = native.packed_attention_bwd(d_o, q, k, v, o, lse2, p.first_key, p.end_query, p.query_order,
-                                                 p.key_order, p.num_tokens, ctx.scale)
+        dq, dk, dv = native.packed_attention_bwd(d_o, q, k, v, o, lse2, *p.tables(), p.num_tokens, ctx.scale)
         return dq, dk, dv, None, None
 
 
