@@ -83,6 +83,7 @@ BgnPackedAttention packed_args(const at::Tensor& q, const at::Tensor& k, const a
   a.query_pair_order = query_pair_order.data_ptr<int>();
   a.key_order = key_order.data_ptr<int>();
   a.rows = int(rows);
+  a.pitch = int(128 * tiles);
   a.valid = int(valid);
   a.heads = int(q.size(1));
   a.kv_heads = int(k.size(1));
@@ -102,7 +103,7 @@ std::vector<at::Tensor> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Ten
   v = readable(v);
   const auto a = packed_args(q, k, v, first_key, end_query, query_order, query_pair_order, key_order, valid, scale);
   auto o = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
-  auto lse2 = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  auto lse2 = at::empty({q.size(1), a.pitch}, q.options().dtype(at::kFloat));
   ran(bgn_packed_attention_fwd(&a, o.data_ptr(), lse2.data_ptr<float>(), bgn_status_word(q), current()),
       "packed_attention_fwd");
   return {o, lse2};
@@ -118,17 +119,18 @@ std::vector<at::Tensor> packed_attention_bwd(at::Tensor d_o, at::Tensor q, at::T
   v = readable(v);
   TORCH_CHECK(d_o.sizes() == q.sizes() && d_o.scalar_type() == q.scalar_type() && d_o.device() == q.device() &&
                   o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.is_contiguous() &&
-                  lse2.scalar_type() == at::kFloat && lse2.is_contiguous() && lse2.numel() == q.size(0) * q.size(1),
+                  lse2.scalar_type() == at::kFloat && lse2.is_contiguous() && lse2.numel() == (q.size(0) + 127) / 128 * 128 * q.size(1),
               "bergson_b200: the output's gradient does not fit the operands");
   d_o = readable(d_o);
   const auto a = packed_args(q, k, v, first_key, end_query, query_order, query_pair_order, key_order, valid, scale);
   auto delta = at::empty_like(lse2);
+  auto do_max = at::empty({lse2.numel() / 32}, lse2.options());
   auto dq = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
   auto dk = at::empty({k.size(0), k.size(1), k.size(2)}, k.options());
   auto dv = at::empty_like(dk);
   const auto [tok, head] = strides_of(d_o);
   ran(bgn_packed_attention_bwd(&a, o.data_ptr(), lse2.data_ptr<float>(), d_o.data_ptr(), tok, head,
-                               delta.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                               delta.data_ptr<float>(), do_max.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                bgn_status_word(q), current()),
       "packed_attention_bwd");
   return {dq, dk, dv};

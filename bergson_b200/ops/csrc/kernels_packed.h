@@ -19,20 +19,21 @@ typedef struct {
   const int* query_pair_order;  // [ceil(rows / 256)]: pairs of neighbouring query tiles, most keys first
   const int* key_order;    // [ceil(rows / 128)]: key tiles of 128 rows, most queries first
   int rows;                // rows of the tensors
+  int pitch;               // rows rounded up to a multiple of 128: floats to a head of lse2 and delta
   int valid;               // rows that belong to documents; the ones behind give zeros
   int heads, kv_heads, dim;
   int type;                // 0 = fp16, 1 = bf16, 2 = fp32
   float scale;             // > 0
 } BgnPackedAttention;
 
-// o [rows, heads, dim] and lse2 [heads, rows] (base-2 logarithm of the softmax denominator of
-// scale * log2(e) * q.k; +inf where a row attends nothing), both contiguous.
+// o [rows, heads, dim] contiguous and lse2 [heads, pitch]: base-2 logarithm of the softmax denominator of
+// scale * log2(e) * q.k; +inf where a row attends nothing, unset from `rows` on.
 int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, float* lse2, int* status, cudaStream_t stream);
 
 // Gradients of the operands (contiguous) from the output's gradient d_o [rows, heads, dim] (strides in
-// elements), the forward's o and lse2.  delta [heads, rows] is scratch.
+// elements), the forward's o and lse2.  Scratch: delta [heads, pitch], do_max [heads, pitch / 32].
 int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const float* lse2, const void* d_o, long do_tok,
-                             long do_head, float* delta, void* dq, void* dk, void* dv, int* status,
+                             long do_head, float* delta, float* do_max, void* dq, void* dk, void* dv, int* status,
                              cudaStream_t stream);
 
 typedef struct {

@@ -1,6 +1,7 @@
 // Host side of the attention over packed documents.
 #include <mutex>
 
+#include "packed_bwd.cuh"
 #include "packed_fwd.cuh"
 #include "packed_simple.cuh"
 
@@ -92,6 +93,7 @@ cudaError_t tensor_fwd(const BgnPackedAttention& a, void* o, float* lse2, int* s
   p.order = p.head_pairs ? a.query_order : a.query_pair_order;
   p.rows = a.rows;
   p.valid = a.valid;
+  p.pitch = a.pitch;
   p.heads = a.heads;
   p.kv_heads = a.kv_heads;
   p.dim = a.dim;
@@ -117,8 +119,65 @@ cudaError_t tensor_fwd(const BgnPackedAttention& a, void* o, float* lse2, int* s
   return cudaGetLastError();
 }
 
+template <int FMT, int DP>
+cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const float* lse2, const void* d_o, long do_tok,
+                       long do_head, float* delta, float* do_max, void* dq, void* dk, void* dv, int* status,
+                       cudaStream_t stream) {
+  ensure_context_bound();
+  CUtensorMap mq, mk, mv, mg;
+  if (!operand_map(&mq, a.q, FMT, a.dim, a.heads, a.valid, a.q_head, a.q_tok) ||
+      !operand_map(&mk, a.k, FMT, a.dim, a.kv_heads, a.valid, a.k_head, a.k_tok) ||
+      !operand_map(&mv, a.v, FMT, a.dim, a.kv_heads, a.valid, a.v_head, a.v_tok) ||
+      !operand_map(&mg, d_o, FMT, a.dim, a.heads, a.valid, do_head, do_tok))
+    return cudaErrorInvalidValue;
+  PackedBwdArgs p = {};
+  p.first_key = a.first_key;
+  p.end_query = a.end_query;
+  p.rows = a.rows;
+  p.valid = a.valid;
+  p.heads = a.heads;
+  p.kv_heads = a.kv_heads;
+  p.dim = a.dim;
+  p.pitch = a.pitch;
+  p.scale = a.scale;
+  p.q = a.q;
+  p.k = a.k;
+  p.v = a.v;
+  p.o = o;
+  p.d_o = d_o;
+  p.q_tok = a.q_tok;
+  p.q_head = a.q_head;
+  p.k_tok = a.k_tok;
+  p.k_head = a.k_head;
+  p.v_tok = a.v_tok;
+  p.v_head = a.v_head;
+  p.do_tok = do_tok;
+  p.do_head = do_head;
+  p.lse2 = lse2;
+  p.delta = delta;
+  p.do_max = do_max;
+  p.dq = dq;
+  p.dk = dk;
+  p.dv = dv;
+  auto kq = packed_dq_kernel<FMT, DP>;
+  auto kk = packed_dkv_kernel<FMT, DP>;
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kq), dq_smem_bytes<DP>());
+  if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(kk), dkv_smem_bytes<DP>());
+  if (e != cudaSuccess) return e;
+  const unsigned tiles = unsigned((a.rows + kTile - 1) / kTile);
+  p.head_pairs = (a.heads / a.kv_heads) % 2 == 0;
+  p.order = p.head_pairs ? a.query_order : a.query_pair_order;
+  const unsigned grid = p.head_pairs ? tiles * unsigned(a.heads / 2) : (tiles + 1) / 2 * unsigned(a.heads);
+  kq<<<grid, kBwdThreads, dq_smem_bytes<DP>(), stream>>>(mq, mg, mk, mv, p, status);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  p.order = a.key_order;
+  kk<<<tiles * unsigned(a.kv_heads), kBwdThreads, dkv_smem_bytes<DP>(), stream>>>(mq, mg, mk, mv, p, status);
+  return cudaGetLastError();
+}
+
 bool sound(const BgnPackedAttention* a) {
-  return a->rows > 0 && a->valid >= 0 && a->valid <= a->rows && a->heads > 0 && a->kv_heads > 0 &&
+  return a->rows > 0 && a->pitch >= a->rows && a->pitch % kTile == 0 && a->valid >= 0 && a->valid <= a->rows && a->heads > 0 && a->kv_heads > 0 &&
          a->heads % a->kv_heads == 0 && a->dim >= 8 && a->dim <= 128 && a->dim % 8 == 0 && a->type >= 0 && a->type <= 2 &&
          a->scale > 0.f;
 }
@@ -136,15 +195,14 @@ extern "C" int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, fl
 }
 
 extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const float* lse2, const void* d_o,
-                                        long do_tok, long do_head, float* delta, void* dq, void* dk, void* dv,
-                                        int* status, cudaStream_t stream) {
+                                        long do_tok, long do_head, float* delta, float* do_max, void* dq, void* dk,
+                                        void* dv, int* status, cudaStream_t stream) {
   if (!sound(a)) return int(cudaErrorInvalidValue);
-  (void)status;
-#define SIMPLE(T) \
-  return int(a->dim <= 64 ? simple_bwd<T, 64>(*a, o, lse2, d_o, do_tok, do_head, delta, dq, dk, dv, stream) \
-                          : simple_bwd<T, 128>(*a, o, lse2, d_o, do_tok, do_head, delta, dq, dk, dv, stream))
-  if (a->type == 2) SIMPLE(float);
-  if (a->type == 1) SIMPLE(__nv_bfloat16);
-  SIMPLE(__half);
-#undef SIMPLE
+  const bool narrow = a->dim <= 64;
+  if (a->type == 2)
+    return int(narrow ? simple_bwd<float, 64>(*a, o, lse2, d_o, do_tok, do_head, delta, dq, dk, dv, stream)
+                      : simple_bwd<float, 128>(*a, o, lse2, d_o, do_tok, do_head, delta, dq, dk, dv, stream));
+  auto run = a->type == 1 ? (narrow ? tensor_bwd<1, 64> : tensor_bwd<1, 128>)
+                          : (narrow ? tensor_bwd<0, 64> : tensor_bwd<0, 128>);
+  return int(run(*a, o, lse2, d_o, do_tok, do_head, delta, do_max, dq, dk, dv, status, stream));
 }

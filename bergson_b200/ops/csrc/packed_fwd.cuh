@@ -39,6 +39,7 @@ struct PackedFwdArgs {
   const int* first_key;
   const int* order;  // tiles (head pairs) or pairs of tiles, most keys first
   int rows, valid, heads, kv_heads, dim;
+  int pitch;       // floats between the heads of lse2
   int head_pairs;  // 1: a block takes two heads of a group; 0: two row tiles of a head
   float scale;
   const void *q, *k, *v;  // for the exact recomputation
@@ -375,7 +376,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     tc_fence_after();
     const bool some = in && first <= row;
     const float lse2 = some ? fmaf(m, c, log2f(l)) : INFINITY;
-    if (row < p.rows) p.lse2[long(my_head) * p.rows + row] = lse2;
+    if (row < p.rows) p.lse2[long(my_head) * p.pitch + row] = lse2;
     using T = typename Type16<FMT>::T;
     T* dst = static_cast<T*>(p.o) + (long(row) * p.heads + my_head) * p.dim;
     const bool exact = *reinterpret_cast<volatile int*>(poison) != 0;

@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPa
     if (row >= a.rows) continue;
     const bool some = row < a.valid && first[i] <= row;
     const float inv = some ? 1.f / l[i] : 0.f;
-    if (tx == 0) lse2[long(head) * a.rows + row] = some ? m[i] + log2f(l[i]) : INFINITY;
+    if (tx == 0) lse2[long(head) * a.pitch + row] = some ? m[i] + log2f(l[i]) : INFINITY;
     T* dst = o + (long(row) * a.heads + head) * a.dim;
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
@@ -207,14 +207,14 @@ packed_dq_simple_kernel(BgnPackedAttention a, const T* o, const float* lse2, con
     const int row = q0 + 4 * ty + i;
     const bool in = row < a.valid;
     first[i] = in ? a.first_key[row] : 0x7fffffff;
-    lse[i] = in ? lse2[long(head) * a.rows + row] : INFINITY;
+    lse[i] = in ? lse2[long(head) * a.pitch + row] : INFINITY;
     float sum = 0.f;
     if (in) {
       const T* orow = o + (long(row) * a.heads + head) * a.dim;
       for (int d = tx; d < a.dim; d += 16) sum = fmaf(to_float<T>(orow[d]), gs[d * kSimplePitch + 4 * ty + i], sum);
     }
     dl[i] = half_warp_sum(sum);
-    if (tx == 0 && row < a.rows) delta[long(head) * a.rows + row] = dl[i];
+    if (tx == 0 && row < a.rows) delta[long(head) * a.pitch + row] = dl[i];
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) out[i][d] = 0.f;
   }
@@ -300,8 +300,8 @@ packed_dkv_simple_kernel(BgnPackedAttention a, const float* lse2, const T* d_o, 
       for (int j = 0; j < 4; ++j) {
         const int row = q0 + 4 * tx + j;
         const bool in_row = row < a.valid;
-        const float lse = in_row ? lse2[long(head) * a.rows + row] : INFINITY;
-        const float dl = in_row ? delta[long(head) * a.rows + row] : 0.f;
+        const float lse = in_row ? lse2[long(head) * a.pitch + row] : INFINITY;
+        const float dl = in_row ? delta[long(head) * a.pitch + row] : 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = k0 + 4 * ty + i;

@@ -14,6 +14,9 @@ def attention64(q, k, v, lens, scale=None, do=None):
       o:  (u + r) sum_j P |v| + u |o|
       delta = o . do is formed from the rounded o: its error is at most e = (2 u + r) sum_d |o| |do|, so
       dS: (u + r) |dS| + P (e + r' sum |do| |v|);  dq, dk: the sums of that against |k|, |q|, times scale; dv like o.
+    fp16 has a smallest step of 2^-24, so rounding is off by up to 2^-25 however small the value is. The kernels
+    round P times 2^10: 2^-35 of P. They round dS times a power of two f that brings the largest |do| of its rows to
+    [1/2, 1): with f >= 1 / (2 max |do|) that is 2^-25 / f <= 2^-24 max |do| of dS.
     r: the scores are fp32 sums of D products (D 2^-24 of the absolute sum), a sum over n keys adds n 2^-24,
     and the exponential and the final division a few more.
     """
@@ -23,6 +26,9 @@ def attention64(q, k, v, lens, scale=None, do=None):
     scale = 1.0 / math.sqrt(d) if scale is None else scale
     u = torch.finfo(q.dtype).eps / 2
     f = torch.finfo(torch.float32).eps / 2
+    step_p = step_ds = 0.0
+    if q.dtype == torch.float16 and do is not None:
+        step_p, step_ds = 2.0**-35, 2.0**-24 * do.abs().nan_to_num(0, 0, 0).max().item()
     names = ["o"] + (["dq", "dk", "dv"] if do is not None else [])
     shapes = {"o": q.shape, "dq": q.shape, "dk": k.shape, "dv": k.shape}
     out = {n: torch.zeros(shapes[n], dtype=torch.float64, device=q.device) for n in names}
@@ -52,10 +58,10 @@ def attention64(q, k, v, lens, scale=None, do=None):
         delta = (O * G).sum(-1, keepdim=True)
         dS = P * (dP - delta)
         e = (2 * u + r) * (A * G.abs()).sum(-1, keepdim=True) + (d + 8) * f * (G.abs() @ V.abs().mT)
-        eS = (u + r) * dS.abs() + P * e
+        eS = (u + r) * dS.abs() + P * e + (step_ds * ~hidden)
         dQ, eQ = scale * dS @ K, scale * eS @ K.abs()
         dK, eK = scale * dS.mT @ Q, scale * eS.mT @ Q.abs()
-        dV, eV = P.mT @ G, (u + r) * (P.mT @ G.abs())
+        dV, eV = P.mT @ G, ((u + r) * P + step_p * ~hidden).mT @ G.abs()
         s = (n * group + 16) * f  # the sum over the rows and the heads of a group
         aQ, aK, aV = scale * dS.abs() @ K.abs(), scale * dS.abs().mT @ Q.abs(), P.mT @ G.abs()
         out["dq"][r_] = dQ.transpose(0, 1)
