@@ -56,8 +56,8 @@ void check_index(const at::Tensor& x, int64_t n, const at::Tensor& like) {
 }
 
 BgnPackedAttention packed_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& first_key,
-                               const at::Tensor& end_query, const at::Tensor& query_order,
-                               const at::Tensor& query_pair_order, const at::Tensor& key_order,
+                               const at::Tensor& end_query, const at::Tensor& query_tiles,
+                               const at::Tensor& query_pairs, const at::Tensor& key_tiles,
                                int64_t valid, double scale) {
   const int64_t rows = q.size(0), tiles = (rows + 127) / 128;
   check_packed(q, k);
@@ -67,9 +67,11 @@ BgnPackedAttention packed_args(const at::Tensor& q, const at::Tensor& k, const a
   TORCH_CHECK(2 * tiles * q.size(1) < (int64_t(1) << 31), "bergson_b200: too many tiles for one launch");
   check_index(first_key, rows, q);
   check_index(end_query, rows, q);
-  check_index(query_order, tiles, q);
-  check_index(query_pair_order, (rows + 255) / 256, q);
-  check_index(key_order, tiles, q);
+  check_index(query_tiles, 4 * tiles, q);
+  check_index(query_pairs, 8 * ((rows + 255) / 256), q);
+  check_index(key_tiles, 4 * tiles, q);
+  for (const auto* t : {&query_tiles, &query_pairs, &key_tiles})
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "bergson_b200: tile tables on 16-byte boundaries");
   BgnPackedAttention a = {};
   a.q = q.data_ptr();
   a.k = k.data_ptr();
@@ -79,9 +81,9 @@ BgnPackedAttention packed_args(const at::Tensor& q, const at::Tensor& k, const a
   std::tie(a.v_tok, a.v_head) = strides_of(v);
   a.first_key = first_key.data_ptr<int>();
   a.end_query = end_query.data_ptr<int>();
-  a.query_order = query_order.data_ptr<int>();
-  a.query_pair_order = query_pair_order.data_ptr<int>();
-  a.key_order = key_order.data_ptr<int>();
+  a.query_tiles = query_tiles.data_ptr<int>();
+  a.query_pairs = query_pairs.data_ptr<int>();
+  a.key_tiles = key_tiles.data_ptr<int>();
   a.rows = int(rows);
   a.pitch = int(128 * tiles);
   a.valid = int(valid);
@@ -94,24 +96,24 @@ BgnPackedAttention packed_args(const at::Tensor& q, const at::Tensor& k, const a
 }
 
 std::vector<at::Tensor> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor first_key,
-                                             at::Tensor end_query, at::Tensor query_order, at::Tensor query_pair_order, at::Tensor key_order,
+                                             at::Tensor end_query, at::Tensor query_tiles, at::Tensor query_pairs, at::Tensor key_tiles,
                                              int64_t valid, double scale) {
   c10::cuda::CUDAGuard guard(q.device());
   check_packed(q, k);
   q = readable(q);
   k = readable(k);
   v = readable(v);
-  const auto a = packed_args(q, k, v, first_key, end_query, query_order, query_pair_order, key_order, valid, scale);
+  const auto a = packed_args(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale);
   auto o = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
-  auto lse2 = at::empty({q.size(1), a.pitch}, q.options().dtype(at::kFloat));
-  ran(bgn_packed_attention_fwd(&a, o.data_ptr(), lse2.data_ptr<float>(), bgn_status_word(q), current()),
+  auto bias2 = at::empty({q.size(1), a.pitch}, q.options().dtype(at::kFloat));
+  ran(bgn_packed_attention_fwd(&a, o.data_ptr(), bias2.data_ptr<float>(), bgn_status_word(q), current()),
       "packed_attention_fwd");
-  return {o, lse2};
+  return {o, bias2};
 }
 
 std::vector<at::Tensor> packed_attention_bwd(at::Tensor d_o, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
-                                             at::Tensor lse2, at::Tensor first_key, at::Tensor end_query,
-                                             at::Tensor query_order, at::Tensor query_pair_order, at::Tensor key_order, int64_t valid, double scale) {
+                                             at::Tensor bias2, at::Tensor first_key, at::Tensor end_query,
+                                             at::Tensor query_tiles, at::Tensor query_pairs, at::Tensor key_tiles, int64_t valid, double scale) {
   c10::cuda::CUDAGuard guard(q.device());
   check_packed(q, k);
   q = readable(q);
@@ -119,17 +121,17 @@ std::vector<at::Tensor> packed_attention_bwd(at::Tensor d_o, at::Tensor q, at::T
   v = readable(v);
   TORCH_CHECK(d_o.sizes() == q.sizes() && d_o.scalar_type() == q.scalar_type() && d_o.device() == q.device() &&
                   o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.is_contiguous() &&
-                  lse2.scalar_type() == at::kFloat && lse2.is_contiguous() && lse2.numel() == (q.size(0) + 127) / 128 * 128 * q.size(1),
+                  bias2.scalar_type() == at::kFloat && bias2.is_contiguous() && bias2.numel() == (q.size(0) + 127) / 128 * 128 * q.size(1),
               "bergson_b200: the output's gradient does not fit the operands");
   d_o = readable(d_o);
-  const auto a = packed_args(q, k, v, first_key, end_query, query_order, query_pair_order, key_order, valid, scale);
-  auto delta = at::empty_like(lse2);
-  auto do_max = at::empty({lse2.numel() / 32}, lse2.options());
+  const auto a = packed_args(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale);
+  auto delta = at::empty_like(bias2);
+  auto do_max = at::empty({bias2.numel() / 32}, bias2.options());
   auto dq = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
   auto dk = at::empty({k.size(0), k.size(1), k.size(2)}, k.options());
   auto dv = at::empty_like(dk);
   const auto [tok, head] = strides_of(d_o);
-  ran(bgn_packed_attention_bwd(&a, o.data_ptr(), lse2.data_ptr<float>(), d_o.data_ptr(), tok, head,
+  ran(bgn_packed_attention_bwd(&a, o.data_ptr(), bias2.data_ptr<float>(), d_o.data_ptr(), tok, head,
                                delta.data_ptr<float>(), do_max.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                bgn_status_word(q), current()),
       "packed_attention_bwd");

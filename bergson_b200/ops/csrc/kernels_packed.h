@@ -15,24 +15,26 @@ typedef struct {
   long q_tok, q_head, k_tok, k_head, v_tok, v_head;
   const int* first_key;    // [rows]: first key that row t attends (its document's first token); t + 1: none
   const int* end_query;    // [rows]: one past the last row that attends key j; j: none
-  const int* query_order;  // [ceil(rows / 128)]: query tiles of 128 rows, most keys first
-  const int* query_pair_order;  // [ceil(rows / 256)]: pairs of neighbouring query tiles, most keys first
-  const int* key_order;    // [ceil(rows / 128)]: key tiles of 128 rows, most queries first
+  // Tiles of 128 rows, most work first, four numbers each, 16-byte aligned:
+  const int* query_tiles;  // [ceil(rows / 128)]: first row, its first key, the last row's first key, last key + 1
+  const int* query_pairs;  // [ceil(rows / 256)][2]: the same for pairs of neighbouring tiles
+  const int* key_tiles;    // [ceil(rows / 128)]: first key, last query + 1, last query + 1 of the first key, 0
   int rows;                // rows of the tensors
-  int pitch;               // rows rounded up to a multiple of 128: floats to a head of lse2 and delta
+  int pitch;               // rows rounded up to a multiple of 128: floats to a head of bias2 and delta
   int valid;               // rows that belong to documents; the ones behind give zeros
   int heads, kv_heads, dim;
   int type;                // 0 = fp16, 1 = bf16, 2 = fp32
   float scale;             // > 0
 } BgnPackedAttention;
 
-// o [rows, heads, dim] contiguous and lse2 [heads, pitch]: base-2 logarithm of the softmax denominator of
-// scale * log2(e) * q.k; +inf where a row attends nothing, unset from `rows` on.
-int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, float* lse2, int* status, cudaStream_t stream);
+// o [rows, heads, dim] contiguous and bias2 [heads, pitch]: minus the base-2 logarithm of the softmax
+// denominator of scale * log2(e) * q.k (for fp16 with 10 added); -inf where a row attends nothing,
+// unset from `rows` on.  The backward pass reads it.
+int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, float* bias2, int* status, cudaStream_t stream);
 
 // Gradients of the operands (contiguous) from the output's gradient d_o [rows, heads, dim] (strides in
-// elements), the forward's o and lse2.  Scratch: delta [heads, pitch], do_max [heads, pitch / 32].
-int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const float* lse2, const void* d_o, long do_tok,
+// elements), the forward's o and bias2.  Scratch: delta [heads, pitch], do_max [heads, pitch / 32].
+int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const float* bias2, const void* d_o, long do_tok,
                              long do_head, float* delta, float* do_max, void* dq, void* dk, void* dv, int* status,
                              cudaStream_t stream);
 

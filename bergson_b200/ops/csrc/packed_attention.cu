@@ -14,19 +14,25 @@ cudaError_t allow_smem(const void* kernel, int bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
+cudaError_t sm_count(int* n) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  return e == cudaSuccess ? cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, device) : e;
+}
+
 template <typename T, int DP>
-cudaError_t simple_fwd(const BgnPackedAttention& a, void* o, float* lse2, cudaStream_t stream) {
+cudaError_t simple_fwd(const BgnPackedAttention& a, void* o, float* bias2, cudaStream_t stream) {
   constexpr int smem = simple_smem<DP>(3);
   auto kern = packed_fwd_simple_kernel<T, DP>;
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
   const unsigned grid = unsigned((a.rows + 127) / 128) * 2u * unsigned(a.heads);
-  kern<<<grid, kSimpleThreads, smem, stream>>>(a, static_cast<T*>(o), lse2);
+  kern<<<grid, kSimpleThreads, smem, stream>>>(a, static_cast<T*>(o), bias2);
   return cudaGetLastError();
 }
 
 template <typename T, int DP>
-cudaError_t simple_bwd(const BgnPackedAttention& a, const void* o, const float* lse2, const void* d_o, long do_tok,
+cudaError_t simple_bwd(const BgnPackedAttention& a, const void* o, const float* bias2, const void* d_o, long do_tok,
                        long do_head, float* delta, void* dq, void* dk, void* dv, cudaStream_t stream) {
   constexpr int smem = simple_smem<DP>(4);
   auto kq = packed_dq_simple_kernel<T, DP>;
@@ -35,12 +41,12 @@ cudaError_t simple_bwd(const BgnPackedAttention& a, const void* o, const float* 
   if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(kk), smem);
   if (e != cudaSuccess) return e;
   const unsigned tiles = unsigned((a.rows + 127) / 128) * 2u;
-  kq<<<tiles * unsigned(a.heads), kSimpleThreads, smem, stream>>>(a, static_cast<const T*>(o), lse2,
+  kq<<<tiles * unsigned(a.heads), kSimpleThreads, smem, stream>>>(a, static_cast<const T*>(o), bias2,
                                                                   static_cast<const T*>(d_o), do_tok, do_head, delta,
                                                                   static_cast<T*>(dq));
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  kk<<<tiles * unsigned(a.kv_heads), kSimpleThreads, smem, stream>>>(a, lse2, static_cast<const T*>(d_o), do_tok,
+  kk<<<tiles * unsigned(a.kv_heads), kSimpleThreads, smem, stream>>>(a, bias2, static_cast<const T*>(d_o), do_tok,
                                                                      do_head, delta, static_cast<T*>(dk),
                                                                      static_cast<T*>(dv));
   return cudaGetLastError();
@@ -79,7 +85,7 @@ bool operand_map(CUtensorMap* map, const void* base, int fmt, int dim, int heads
 }
 
 template <int FMT, int DP>
-cudaError_t tensor_fwd(const BgnPackedAttention& a, void* o, float* lse2, int* status, cudaStream_t stream) {
+cudaError_t tensor_fwd(const BgnPackedAttention& a, void* o, float* bias2, int* status, cudaStream_t stream) {
   ensure_context_bound();
   CUtensorMap mq, mk, mv;
   if (!operand_map(&mq, a.q, FMT, a.dim, a.heads, a.valid, a.q_head, a.q_tok) ||
@@ -90,7 +96,9 @@ cudaError_t tensor_fwd(const BgnPackedAttention& a, void* o, float* lse2, int* s
   // Two heads of a group always see the same keys; two row tiles of a head do not.
   p.head_pairs = (a.heads / a.kv_heads) % 2 == 0;
   p.first_key = a.first_key;
-  p.order = p.head_pairs ? a.query_order : a.query_pair_order;
+  const int tiles = (a.rows + kTile - 1) / kTile;
+  p.tiles = reinterpret_cast<const int4*>(p.head_pairs ? a.query_tiles : a.query_pairs);
+  p.units = p.head_pairs ? tiles * (a.heads / 2) : (tiles + 1) / 2 * a.heads;
   p.rows = a.rows;
   p.valid = a.valid;
   p.pitch = a.pitch;
@@ -108,19 +116,20 @@ cudaError_t tensor_fwd(const BgnPackedAttention& a, void* o, float* lse2, int* s
   p.v_tok = a.v_tok;
   p.v_head = a.v_head;
   p.o = o;
-  p.lse2 = lse2;
+  p.bias2 = bias2;
   constexpr int smem = fwd_smem_bytes<DP>();
   auto kern = packed_fwd_kernel<FMT, DP>;
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
-  const unsigned tiles = unsigned((a.rows + kTile - 1) / kTile);
-  const unsigned grid = p.head_pairs ? tiles * unsigned(a.heads / 2) : (tiles + 1) / 2 * unsigned(a.heads);
-  kern<<<grid, kFwdThreads, smem, stream>>>(mq, mk, mv, p, status);
+  int sms = 0;
+  e = sm_count(&sms);
+  if (e != cudaSuccess) return e;
+  kern<<<unsigned(p.units < sms ? p.units : sms), kFwdThreads, smem, stream>>>(mq, mk, mv, p, status);
   return cudaGetLastError();
 }
 
 template <int FMT, int DP>
-cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const float* lse2, const void* d_o, long do_tok,
+cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const float* bias2, const void* d_o, long do_tok,
                        long do_head, float* delta, float* do_max, void* dq, void* dk, void* dv, int* status,
                        cudaStream_t stream) {
   ensure_context_bound();
@@ -153,8 +162,8 @@ cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const float* 
   p.v_head = a.v_head;
   p.do_tok = do_tok;
   p.do_head = do_head;
-  p.lse2 = lse2;
-  p.delta = delta;
+  p.bias2 = bias2;
+  p.neg_delta = delta;
   p.do_max = do_max;
   p.dq = dq;
   p.dk = dk;
@@ -164,15 +173,18 @@ cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const float* 
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kq), dq_smem_bytes<DP>());
   if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(kk), dkv_smem_bytes<DP>());
   if (e != cudaSuccess) return e;
-  const unsigned tiles = unsigned((a.rows + kTile - 1) / kTile);
-  p.head_pairs = (a.heads / a.kv_heads) % 2 == 0;
-  p.order = p.head_pairs ? a.query_order : a.query_pair_order;
-  const unsigned grid = p.head_pairs ? tiles * unsigned(a.heads / 2) : (tiles + 1) / 2 * unsigned(a.heads);
-  kq<<<grid, kBwdThreads, dq_smem_bytes<DP>(), stream>>>(mq, mg, mk, mv, p, status);
+  int sms = 0;
+  e = sm_count(&sms);
+  if (e != cudaSuccess) return e;
+  const int tiles = (a.rows + kTile - 1) / kTile;
+  p.tiles = reinterpret_cast<const int4*>(a.query_tiles);
+  p.units = tiles * a.heads;
+  kq<<<unsigned(p.units < sms ? p.units : sms), kBwdThreads, dq_smem_bytes<DP>(), stream>>>(mq, mg, mk, mv, p, status);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  p.order = a.key_order;
-  kk<<<tiles * unsigned(a.kv_heads), kBwdThreads, dkv_smem_bytes<DP>(), stream>>>(mq, mg, mk, mv, p, status);
+  p.tiles = reinterpret_cast<const int4*>(a.key_tiles);
+  p.units = tiles * a.kv_heads;
+  kk<<<unsigned(p.units < sms ? p.units : sms), kBwdThreads, dkv_smem_bytes<DP>(), stream>>>(mq, mg, mk, mv, p, status);
   return cudaGetLastError();
 }
 
@@ -184,25 +196,25 @@ bool sound(const BgnPackedAttention* a) {
 
 }  // namespace
 
-extern "C" int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, float* lse2, int* status,
+extern "C" int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, float* bias2, int* status,
                                         cudaStream_t stream) {
   if (!sound(a)) return int(cudaErrorInvalidValue);
   const bool narrow = a->dim <= 64;
-  if (a->type == 2) return int(narrow ? simple_fwd<float, 64>(*a, o, lse2, stream) : simple_fwd<float, 128>(*a, o, lse2, stream));
+  if (a->type == 2) return int(narrow ? simple_fwd<float, 64>(*a, o, bias2, stream) : simple_fwd<float, 128>(*a, o, bias2, stream));
   if (a->type == 1)
-    return int(narrow ? tensor_fwd<1, 64>(*a, o, lse2, status, stream) : tensor_fwd<1, 128>(*a, o, lse2, status, stream));
-  return int(narrow ? tensor_fwd<0, 64>(*a, o, lse2, status, stream) : tensor_fwd<0, 128>(*a, o, lse2, status, stream));
+    return int(narrow ? tensor_fwd<1, 64>(*a, o, bias2, status, stream) : tensor_fwd<1, 128>(*a, o, bias2, status, stream));
+  return int(narrow ? tensor_fwd<0, 64>(*a, o, bias2, status, stream) : tensor_fwd<0, 128>(*a, o, bias2, status, stream));
 }
 
-extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const float* lse2, const void* d_o,
+extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const float* bias2, const void* d_o,
                                         long do_tok, long do_head, float* delta, float* do_max, void* dq, void* dk,
                                         void* dv, int* status, cudaStream_t stream) {
   if (!sound(a)) return int(cudaErrorInvalidValue);
   const bool narrow = a->dim <= 64;
   if (a->type == 2)
-    return int(narrow ? simple_bwd<float, 64>(*a, o, lse2, d_o, do_tok, do_head, delta, dq, dk, dv, stream)
-                      : simple_bwd<float, 128>(*a, o, lse2, d_o, do_tok, do_head, delta, dq, dk, dv, stream));
+    return int(narrow ? simple_bwd<float, 64>(*a, o, bias2, d_o, do_tok, do_head, delta, dq, dk, dv, stream)
+                      : simple_bwd<float, 128>(*a, o, bias2, d_o, do_tok, do_head, delta, dq, dk, dv, stream));
   auto run = a->type == 1 ? (narrow ? tensor_bwd<1, 64> : tensor_bwd<1, 128>)
                           : (narrow ? tensor_bwd<0, 64> : tensor_bwd<0, 128>);
-  return int(run(*a, o, lse2, d_o, do_tok, do_head, delta, do_max, dq, dk, dv, status, stream));
+  return int(run(*a, o, bias2, d_o, do_tok, do_head, delta, do_max, dq, dk, dv, status, stream));
 }

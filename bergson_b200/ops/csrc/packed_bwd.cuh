@@ -1,6 +1,6 @@
 // Backward pass of the causal attention over packed documents on the tensor cores (fp16, bf16).
 //
-//   P = 2^(c q.k - lse2),  delta_t = do_t . o_t,  dS = P (do.v - delta)
+//   P = 2^(c q.k + bias2),  delta_t = do_t . o_t,  dS = P (do.v - delta)
 //   dQ = scale dS k,   dK = scale dS^T q,   dV = P^T do      (dK, dV summed over the heads of a group)
 //
 // Two kernels, each of which keeps its sums in TMEM from the first to the last tile: one block for the
@@ -25,24 +25,18 @@ constexpr int kBwdThreads = 384;
 struct PackedBwdArgs {
   const int* first_key;
   const int* end_query;
-  const int* order;
+  const int4* tiles;  // query_tiles or key_tiles
+  int units;          // tiles x heads of queries or of keys
   int rows, valid, heads, kv_heads, dim;
-  int head_pairs;  // dQ: as in the forward pass
-  int pitch;       // floats between the heads of lse2 and delta, a multiple of 128
+  int pitch;  // floats between the heads of bias2 and neg_delta, a multiple of 128
   float scale;
   const void *q, *k, *v, *o, *d_o;
   long q_tok, q_head, k_tok, k_head, v_tok, v_head, do_tok, do_head;
-  const float* lse2;
-  float* delta;
+  const float* bias2;
+  float* neg_delta;
   float* do_max;  // [heads, pitch / 32]: largest |do| of 32 rows (fp16)
   void *dq, *dk, *dv;
 };
-
-// fp16 only: P carries 2^10.
-template <int FMT>
-constexpr float p_shift() {
-  return FMT == 0 ? 10.f : 0.f;
-}
 
 // The power of two that brings `top` to [1/2, 1); 1 where there is nothing to scale.
 __device__ __forceinline__ float power_below_one(float top) {
@@ -59,25 +53,42 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
+// P (with its factor) of two columns in place: 2^(c s + bias).
+__device__ __forceinline__ void prob_pair(uint32_t& s0, uint32_t& s1, float2 c2, float2 bias) {
+  const float2 x = fma2(make_float2(__uint_as_float(s0), __uint_as_float(s1)), c2, bias);
+  s0 = __float_as_uint(fast_exp2(x.x));
+  s1 = __float_as_uint(fast_exp2(x.y));
+}
+
+// dS (with its factor) of two columns: P (dP - delta).
+template <int FMT>
+__device__ __forceinline__ float2 score_gradient(uint32_t p0, uint32_t p1, uint32_t d0, uint32_t d1, float2 neg_delta,
+                                                 float2 factor) {
+  float2 x = mul2(make_float2(__uint_as_float(p0), __uint_as_float(p1)),
+                  add2(make_float2(__uint_as_float(d0), __uint_as_float(d1)), neg_delta));
+  return FMT == 0 ? mul2(x, factor) : x;
+}
+
 // ---- dQ -------------------------------------------------------------------------------
 //
-// A block has two tiles of 128 query rows, as in the forward pass, and goes through their key tiles
-// step by step (a step is one key tile for one of the two):
-//   S = q k^T -> softmax warps of that tile: P in registers -> dP = do v^T -> dS over dP -> dQ += dS k.
-// The tensor core takes S of step n, then dQ of step n - 1, then dP of step n, so that it has work while
-// the softmax warps of either tile compute.
+// A unit is one tile of 128 query rows of a head.  Per key tile: S = q k^T and dP = do v^T, the softmax
+// warps turn them into dS (P stays in registers), dQ += dS k.  S is free again as soon as it is read and
+// dP has two places, so the two products of the next key tile run while this one's dS is formed.
 //
-// TMEM: dQ of the two tiles (256 columns), S (128), dP (128; dS in 16 bits over its first half).
-// Shared memory: q and do of the two tiles, two key tiles, one value tile (7 tiles of 32 KB at 128
-// features).  Warps: as in the forward pass; warps 10-11 look through partly masked key tiles.
+// TMEM: dQ, S, dP twice (128 columns each; dS in 16 bits over its dP).  Shared memory: q, do, three
+// key and two value tiles (7 tiles of 32 KB at 128 features).  Warps 0-7: softmax, warps 0-3 on the first 64 keys of a tile, 4-7 on the rest;
+// two threads share a row.  8 TMA, 9 MMA, 10-11 look through partly masked key tiles.
+
+constexpr int kDqKStages = 3;  // a key tile stays until dQ of its step, which comes after S and dP of the next
+constexpr int kDqVStages = 2;
 
 template <int DP>
 constexpr int dq_smem_bytes() {
-  return 7 * tile_bytes<DP>() + 1024 + 256;
+  return (2 + kDqKStages + kDqVStages) * tile_bytes<DP>() + 1024 + 256;
 }
 
 template <int FMT, int DP>
-__device__ __noinline__ void exact_dq_row(const PackedBwdArgs& p, int row, int head, float lse2, float delta, int lane) {
+__device__ __noinline__ void exact_dq_row(const PackedBwdArgs& p, int row, int head, float bias2, float neg_delta, int lane) {
   using T = typename Type16<FMT>::T;
   const int kv = head / (p.heads / p.kv_heads), first = p.first_key[row];
   const float c = p.scale * kPackedLog2e;
@@ -88,7 +99,7 @@ __device__ __noinline__ void exact_dq_row(const PackedBwdArgs& p, int row, int h
     float k[DP / 32], v[DP / 32];
     load_row<FMT, DP>(k, p.k, long(j) * p.k_tok + long(kv) * p.k_head, p.dim, lane);
     load_row<FMT, DP>(v, p.v, long(j) * p.v_tok + long(kv) * p.v_head, p.dim, lane);
-    const float ds = exp2f(warp_dot(q, k) * c - lse2) * (warp_dot(g, v) - delta);
+    const float ds = exp2f(warp_dot(q, k) * c + (bias2 - p_shift<FMT>())) * (warp_dot(g, v) + neg_delta);
 #pragma unroll
     for (int e = 0; e < DP / 32; ++e) dq[e] = fmaf(ds, k[e], dq[e]);
   }
@@ -106,69 +117,48 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   constexpr int kTileBytes = tile_bytes<DP>();
   constexpr int kSlabs = DP / 64;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* q_tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* g_tiles = q_tiles + 2 * kTileBytes;
-  uint8_t* k_tiles = g_tiles + 2 * kTileBytes;  // two
-  uint8_t* v_tile = k_tiles + 2 * kTileBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(v_tile + kTileBytes);
-  uint64_t* q_full = bars;         // [2]: q and do of a tile
-  uint64_t* k_full = q_full + 2;   // [2]
-  uint64_t* k_empty = k_full + 2;  // [2]
-  uint64_t* v_full = k_empty + 2;
-  uint64_t* v_empty = v_full + 1;
-  uint64_t* s_full = v_empty + 1;   // [2] per tile, as the following
-  uint64_t* s_read = s_full + 2;
-  uint64_t* dp_full = s_read + 2;
-  uint64_t* ds_full = dp_full + 2;
-  uint64_t* dq_full = ds_full + 2;  // [1]
-  uint64_t* checked = dq_full + 1;  // [1]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(checked + 1);
-  int* poison = reinterpret_cast<int*>(tmem_slot + 1);
+  uint8_t* q_tile = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* g_tile = q_tile + kTileBytes;
+  uint8_t* k_tiles = g_tile + kTileBytes;
+  uint8_t* v_tiles = k_tiles + kDqKStages * kTileBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(v_tiles + kDqVStages * kTileBytes);
+  uint64_t* q_full = bars;  // q and do
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* k_full = q_empty + 1;  // [3]
+  uint64_t* k_empty = k_full + kDqKStages;
+  uint64_t* v_full = k_empty + kDqKStages;  // [2]
+  uint64_t* v_empty = v_full + kDqVStages;
+  uint64_t* s_full = v_empty + kDqVStages;
+  uint64_t* s_read = s_full + 1;
+  uint64_t* dp_full = s_read + 1;   // [2]
+  uint64_t* ds_full = dp_full + 2;  // [2]
+  uint64_t* dq_full = ds_full + 2;
+  uint64_t* checked = dq_full + 1;  // [2]: units in turn
+  uint64_t* seen = checked + 2;     // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(seen + 2);
+  int* poison = reinterpret_cast<int*>(tmem_slot + 1);  // [2][2]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  int row0[2], head[2];
-  {
-    const int per = p.head_pairs ? p.heads / 2 : p.heads;
-    const int slot = __ldg(p.order + blockIdx.x / per), h = blockIdx.x % per;
-    if (p.head_pairs) {
-      row0[0] = row0[1] = slot * kTile;
-      head[0] = 2 * h;
-      head[1] = 2 * h + 1;
-    } else {
-      row0[0] = 2 * slot * kTile;
-      row0[1] = row0[0] + kTile;
-      head[0] = head[1] = h;
-    }
-  }
-  const int kv_head = head[0] / (p.heads / p.kv_heads);
-  KeyRange range[2] = {key_range(p.first_key, row0[0], p.valid), key_range(p.first_key, row0[1], p.valid)};
-  const bool some0 = range[0].hi > range[0].lo, some1 = range[1].hi > range[1].lo;
-  const int base = some0 ? (some1 ? min(range[0].lo, range[1].lo) : range[0].lo) : range[1].lo;
-  int i0[2], i1[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const bool some = t ? some1 : some0;
-    i0[t] = some ? (range[t].lo - base) / kTile : 0;
-    i1[t] = some ? (range[t].hi - base + kTile - 1) / kTile : 0;
-  }
-  const int n = max(i1[0], i1[1]);
+  const int group = p.heads / p.kv_heads;
 
   if (threadIdx.x == 0) {
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(&q_full[t], 1);
-      mbar_init(&k_full[t], 1);
-      mbar_init(&k_empty[t], 3);  // the MMA warp's commit and the two looking warps
-      mbar_init(&s_full[t], 1);
-      mbar_init(&s_read[t], 4);
-      mbar_init(&dp_full[t], 1);
-      mbar_init(&ds_full[t], 4);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 9);  // the MMA warp's commit and the softmax warps, which read do
+    for (int s = 0; s < kDqKStages; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 3);  // commit and the two looking warps
     }
-    mbar_init(v_full, 1);
-    mbar_init(v_empty, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&v_full[t], 1);
+      mbar_init(&v_empty[t], 1);
+      mbar_init(&dp_full[t], 1);
+      mbar_init(&ds_full[t], 8);
+      mbar_init(&checked[t], 2);
+      mbar_init(&seen[t], 8);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(s_read, 8);
     mbar_init(dq_full, 1);
-    mbar_init(checked, 2);
-    *poison = 0;
     fence_barrier_init();
     tma_prefetch_desc(&map_q);
     tma_prefetch_desc(&map_do);
@@ -183,242 +173,298 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t tmem_s = tmem + 256, tmem_dp = tmem + 384;
+  const uint32_t tmem_dq = tmem, tmem_s = tmem + 128, tmem_dp = tmem + 256;  // dp: two places
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");  // 3 * 168 >= 2 * 208 + 80
-    if (warp == 8) {
-      if (lane == 0) {
-        bool ok = true;
-        for (int t = 0; t < 2; ++t) {
-          if (i1[t] == 0) continue;
-          mbar_expect_tx(&q_full[t], 2 * kTileBytes);
-#pragma unroll
-          for (int s = 0; s < kSlabs; ++s) {
-            tma_load_3d(q_tiles + t * kTileBytes + s * kSlabBytes, &map_q, &q_full[t], 64 * s, head[t], row0[t]);
-            tma_load_3d(g_tiles + t * kTileBytes + s * kSlabBytes, &map_do, &q_full[t], 64 * s, head[t], row0[t]);
-          }
-        }
-        for (int i = 0; i < n && ok; ++i) {
-          const int st = i & 1, key = base + i * kTile;
-          ok = mbar_wait_bounded(&k_empty[st], ((i >> 1) & 1) ^ 1);
+  int unit = nth_unit(0, p.units);
+  int4 entry = unit >= 0 ? __ldg(p.tiles + unit / p.heads) : make_int4(0, 0, 0, 0);
+  // Of the unit at hand: first row, first key, key tiles.
+  const auto steps_of = [](const int4& e) { return e.w > e.y ? (e.w - e.y + kTile - 1) / kTile : 0; };
+
+  if (warp == 8) {
+    if (lane == 0) {
+      bool ok = true;
+      int j = 0, uses = 0;
+      for (int r = 0; unit >= 0 && ok; ++r) {
+        const int after = nth_unit(r + 1, p.units);
+        const int4 next = after >= 0 ? __ldg(p.tiles + after / p.heads) : entry;
+        const int head = unit % p.heads, kv_head = head / group, n = steps_of(entry);
+        for (int i = 0; i < n && ok; ++i, ++j) {
+          const int st = j % kDqKStages, vst = j % kDqVStages, key = entry.y + i * kTile;
+          ok = mbar_wait_bounded(&k_empty[st], ((j / kDqKStages) & 1) ^ 1);
           if (!ok) break;
           mbar_expect_tx(&k_full[st], kTileBytes);
 #pragma unroll
           for (int s = 0; s < kSlabs; ++s)
             tma_load_3d(k_tiles + st * kTileBytes + s * kSlabBytes, &map_k, &k_full[st], 64 * s, kv_head, key);
-          ok = mbar_wait_bounded(v_empty, (i & 1) ^ 1);
+          if (i == 0) {
+            ok = mbar_wait_bounded(q_empty, (uses & 1) ^ 1);
+            if (!ok) break;
+            ++uses;
+            mbar_expect_tx(q_full, 2 * kTileBytes);
+#pragma unroll
+            for (int s = 0; s < kSlabs; ++s) {
+              tma_load_3d(q_tile + s * kSlabBytes, &map_q, q_full, 64 * s, head, entry.x);
+              tma_load_3d(g_tile + s * kSlabBytes, &map_do, q_full, 64 * s, head, entry.x);
+            }
+          }
+          ok = mbar_wait_bounded(&v_empty[vst], ((j / kDqVStages) & 1) ^ 1);
           if (!ok) break;
-          mbar_expect_tx(v_full, kTileBytes);
+          mbar_expect_tx(&v_full[vst], kTileBytes);
 #pragma unroll
           for (int s = 0; s < kSlabs; ++s)
-            tma_load_3d(v_tile + s * kSlabBytes, &map_v, v_full, 64 * s, kv_head, key);
+            tma_load_3d(v_tiles + vst * kTileBytes + s * kSlabBytes, &map_v, &v_full[vst], 64 * s, kv_head, key);
         }
-        if (!ok) {
-          atomicCAS(status, kStatusOk, kStatusTimeoutProducer);
-          drain_copies();
-        }
+        unit = after;
+        entry = next;
+      }
+      if (!ok) {
+        atomicCAS(status, kStatusOk, kStatusTimeoutProducer);
+        drain_copies();
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    constexpr uint32_t idesc_s = make_idesc_f16(kTile, kTile, FMT, 0, 0);
+    constexpr uint32_t idesc_dq = make_idesc_f16(kTile, DP, FMT, 0, 1);
+    bool ok = true;
+    int j = 0, uses = 0;
+    const uint64_t dq = make_kmajor_sw128_desc(smem_u32(q_tile)), dg = make_kmajor_sw128_desc(smem_u32(g_tile));
+    const uint64_t dk = make_kmajor_sw128_desc(smem_u32(k_tiles)), dv = make_kmajor_sw128_desc(smem_u32(v_tiles));
+    const uint64_t dk_mn = make_mnmajor_sw128_desc(smem_u32(k_tiles), kSlabBytes);
+    constexpr uint64_t kStage = kTileBytes >> 4;
+    const auto scores = [&](uint32_t tmem_d, uint64_t a, uint64_t b) {  // one thread
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint64_t off = uint64_t(((k / 4) * kSlabBytes + (k % 4) * 32) >> 4);
+        umma_f16(tmem_d, a + off, b + off, idesc_s, k > 0 ? 1u : 0u);
+      }
+    };
+    // The two halves of the softmax warps leave their 64 keys over their own columns.
+    const auto add_dq = [&](int jj, bool first) {
+      const int st = jj % kDqKStages;
+      ok = ok && warp_wait(&ds_full[jj & 1], (jj >> 1) & 1);
+      if (!ok) return;
+      tc_fence_after();
+      const uint64_t b = dk_mn + st * kStage;
+      const uint32_t a = tmem_dp + 128 * (jj & 1);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          umma_f16_ts(tmem_dq, a + (k / 4) * 64 + (k % 4) * 8, b + uint64_t((2048 * k) >> 4), idesc_dq,
+                      (!first || k > 0) ? 1u : 0u);
+        umma_commit(&k_empty[st]);
       }
       __syncwarp();
-    } else if (warp == 9) {
-      constexpr uint32_t idesc_s = make_idesc_f16(kTile, kTile, FMT, 0, 0);
-      constexpr uint32_t idesc_dq = make_idesc_f16(kTile, DP, FMT, 0, 1);
-      if (lane == 0 && n > 0) {
-        bool ok = true;
-        int prev_t = -1, prev_i = 0;
-        const auto add_dq = [&](int t, int i) {  // dQ of a finished step
-          ok = ok && mbar_wait_bounded(&ds_full[t], (i - i0[t]) & 1);
-          if (!ok) return;
-          tc_fence_after();
-          const uint64_t dk = make_mnmajor_sw128_desc(smem_u32(k_tiles + (i & 1) * kTileBytes), kSlabBytes);
-#pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            umma_f16_ts(tmem + 128 * t, tmem_dp + 8 * k, dk + uint64_t((2048 * k) >> 4), idesc_dq,
-                        (i > i0[t] || k > 0) ? 1u : 0u);
-        };
-        for (int i = 0; i < n && ok; ++i) {
-          const uint32_t k_addr = smem_u32(k_tiles + (i & 1) * kTileBytes);
-          ok = mbar_wait_bounded(&k_full[i & 1], (i >> 1) & 1);
-          bool v_there = false;
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (i < i0[t] || i >= i1[t]) continue;
-            if (i == i0[t]) ok = mbar_wait_bounded(&q_full[t], 0);
-            if (prev_t >= 0) ok = ok && mbar_wait_bounded(&s_read[prev_t], (prev_i - i0[prev_t]) & 1);
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t dq = make_kmajor_sw128_desc(smem_u32(q_tiles + t * kTileBytes));
-            const uint64_t dk = make_kmajor_sw128_desc(k_addr);
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-              const uint64_t off = uint64_t(((k / 4) * kSlabBytes + (k % 4) * 32) >> 4);
-              umma_f16(tmem_s, dq + off, dk + off, idesc_s, k > 0 ? 1u : 0u);
-            }
-            umma_commit(&s_full[t]);
-            if (prev_t >= 0) {
-              add_dq(prev_t, prev_i);
-              if (!ok) break;
-              if (prev_i < i) umma_commit(&k_empty[prev_i & 1]);
-            }
-            if (!v_there) {
-              ok = mbar_wait_bounded(v_full, i & 1);
-              if (!ok) break;
-              v_there = true;
-            }
-            tc_fence_after();
-            const uint64_t dg = make_kmajor_sw128_desc(smem_u32(g_tiles + t * kTileBytes));
-            const uint64_t dv = make_kmajor_sw128_desc(smem_u32(v_tile));
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-              const uint64_t off = uint64_t(((k / 4) * kSlabBytes + (k % 4) * 32) >> 4);
-              umma_f16(tmem_dp, dg + off, dv + off, idesc_s, k > 0 ? 1u : 0u);
-            }
-            umma_commit(&dp_full[t]);
-            prev_t = t;
-            prev_i = i;
-          }
-          if (ok) umma_commit(v_empty);
+    };
+    for (int r = 0; unit >= 0 && ok; ++r) {
+      const int after = nth_unit(r + 1, p.units);
+      const int4 next = after >= 0 ? __ldg(p.tiles + after / p.heads) : entry;
+      const int n = steps_of(entry);
+      for (int i = 0; i < n && ok; ++i, ++j) {
+        const int st = j % kDqKStages, vst = j % kDqVStages;
+        if (i == 0) {
+          ok = warp_wait(q_full, uses & 1);
+          ++uses;
         }
-        if (ok) add_dq(prev_t, prev_i);
-        if (ok) umma_commit(dq_full);
-        if (!ok) atomicCAS(status, kStatusOk, kStatusTimeoutMma);
-      }
-      __syncwarp();
-    } else {
-      bool bad = false, ok = true;
-      for (int i = 0; i < n && ok; ++i) {
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&k_full[i & 1], (i >> 1) & 1));
-        const int key = base + i * kTile;
-        bool masked = false;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          masked |= i >= i0[t] && i < i1[t] && (key + kTile - 1 > row0[t] || key < range[t].last_first);
-        if (masked && ok) bad |= scan_not_finite<FMT>(k_tiles + (i & 1) * kTileBytes, kTileBytes, warp - 10, 2, lane);
+        ok = ok && warp_wait(&k_full[st], (j / kDqKStages) & 1);
+        ok = ok && (j == 0 || warp_wait(s_read, (j - 1) & 1));
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          scores(tmem_s, dq, dk + st * kStage);
+          umma_commit(s_full);
+        }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&k_empty[i & 1]);
+        ok = warp_wait(&v_full[vst], (j / kDqVStages) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          scores(tmem_dp + 128 * (j & 1), dg, dv + vst * kStage);
+          umma_commit(&dp_full[j & 1]);
+          umma_commit(&v_empty[vst]);
+          if (i == n - 1) umma_commit(q_empty);
+        }
+        __syncwarp();
+        if (i > 0) add_dq(j - 1, i == 1);
       }
-      if (__any_sync(0xffffffffu, bad) && lane == 0) *poison = 1;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(checked);
+      if (n > 0 && ok) {
+        add_dq(j - 1, n == 1);
+        if (ok && elect_one()) umma_commit(dq_full);
+        __syncwarp();
+      }
+      unit = after;
+      entry = next;
+    }
+    if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutMma);
+  } else if (warp >= 10) {
+    bool ok = true;
+    int j = 0, count = 0;
+    for (int r = 0; unit >= 0 && ok; ++r) {
+      const int after = nth_unit(r + 1, p.units);
+      const int4 next = after >= 0 ? __ldg(p.tiles + after / p.heads) : entry;
+      const int n = steps_of(entry);
+      bool bad = false;
+      for (int i = 0; i < n && ok; ++i, ++j) {
+        const int st = j % kDqKStages, key = entry.y + i * kTile;
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&k_full[st], (j / kDqKStages) & 1));
+        const bool masked = key + kTile - 1 > entry.x || key < entry.z;
+        if (masked && ok) bad |= scan_not_finite<FMT>(k_tiles + st * kTileBytes, kTileBytes, warp - 10, 2, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&k_empty[st]);
+      }
+      if (n > 0) {
+        const int slot = count & 1;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&seen[slot], ((count >> 1) & 1) ^ 1));
+        bad = __any_sync(0xffffffffu, bad);
+        if (lane == 0) {
+          poison[2 * slot + warp - 10] = bad;
+          mbar_arrive(&checked[slot]);
+        }
+        ++count;
+      }
+      unit = after;
+      entry = next;
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     using T = typename Type16<FMT>::T;
-    const int t = warp >> 2, quad = warp & 3;
-    const int my_i0 = t ? i0[1] : i0[0], my_i1 = t ? i1[1] : i1[0];
-    const int warp_row0 = (t ? row0[1] : row0[0]) + quad * 32, my_head = t ? head[1] : head[0];
-    const int row = warp_row0 + lane, tile_row = quad * 32 + lane;
-    const bool in = row < p.valid;
-    const int first = in ? __ldg(p.first_key + row) : 0x7fffffff;
-    const int all_from = __shfl_sync(0xffffffffu, in ? first : 0x7fffffff, 31);
+    const int half = warp >> 2, quad = warp & 3;
+    const int tile_row = quad * 32 + lane;
     const uint32_t lane_base = uint32_t(quad * 32) << 16;
-    const uint32_t ts = tmem_s + lane_base, tp = tmem_dp + lane_base;
+    const uint32_t ts = tmem_s + lane_base + 64 * half;
     const float c = p.scale * kPackedLog2e;
-    const float lse2 = in ? p.lse2[long(my_head) * p.pitch + row] : INFINITY;
     bool ok = true;
+    int j = 0, count = 0;
+    for (int r = 0; unit >= 0 && ok; ++r) {
+      const int head = unit % p.heads, n = steps_of(entry);
+      const int warp_row0 = entry.x + quad * 32, row = warp_row0 + lane;
+      const bool in = row < p.valid;
+      const long at = (long(row) * p.heads + head) * p.dim;
+      const int first = in ? __ldg(p.first_key + row) : 0x7fffffff;
+      const float bias2 = in ? p.bias2[long(head) * p.pitch + row] : -INFINITY;
+      const int all_from = __shfl_sync(0xffffffffu, first, 31);
 
-    // delta = do . o; do from the tile in shared memory (swizzled rows of 128 bytes).
-    float delta = 0.f, top = 0.f;
-    if (my_i1 > my_i0) {
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&q_full[t], 0));
-      if (ok && in) {
-        const uint8_t* g = g_tiles + t * kTileBytes + tile_row * 128;
-        const T* orow = static_cast<const T*>(p.o) + (long(row) * p.heads + my_head) * p.dim;
-#pragma unroll 4
-        for (int d = 0; d < p.dim; d += 8) {
-          union { uint4 u; T h[8]; } a, b;
-          a.u = *reinterpret_cast<const uint4*>(orow + d);
-          b.u = *reinterpret_cast<const uint4*>(g + (d / 64) * kSlabBytes + ((((d % 64) / 8) ^ (tile_row & 7)) << 4));
+      // delta = do . o: o from memory, asked for before do arrives in shared memory (swizzled rows of
+      // 128 bytes).  Both threads of a row compute it.
+      float neg_delta = 0.f, factor = 1.f;
+      if (n > 0) {
+        uint4 o_row[DP / 8];
+        const T* orow = static_cast<const T*>(p.o) + at;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x = to_float<T>(b.h[e]);
-            delta = fmaf(to_float<T>(a.h[e]), x, delta);
-            top = fmaxf(top, fabsf(x));
+        for (int d = 0; d < DP / 8; ++d)
+          o_row[d] = in && 8 * d < p.dim ? __ldg(reinterpret_cast<const uint4*>(orow + 8 * d)) : make_uint4(0, 0, 0, 0);
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(q_full, count & 1));
+        if (!ok) break;
+        float top = 0.f;
+        if (in) {
+          const uint8_t* g = g_tile + tile_row * 128;
+#pragma unroll
+          for (int d = 0; d < DP / 8; ++d) {
+            union { uint4 u; T h[8]; } a, b;
+            a.u = o_row[d];
+            b.u = *reinterpret_cast<const uint4*>(g + (d / 8) * kSlabBytes + (((d % 8) ^ (tile_row & 7)) << 4));
+            if (8 * d < p.dim) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float x = to_float<T>(b.h[e]);
+                neg_delta = fmaf(-to_float<T>(a.h[e]), x, neg_delta);
+                top = fmaxf(top, fabsf(x));
+              }
+            }
           }
         }
-      }
-    }
-    if (row < p.rows) p.delta[long(my_head) * p.pitch + row] = delta;
-    float factor = 1.f;
-    if (FMT == 0) {
-      top = warp_max(top);
-      if (lane == 0 && warp_row0 < p.pitch) p.do_max[(long(my_head) * p.pitch + warp_row0) / 32] = top;
-      factor = power_below_one(top);
-    }
-    const float base2 = -(lse2 - p_shift<FMT>());
-    const float ds_factor = FMT == 0 ? factor * (1.f / 1024.f) : 1.f;
-    const bool lone = first == row;  // one key: P = 1, and nothing goes through the softmax
-
-    for (int i = my_i0; i < my_i1 && ok; ++i) {
-      const int parity = (i - my_i0) & 1;
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[t], parity));
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) tmem_ld_32(ts + 32 * g, s[g]);
-      tmem_ld_wait();
-#pragma unroll
-      for (int g = 0; g < 4; ++g) pin_32(s[g]);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_read[t]);
-      const int key = base + i * kTile;
-      const bool masked = key + kTile - 1 > warp_row0 || key < all_from;
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-          s[g][e] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(s[g][e]), c, base2)));
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&dp_full[t], parity));
-      if (!ok) break;
-      tc_fence_after();
-      const int from = lone ? 0x7fffffff : first - key, upto = row - key;
-#pragma unroll
-      for (int g = 0; g < 4; g += 2) {
-        uint32_t w[32];
-#pragma unroll
-        for (int gg = g; gg < g + 2; ++gg) {
-          uint32_t d[32];
-          tmem_ld_32(tp + 32 * gg, d);
-          tmem_ld_wait();
-          pin_32(d);
-          float x[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            x[e] = __uint_as_float(s[gg][e]) * (__uint_as_float(d[e]) - delta);
-            if (FMT == 0) x[e] *= ds_factor;
-          }
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * gg + e < from || 32 * gg + e > upto) x[e] = 0.f;
-          }
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) w[(gg - g) * 16 + e / 2] = pack16<FMT>(x[e], x[e + 1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_empty);
+        if (FMT == 0) {
+          top = warp_max(top);
+          factor = power_below_one(top);
+          if (half == 0 && lane == 0) p.do_max[(long(head) * p.pitch + warp_row0) / 32] = top;
         }
-        tmem_st_32(tp + 16 * g, w);
+      } else if (FMT == 0 && half == 0 && lane == 0) {
+        p.do_max[(long(head) * p.pitch + warp_row0) / 32] = 0.f;
       }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ds_full[t]);
+      if (half == 0 && row < p.rows) p.neg_delta[long(head) * p.pitch + row] = neg_delta;
+      const float ds_factor = FMT == 0 ? factor * (1.f / 1024.f) : 1.f;
+      const bool lone = first == row;  // one key: P = 1, and nothing goes through the softmax
+      const float2 c2 = make_float2(c, c), b2 = make_float2(bias2, bias2), d2 = make_float2(neg_delta, neg_delta);
+      const float2 f2 = make_float2(ds_factor, ds_factor);
+
+      for (int i = 0; i < n; ++i, ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_full, j & 1));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[2][32];
+        tmem_ld_32(ts, s[0]);
+        tmem_ld_32(ts + 32, s[1]);
+        tmem_ld_wait();
+        pin_32(s[0]);
+        pin_32(s[1]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_read);
+        const int key = entry.y + i * kTile + 64 * half;  // first key of this half
+        const bool masked = key + 63 > warp_row0 || key < all_from;
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) prob_pair(s[g][e], s[g][e + 1], c2, b2);
+        const uint32_t tp = tmem_dp + 128 * (j & 1) + lane_base + 64 * half;
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&dp_full[j & 1], (j >> 1) & 1));
+        if (!ok) break;
+        tc_fence_after();
+        const int from = lone ? 0x7fffffff : first - key, upto = row - key;
+        uint32_t d[2][32];
+        tmem_ld_32(tp, d[0]);
+        tmem_ld_32(tp + 32, d[1]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          pin_32(d[g]);
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 x = score_gradient<FMT>(s[g][e], s[g][e + 1], d[g][e], d[g][e + 1], d2, f2);
+            d[g][e] = __float_as_uint(x.x);
+            d[g][e + 1] = __float_as_uint(x.y);
+          }
+          if (masked) hide(d[g], bit_range(from - 32 * g, upto - 32 * g), 0u);
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = pack16<FMT>(__uint_as_float(d[g][2 * e]), __uint_as_float(d[g][2 * e + 1]));
+          tmem_st_16(tp + 16 * g, w);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ds_full[j & 1]);
+      }
+      if (!ok) break;
+      // the next unit, under what is left of this one
+      unit = nth_unit(r + 1, p.units);
+      if (unit >= 0) entry = __ldg(p.tiles + unit / p.heads);
+      const bool some = in && first <= row;
+      T* dst = static_cast<T*>(p.dq) + at;
+      if (n > 0) {
+        const int slot = count & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&checked[slot], (count >> 1) & 1));
+        const bool exact = (poison[2 * slot] | poison[2 * slot + 1]) != 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&seen[slot]);
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(dq_full, count & 1)) && ok;
+        ++count;
+        if (!ok) break;
+        tc_fence_after();
+        // each of the two threads of a row stores one half of the features
+        if (!exact) store_row<FMT, DP>(tmem_dq + lane_base, p.scale / factor, dst, p.dim, some, half);
+        for (int rr = half; exact && rr < 32; rr += 2) {
+          const float bias_r = __shfl_sync(0xffffffffu, bias2, rr), delta_r = __shfl_sync(0xffffffffu, neg_delta, rr);
+          if (__shfl_sync(0xffffffffu, int(some), rr))
+            exact_dq_row<FMT, DP>(p, warp_row0 + rr, head, bias_r, delta_r, lane);
+        }
+        tc_fence_before();
+      }
+      if (!some && row < p.rows && half == 0)
+        for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
     }
-    if (ok && my_i1 > my_i0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(dq_full, 0));
-    ok = __all_sync(0xffffffffu, mbar_wait_bounded(checked, 0)) && ok;
     if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutEpilogue);
-    tc_fence_after();
-    const bool some = in && first <= row;
-    T* dst = static_cast<T*>(p.dq) + (long(row) * p.heads + my_head) * p.dim;
-    const bool exact = *reinterpret_cast<volatile int*>(poison) != 0;
-    if (my_i1 > my_i0 && ok) {
-      if (!exact) store_row<FMT, DP>(tmem + 128 * t + lane_base, p.scale / factor, dst, p.dim, some);
-      for (int r = 0; exact && r < 32; ++r) {
-        const float lse_r = __shfl_sync(0xffffffffu, lse2, r), delta_r = __shfl_sync(0xffffffffu, delta, r);
-        if (__shfl_sync(0xffffffffu, int(some), r)) exact_dq_row<FMT, DP>(p, warp_row0 + r, my_head, lse_r, delta_r, lane);
-      }
-    }
-    if (!some && row < p.rows)
-      for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
   }
 
   tc_fence_before();
@@ -431,20 +477,20 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 
 // ---- dK, dV ---------------------------------------------------------------------------
 //
-// A block has 128 key rows of one key head and goes through the query tiles that may attend them, for
+// A unit is 128 key rows of one key head: it goes through the query tiles that may attend them, for
 // one head of the group after the other.  Scores are transposed, keys along the lanes:
 //   S^T = k q^T -> P^T in 16 bits over S^T -> dV += P^T do;   dP^T = v do^T -> dS^T over dP^T -> dK += dS^T q.
 // The tensor core takes dV of step j, S^T of j + 1, dK of j, dP^T of j + 1: the softmax warps turn S^T into
 // P^T under dK and dP^T, and dP^T into dS^T under dV and S^T.
 //
 // TMEM: dV, dK (up to 128 columns each), S^T, dP^T (128 each).  Shared memory: k, v, three query tiles,
-// two tiles of do with the rows' lse2 and delta.  Warps 0-7: softmax, warps 0-3 on the first 64
-// queries of a tile, 4-7 on the rest; a thread has a key.  8 TMA, 9 MMA, 10-11 look through partly
-// masked tiles of q and do.
+// two tiles of do with the rows' bias2 and delta.  Warps 0-7: softmax, warps 0-3 on the first 64
+// queries of a tile, 4-7 on the rest; two threads share a key.  8 TMA, 9 MMA, 10-11 look through
+// partly masked tiles of q and do.
 
 constexpr int kDkvQStages = 3;
 constexpr int kDkvGStages = 2;
-constexpr int kDkvRowBytes = 2 * kTile * 4;  // lse2 and delta of a query tile
+constexpr int kDkvRowBytes = 2 * kTile * 4;  // bias2 and delta of a query tile
 
 template <int DP>
 constexpr int dkv_smem_bytes() {
@@ -464,8 +510,8 @@ __device__ __noinline__ void exact_dkv_row(const PackedBwdArgs& p, int key, int 
       float q[DP / 32], g[DP / 32];
       load_row<FMT, DP>(q, p.q, long(row) * p.q_tok + long(head) * p.q_head, p.dim, lane);
       load_row<FMT, DP>(g, p.d_o, long(row) * p.do_tok + long(head) * p.do_head, p.dim, lane);
-      const float w = exp2f(warp_dot(q, k) * c - p.lse2[long(head) * p.pitch + row]);
-      const float ds = row == first ? 0.f : w * (warp_dot(g, v) - p.delta[long(head) * p.pitch + row]);
+      const float w = exp2f(warp_dot(q, k) * c + (p.bias2[long(head) * p.pitch + row] - p_shift<FMT>()));
+      const float ds = row == first ? 0.f : w * (warp_dot(g, v) + p.neg_delta[long(head) * p.pitch + row]);
 #pragma unroll
       for (int e = 0; e < DP / 32; ++e) {
         dv[e] = fmaf(w, g[e], dv[e]);
@@ -499,10 +545,13 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint8_t* v_tile = k_tile + kTileBytes;
   uint8_t* q_tiles = v_tile + kTileBytes;
   uint8_t* g_tiles = q_tiles + kDkvQStages * kTileBytes;
-  float* row_values = reinterpret_cast<float*>(g_tiles + kDkvGStages * kTileBytes);  // [stage][lse2, delta][128]
+  float* row_values = reinterpret_cast<float*>(g_tiles + kDkvGStages * kTileBytes);  // [stage][bias2, -delta][128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(row_values) + kDkvGStages * kDkvRowBytes);
-  uint64_t* kv_full = bars;
-  uint64_t* q_full = kv_full + 1;            // [3]
+  uint64_t* k_full = bars;
+  uint64_t* k_empty = k_full + 1;
+  uint64_t* v_full = k_empty + 1;
+  uint64_t* v_empty = v_full + 1;
+  uint64_t* q_full = v_empty + 1;            // [3]
   uint64_t* q_empty = q_full + kDkvQStages;  // [3]
   uint64_t* g_full = q_empty + kDkvQStages;  // [2]
   uint64_t* g_empty = g_full + kDkvGStages;  // [2]
@@ -511,25 +560,22 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint64_t* dp_full = p_full + 1;
   uint64_t* ds_full = dp_full + 1;
   uint64_t* done = ds_full + 1;
-  uint64_t* checked = done + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(checked + 1);
-  int* poison = reinterpret_cast<int*>(tmem_slot + 1);
-  float* tops = reinterpret_cast<float*>(poison + 1);  // [12]: per warp
+  uint64_t* checked = done + 1;  // [2]: units in turn
+  uint64_t* seen = checked + 2;  // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(seen + 2);
+  int* poison = reinterpret_cast<int*>(tmem_slot + 1);  // [2][2]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kv_head = blockIdx.x % p.kv_heads, group = p.heads / p.kv_heads;
-  const int k0 = __ldg(p.order + blockIdx.x / p.kv_heads) * kTile;
-  const int k1 = min(k0 + kTile, p.valid);
-  const int q_end = k1 > k0 ? min(__ldg(p.end_query + k1 - 1), p.valid) : k0;
-  const int first_end = k1 > k0 ? __ldg(p.end_query + k0) : 0;
-  const int per_head = (q_end - k0 + kTile - 1) / kTile;
-  const int n = per_head * group;
+  const int group = p.heads / p.kv_heads;
 
   if (threadIdx.x == 0) {
-    mbar_init(kv_full, 1);
+    mbar_init(k_full, 1);
+    mbar_init(k_empty, 1);
+    mbar_init(v_full, 1);
+    mbar_init(v_empty, 1);
     for (int s = 0; s < kDkvQStages; ++s) {
       mbar_init(&q_full[s], 1);
-      mbar_init(&q_empty[s], 3);
+      mbar_init(&q_empty[s], 3);  // commit, 2 looking warps
     }
     for (int s = 0; s < kDkvGStages; ++s) {
       mbar_init(&g_full[s], 1);
@@ -540,8 +586,10 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     mbar_init(dp_full, 1);
     mbar_init(ds_full, 8);
     mbar_init(done, 1);
-    mbar_init(checked, 2);
-    *poison = 0;
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&checked[t], 2);
+      mbar_init(&seen[t], 8);
+    }
     fence_barrier_init();
     tma_prefetch_desc(&map_q);
     tma_prefetch_desc(&map_do);
@@ -552,55 +600,64 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  // fp16: the largest |do| among the rows of all steps sets the factor of dS.
-  float factor = 1.f;
-  if (FMT == 0) {
-    float top = 0.f;
-    for (int i = threadIdx.x; i < n * 4; i += kBwdThreads) {
-      const int h = kv_head * group + i / (per_head * 4);
-      top = fmaxf(top, p.do_max[(long(h) * p.pitch + k0) / 32 + i % (per_head * 4)]);
-    }
-    top = warp_max(top);
-    if (lane == 0) tops[warp] = top;
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (FMT == 0) {
-    float top = 0.f;
-    for (int w = 0; w < kBwdThreads / 32; ++w) top = fmaxf(top, tops[w]);
-    factor = power_below_one(top);
-  }
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_dv = tmem, tmem_dk = tmem + 128, tmem_s = tmem + 256, tmem_dp = tmem + 384;
 
+  int unit = nth_unit(0, p.units);
+  int4 entry = unit >= 0 ? __ldg(p.tiles + unit / p.kv_heads) : make_int4(0, 0, 0, 0);
+  const auto tiles_of = [](const int4& e) { return (e.y - e.x + kTile - 1) / kTile; };  // query tiles of a head
+
   if (warp == 8) {
-    if (lane == 0 && n > 0) {
+    if (lane == 0) {
       bool ok = true;
-      mbar_expect_tx(kv_full, 2 * kTileBytes);
+      int base = 0, uses = 0;
+      for (int r = 0; unit >= 0 && ok; ++r) {
+        const int after = nth_unit(r + 1, p.units);
+        const int4 next = after >= 0 ? __ldg(p.tiles + after / p.kv_heads) : entry;
+        const int kv_head = unit % p.kv_heads, per_head = tiles_of(entry), n = per_head * group;
+        for (int i = 0; i < n && ok; ++i) {
+          const int j = base + i;
+          const int h = kv_head * group + i / per_head, q0 = entry.x + (i % per_head) * kTile;
+          const int qs = j % kDkvQStages, gs = j % kDkvGStages;
+          if (i == 0) {
+            ok = mbar_wait_bounded(k_empty, (uses & 1) ^ 1);
+            if (!ok) break;
+            mbar_expect_tx(k_full, kTileBytes);
 #pragma unroll
-      for (int s = 0; s < kSlabs; ++s) {
-        tma_load_3d(k_tile + s * kSlabBytes, &map_k, kv_full, 64 * s, kv_head, k0);
-        tma_load_3d(v_tile + s * kSlabBytes, &map_v, kv_full, 64 * s, kv_head, k0);
-      }
-      for (int j = 0; j < n && ok; ++j) {
-        const int h = kv_head * group + j / per_head, q0 = k0 + (j % per_head) * kTile;
-        const int qs = j % kDkvQStages, gs = j % kDkvGStages;
-        ok = mbar_wait_bounded(&q_empty[qs], ((j / kDkvQStages) & 1) ^ 1);
-        if (!ok) break;
-        mbar_expect_tx(&q_full[qs], kTileBytes);
+            for (int s = 0; s < kSlabs; ++s)
+              tma_load_3d(k_tile + s * kSlabBytes, &map_k, k_full, 64 * s, kv_head, entry.x);
+          }
+          ok = mbar_wait_bounded(&q_empty[qs], ((j / kDkvQStages) & 1) ^ 1);
+          if (!ok) break;
+          mbar_expect_tx(&q_full[qs], kTileBytes);
 #pragma unroll
-        for (int s = 0; s < kSlabs; ++s)
-          tma_load_3d(q_tiles + qs * kTileBytes + s * kSlabBytes, &map_q, &q_full[qs], 64 * s, h, q0);
-        ok = mbar_wait_bounded(&g_empty[gs], ((j / kDkvGStages) & 1) ^ 1);
-        if (!ok) break;
-        mbar_expect_tx(&g_full[gs], kTileBytes + kDkvRowBytes);
+          for (int s = 0; s < kSlabs; ++s)
+            tma_load_3d(q_tiles + qs * kTileBytes + s * kSlabBytes, &map_q, &q_full[qs], 64 * s, h, q0);
+          if (i == 0) {
+            ok = mbar_wait_bounded(v_empty, (uses & 1) ^ 1);
+            if (!ok) break;
+            ++uses;
+            mbar_expect_tx(v_full, kTileBytes);
 #pragma unroll
-        for (int s = 0; s < kSlabs; ++s)
-          tma_load_3d(g_tiles + gs * kTileBytes + s * kSlabBytes, &map_do, &g_full[gs], 64 * s, h, q0);
-        // lse2 and delta have whole tiles of rows to a head, so the copy stays inside
-        bulk_load(row_values + gs * 2 * kTile, p.lse2 + long(h) * p.pitch + q0, kTile * 4, &g_full[gs]);
-        bulk_load(row_values + gs * 2 * kTile + kTile, p.delta + long(h) * p.pitch + q0, kTile * 4, &g_full[gs]);
+            for (int s = 0; s < kSlabs; ++s)
+              tma_load_3d(v_tile + s * kSlabBytes, &map_v, v_full, 64 * s, kv_head, entry.x);
+          }
+          ok = mbar_wait_bounded(&g_empty[gs], ((j / kDkvGStages) & 1) ^ 1);
+          if (!ok) break;
+          mbar_expect_tx(&g_full[gs], kTileBytes + kDkvRowBytes);
+#pragma unroll
+          for (int s = 0; s < kSlabs; ++s)
+            tma_load_3d(g_tiles + gs * kTileBytes + s * kSlabBytes, &map_do, &g_full[gs], 64 * s, h, q0);
+          // bias2 and delta have whole tiles of rows to a head, so the copies stay inside
+          bulk_load(row_values + gs * 2 * kTile, p.bias2 + long(h) * p.pitch + q0, kTile * 4, &g_full[gs]);
+          bulk_load(row_values + gs * 2 * kTile + kTile, p.neg_delta + long(h) * p.pitch + q0, kTile * 4, &g_full[gs]);
+        }
+        base += n;
+        unit = after;
+        entry = next;
       }
       if (!ok) {
         atomicCAS(status, kStatusOk, kStatusTimeoutProducer);
@@ -611,189 +668,250 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   } else if (warp == 9) {
     constexpr uint32_t idesc_s = make_idesc_f16(kTile, kTile, FMT, 0, 0);
     constexpr uint32_t idesc_d = make_idesc_f16(kTile, DP, FMT, 0, 1);
-    if (lane == 0 && n > 0) {
-      bool ok = mbar_wait_bounded(kv_full, 0);
-      const uint64_t dk = make_kmajor_sw128_desc(smem_u32(k_tile)), dv = make_kmajor_sw128_desc(smem_u32(v_tile));
-      const auto scores = [&](uint32_t tmem_d, uint64_t a, const uint8_t* b_tile, uint64_t* bar) {
-        tc_fence_after();
-        const uint64_t b = make_kmajor_sw128_desc(smem_u32(b_tile));
+    bool ok = true;
+    const uint64_t dk = make_kmajor_sw128_desc(smem_u32(k_tile)), dv = make_kmajor_sw128_desc(smem_u32(v_tile));
+    const uint64_t dq = make_kmajor_sw128_desc(smem_u32(q_tiles)), dg = make_kmajor_sw128_desc(smem_u32(g_tiles));
+    const uint64_t dq_mn = make_mnmajor_sw128_desc(smem_u32(q_tiles), kSlabBytes);
+    const uint64_t dg_mn = make_mnmajor_sw128_desc(smem_u32(g_tiles), kSlabBytes);
+    constexpr uint64_t kStage = kTileBytes >> 4;
+    const auto scores = [&](uint32_t tmem_d, uint64_t a, uint64_t b) {  // one thread
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint64_t off = uint64_t(((k / 4) * kSlabBytes + (k % 4) * 32) >> 4);
-          umma_f16(tmem_d, a + off, b + off, idesc_s, k > 0 ? 1u : 0u);
-        }
-        umma_commit(bar);
-      };
-      // The two halves of the softmax warps leave their 64 queries over their own columns.
-      const auto add = [&](uint32_t tmem_d, uint32_t tmem_a, const uint8_t* b_tile, bool first) {
-        tc_fence_after();
-        const uint64_t b = make_mnmajor_sw128_desc(smem_u32(b_tile), kSlabBytes);
-#pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          umma_f16_ts(tmem_d, tmem_a + (k / 4) * 64 + (k % 4) * 8, b + uint64_t((2048 * k) >> 4), idesc_d,
-                      (!first || k > 0) ? 1u : 0u);
-      };
-      ok = ok && mbar_wait_bounded(&q_full[0], 0);
-      if (ok) scores(tmem_s, dk, q_tiles, s_full);
-      ok = ok && mbar_wait_bounded(&g_full[0], 0);
-      if (ok) scores(tmem_dp, dv, g_tiles, dp_full);
-      for (int j = 0; j < n && ok; ++j) {
-        const int qs = j % kDkvQStages, gs = j % kDkvGStages;
-        const int qn = (j + 1) % kDkvQStages, gn = (j + 1) % kDkvGStages;
-        ok = mbar_wait_bounded(p_full, j & 1);
-        if (!ok) break;
-        add(tmem_dv, tmem_s, g_tiles + gs * kTileBytes, j == 0);
-        umma_commit(&g_empty[gs]);
-        if (j + 1 < n) {
-          ok = mbar_wait_bounded(&q_full[qn], ((j + 1) / kDkvQStages) & 1);
-          if (!ok) break;
-          scores(tmem_s, dk, q_tiles + qn * kTileBytes, s_full);
-        }
-        ok = mbar_wait_bounded(ds_full, j & 1);
-        if (!ok) break;
-        add(tmem_dk, tmem_dp, q_tiles + qs * kTileBytes, j == 0);
-        umma_commit(&q_empty[qs]);
-        if (j + 1 < n) {
-          ok = mbar_wait_bounded(&g_full[gn], ((j + 1) / kDkvGStages) & 1);
-          if (!ok) break;
-          scores(tmem_dp, dv, g_tiles + gn * kTileBytes, dp_full);
-        }
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint64_t off = uint64_t(((k / 4) * kSlabBytes + (k % 4) * 32) >> 4);
+        umma_f16(tmem_d, a + off, b + off, idesc_s, k > 0 ? 1u : 0u);
       }
-      if (ok) umma_commit(done);
-      if (!ok) atomicCAS(status, kStatusOk, kStatusTimeoutMma);
+    };
+    // The two halves of the softmax warps leave their 64 queries over their own columns.
+    const auto add = [&](uint32_t tmem_d, uint32_t tmem_a, uint64_t b, bool first) {  // one thread
+#pragma unroll
+      for (int k = 0; k < kTile / 16; ++k)
+        umma_f16_ts(tmem_d, tmem_a + (k / 4) * 64 + (k % 4) * 8, b + uint64_t((2048 * k) >> 4), idesc_d,
+                    (!first || k > 0) ? 1u : 0u);
+    };
+    int base = 0, uses = 0;
+    for (int r = 0; unit >= 0 && ok; ++r) {
+      const int after = nth_unit(r + 1, p.units);
+      const int4 next = after >= 0 ? __ldg(p.tiles + after / p.kv_heads) : entry;
+      const int n = tiles_of(entry) * group;
+      const auto first_product = [&](int i) {
+        const int j = base + i, qs = j % kDkvQStages;
+        ok = ok && warp_wait(&q_full[qs], (j / kDkvQStages) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        if (elect_one()) {
+          scores(tmem_s, dk, dq + qs * kStage);
+          umma_commit(s_full);
+          if (i == n - 1) umma_commit(k_empty);
+        }
+        __syncwarp();
+      };
+      const auto third_product = [&](int i) {
+        const int j = base + i, gs = j % kDkvGStages;
+        ok = ok && warp_wait(&g_full[gs], (j / kDkvGStages) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        if (elect_one()) {
+          scores(tmem_dp, dv, dg + gs * kStage);
+          umma_commit(dp_full);
+          if (i == n - 1) umma_commit(v_empty);
+        }
+        __syncwarp();
+      };
+      if (n > 0) {
+        ok = warp_wait(k_full, uses & 1);
+        first_product(0);
+        ok = ok && warp_wait(v_full, uses & 1);
+        third_product(0);
+        ++uses;
+      }
+      for (int i = 0; i < n && ok; ++i) {
+        const int j = base + i;
+        const int qs = j % kDkvQStages, gs = j % kDkvGStages;
+        ok = warp_wait(p_full, j & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          add(tmem_dv, tmem_s, dg_mn + gs * kStage, i == 0);
+          umma_commit(&g_empty[gs]);
+        }
+        __syncwarp();
+        if (i + 1 < n) first_product(i + 1);
+        ok = ok && warp_wait(ds_full, j & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          add(tmem_dk, tmem_dp, dq_mn + qs * kStage, i == 0);
+          umma_commit(&q_empty[qs]);
+          if (i == n - 1) umma_commit(done);
+        }
+        __syncwarp();
+        if (i + 1 < n) third_product(i + 1);
+      }
+      base += n;
+      unit = after;
+      entry = next;
     }
-    __syncwarp();
+    if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutMma);
   } else if (warp >= 10) {
-    bool bad = false, ok = true;
-    for (int j = 0; j < n && ok; ++j) {
-      const int q0 = k0 + (j % per_head) * kTile;
-      const int qs = j % kDkvQStages, gs = j % kDkvGStages;
-      const bool masked = q0 < k0 + kTile || q0 + kTile > first_end;
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&q_full[qs], (j / kDkvQStages) & 1));
-      if (masked && ok) bad |= scan_not_finite<FMT>(q_tiles + qs * kTileBytes, kTileBytes, warp - 10, 2, lane);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_empty[qs]);
-      ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&g_full[gs], (j / kDkvGStages) & 1));
-      if (masked && ok) bad |= scan_not_finite<FMT>(g_tiles + gs * kTileBytes, kTileBytes, warp - 10, 2, lane);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&g_empty[gs]);
+    bool ok = true;
+    int j = 0, count = 0;
+    for (int r = 0; unit >= 0 && ok; ++r) {
+      const int after = nth_unit(r + 1, p.units);
+      const int4 next = after >= 0 ? __ldg(p.tiles + after / p.kv_heads) : entry;
+      const int per_head = tiles_of(entry), n = per_head * group;
+      bool bad = false;
+      for (int i = 0; i < n && ok; ++i, ++j) {
+        const int q0 = entry.x + (i % per_head) * kTile;
+        const int qs = j % kDkvQStages, gs = j % kDkvGStages;
+        const bool masked = q0 < entry.x + kTile || q0 + kTile > entry.z;
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&q_full[qs], (j / kDkvQStages) & 1));
+        if (masked && ok) bad |= scan_not_finite<FMT>(q_tiles + qs * kTileBytes, kTileBytes, warp - 10, 2, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_empty[qs]);
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&g_full[gs], (j / kDkvGStages) & 1));
+        if (masked && ok) bad |= scan_not_finite<FMT>(g_tiles + gs * kTileBytes, kTileBytes, warp - 10, 2, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&g_empty[gs]);
+      }
+      if (n > 0) {
+        const int slot = count & 1;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&seen[slot], ((count >> 1) & 1) ^ 1));
+        bad = __any_sync(0xffffffffu, bad);
+        if (lane == 0) {
+          poison[2 * slot + warp - 10] = bad;
+          mbar_arrive(&checked[slot]);
+        }
+        ++count;
+      }
+      unit = after;
+      entry = next;
     }
-    if (__any_sync(0xffffffffu, bad) && lane == 0) *poison = 1;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(checked);
   } else {
     using T = typename Type16<FMT>::T;
     const int half = warp >> 2, quad = warp & 3;
-    const int key = k0 + quad * 32 + lane;
-    const bool in = key < p.valid;
-    const int end = in ? __ldg(p.end_query + key) : 0;
-    const bool opens = in && __ldg(p.first_key + key) == key;  // its own row attends nothing else
-    const int warp_key_last = k0 + quad * 32 + 31;
-    const int min_end = __reduce_min_sync(0xffffffffu, end);
     const uint32_t lane_base = uint32_t(quad * 32) << 16;
     const uint32_t ts = tmem_s + lane_base + 64 * half, tp = tmem_dp + lane_base + 64 * half;
     const float c = p.scale * kPackedLog2e;
-    const float ds_factor = FMT == 0 ? factor * (1.f / 1024.f) : 1.f;
+    const float2 c2 = make_float2(c, c);
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      const int gs = j % kDkvGStages;
-      const int q0 = k0 + (j % per_head) * kTile + 64 * half;  // first query of this half
-      ok = mbar_wait_bounded(&g_full[gs], (j / kDkvGStages) & 1);
-      ok = mbar_wait_bounded(s_full, j & 1) && ok;
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t s[2][32];
-      tmem_ld_32(ts, s[0]);
-      tmem_ld_32(ts + 32, s[1]);
-      tmem_ld_wait();
-      pin_32(s[0]);
-      pin_32(s[1]);
-      const bool masked = q0 < warp_key_last || q0 + 64 > min_end;
-      const int from = key - q0, to = end - q0;  // columns [from, to) attend this key
-      const float4* lse = reinterpret_cast<const float4*>(row_values + gs * 2 * kTile + 64 * half);
-      uint32_t w[32];
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 x = lse[g * 8 + e / 4];
-          const float xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            s[g][e + u] = __float_as_uint(
-                fast_exp2(fmaf(__uint_as_float(s[g][e + u]), c, FMT == 0 ? p_shift<FMT>() - xs[u] : -xs[u])));
+    int j = 0, count = 0;
+    for (int r = 0; unit >= 0 && ok; ++r) {
+      const int kv_head = unit % p.kv_heads, per_head = tiles_of(entry), n = per_head * group;
+      const int warp_key0 = entry.x + quad * 32, key = warp_key0 + lane;
+      const bool in = key < p.valid;
+      const int end = in ? __ldg(p.end_query + key) : 0;
+      const bool opens = in && __ldg(p.first_key + key) == key;  // its own row attends nothing else
+      const int min_end = __reduce_min_sync(0xffffffffu, end);
+      // fp16: the largest |do| among the rows of all steps sets the factor of dS.
+      float factor = 1.f;
+      if (FMT == 0) {
+        float top = 0.f;
+        for (int i = lane; i < n * 4; i += 32) {
+          const int h = kv_head * group + i / (per_head * 4);
+          top = fmaxf(top, p.do_max[(long(h) * p.pitch + entry.x) / 32 + i % (per_head * 4)]);
         }
-        if (masked) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (32 * g + e < from || 32 * g + e >= to) s[g][e] = 0u;
-        }
-#pragma unroll
-        for (int e = 0; e < 32; e += 2)
-          w[16 * g + e / 2] = pack16<FMT>(__uint_as_float(s[g][e]), __uint_as_float(s[g][e + 1]));
+        factor = power_below_one(warp_max(top));
       }
-      tmem_st_32(ts, w);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
-
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(dp_full, j & 1));
-      if (!ok) break;
-      tc_fence_after();
-      const float4* dl = reinterpret_cast<const float4*>(row_values + gs * 2 * kTile + kTile + 64 * half);
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        uint32_t d[32];
-        tmem_ld_32(tp + 32 * g, d);
+      const float ds_factor = FMT == 0 ? factor * (1.f / 1024.f) : 1.f;
+      const float2 f2 = make_float2(ds_factor, ds_factor);
+      for (int i = 0; i < n; ++i, ++j) {
+        const int gs = j % kDkvGStages;
+        const int q0 = entry.x + (i % per_head) * kTile + 64 * half;  // first query of this half
+        ok = mbar_wait_bounded(&g_full[gs], (j / kDkvGStages) & 1);
+        ok = mbar_wait_bounded(s_full, j & 1) && ok;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const bool masked = q0 < warp_key0 + 31 || q0 + 64 > min_end;
+        const int from = key - q0, upto = end - 1 - q0;  // columns that attend this key
+        const float4* bias = reinterpret_cast<const float4*>(row_values + gs * 2 * kTile + 64 * half);
+        uint32_t s[2][32];
+        tmem_ld_32(ts, s[0]);
+        tmem_ld_32(ts + 32, s[1]);
         tmem_ld_wait();
-        pin_32(d);
-        float x[32];
+        pin_32(s[0]);
+        pin_32(s[1]);
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 y = dl[g * 8 + e / 4];
-          const float ys[4] = {y.x, y.y, y.z, y.w};
+        for (int g = 0; g < 2; ++g) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            x[e + u] = __uint_as_float(s[g][e + u]) * (__uint_as_float(d[e + u]) - ys[u]);
-            if (FMT == 0) x[e + u] *= ds_factor;
+          for (int e = 0; e < 32; e += 4) {
+            const float4 x = bias[g * 8 + e / 4];
+            prob_pair(s[g][e], s[g][e + 1], c2, make_float2(x.x, x.y));
+            prob_pair(s[g][e + 2], s[g][e + 3], c2, make_float2(x.z, x.w));
           }
+          if (masked) hide(s[g], bit_range(from - 32 * g, upto - 32 * g), 0u);
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = pack16<FMT>(__uint_as_float(s[g][2 * e]), __uint_as_float(s[g][2 * e + 1]));
+          tmem_st_16(ts + 16 * g, w);
         }
-        if (masked) {
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full);
+
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(dp_full, j & 1));
+        if (!ok) break;
+        tc_fence_after();
+        const float4* dl = reinterpret_cast<const float4*>(row_values + gs * 2 * kTile + kTile + 64 * half);
+        uint32_t d[2][32];
+        tmem_ld_32(tp, d[0]);
+        tmem_ld_32(tp + 32, d[1]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          pin_32(d[g]);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 y = dl[g * 8 + e / 4];
+            const float2 x0 = score_gradient<FMT>(s[g][e], s[g][e + 1], d[g][e], d[g][e + 1], make_float2(y.x, y.y), f2);
+            const float2 x1 = score_gradient<FMT>(s[g][e + 2], s[g][e + 3], d[g][e + 2], d[g][e + 3], make_float2(y.z, y.w), f2);
+            d[g][e] = __float_as_uint(x0.x);
+            d[g][e + 1] = __float_as_uint(x0.y);
+            d[g][e + 2] = __float_as_uint(x1.x);
+            d[g][e + 3] = __float_as_uint(x1.y);
+          }
           // what is masked may be infinite or NaN; the first row of a document has a single key
+          if (masked) hide(d[g], bit_range(from + opens - 32 * g, upto - 32 * g), 0u);
+          uint32_t w[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (32 * g + e < from || 32 * g + e >= to || (opens && 32 * g + e == from)) x[e] = 0.f;
+          for (int e = 0; e < 16; ++e) w[e] = pack16<FMT>(__uint_as_float(d[g][2 * e]), __uint_as_float(d[g][2 * e + 1]));
+          tmem_st_16(tp + 16 * g, w);
         }
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) w[16 * g + e / 2] = pack16<FMT>(x[e], x[e + 1]);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(ds_full);
+          mbar_arrive(&g_empty[gs]);  // bias2 and delta are read
+        }
       }
-      tmem_st_32(tp, w);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(ds_full);
-        mbar_arrive(&g_empty[gs]);  // lse2 and delta are read
+      if (!ok) break;
+      // the next unit, under what is left of this one
+      unit = nth_unit(r + 1, p.units);
+      if (unit >= 0) entry = __ldg(p.tiles + unit / p.kv_heads);
+      T* dst = static_cast<T*>(half ? p.dk : p.dv) + (long(key) * p.kv_heads + kv_head) * p.dim;
+      if (n > 0) {
+        const int slot = count & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&checked[slot], (count >> 1) & 1));
+        const bool exact = (poison[2 * slot] | poison[2 * slot + 1]) != 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&seen[slot]);
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(done, count & 1)) && ok;
+        ++count;
+        if (!ok) break;
+        tc_fence_after();
+        const float out = half ? p.scale / factor : (FMT == 0 ? 1.f / 1024.f : 1.f);
+        if (!exact) store_row<FMT, DP>((half ? tmem_dk : tmem_dv) + lane_base, out, dst, p.dim, in);
+        // both halves share the rows: even ones here, odd ones there
+        for (int rr = half; exact && rr < 32; rr += 2)
+          if (warp_key0 + rr < p.valid) exact_dkv_row<FMT, DP>(p, warp_key0 + rr, kv_head, lane);
+        tc_fence_before();
       }
+      if (!in && key < p.rows)
+        for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
     }
-    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(done, 0));
-    ok = __all_sync(0xffffffffu, mbar_wait_bounded(checked, 0)) && ok;
     if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutEpilogue);
-    tc_fence_after();
-    const long at = (long(key) * p.kv_heads + kv_head) * p.dim;
-    T* dst = static_cast<T*>(half ? p.dk : p.dv) + at;
-    const bool exact = *reinterpret_cast<volatile int*>(poison) != 0;
-    if (n > 0 && ok) {
-      const float factor_out = half ? p.scale / factor : (FMT == 0 ? 1.f / 1024.f : 1.f);
-      if (!exact) store_row<FMT, DP>((half ? tmem_dk : tmem_dv) + lane_base, factor_out, dst, p.dim, in);
-      // both halves share the rows: even ones here, odd ones there
-      for (int r = half; exact && r < 32; r += 2)
-        if (k0 + quad * 32 + r < p.valid) exact_dkv_row<FMT, DP>(p, k0 + quad * 32 + r, kv_head, lane);
-    }
-    if (!in && key < p.rows)
-      for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
   }
 
   tc_fence_before();

@@ -2,19 +2,24 @@
 //
 //   S = q k^T,  P = 2^(c S - c m),  O = sum P v / sum P        (c = scale * log2 e, m: running maximum)
 //
-// A block works on two tiles of 128 query rows at once, so that the softmax of one runs under the
-// products of the other: two heads of a group at the same rows (they share every key tile), or, where
-// a group has an odd number of heads, two neighbouring row tiles of a head.  Tiles are cut from the
-// packed axis without regard to documents; a tile of rows [r, r + 128) visits the keys from the first
-// key of row r to its last row, and each row masks its own range [first_key, row].  Short documents
-// so share tiles, and nothing depends on how documents lie in them.
+// One block per SM works through its share of the units.  A unit is two tiles of 128 query rows, so
+// that the softmax of one runs under the products of the other: two heads of a group at the same
+// rows (they share every key tile), or, where a group has an odd number of heads, two neighbouring row
+// tiles of a head.  Tiles are cut from the packed axis without regard to documents; a tile of rows
+// [r, r + 128) visits the keys from the first key of row r to its last row, and each row masks its own
+// range [first_key, row].  Short documents so share tiles, and nothing depends on how they lie.
 //
 // TMEM (512 columns): S of the two tiles (128 each, P in 16 bits over the first half of the same
 // columns: the A operand of the second product) and O of the two (up to 128 each).
 //
-// Warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread has a row), 8 TMA, 9 MMA, 10-11 look for
-// infinities and NaN in value tiles that are partly masked: 0 * NaN would carry them into rows that
-// do not attend them.  If there are any, the block's rows are computed again, row by row.
+// Warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread has a row), 8 TMA, 9 and 10 MMA of tile 0 and 1,
+// 11 looks for infinities and NaN in value tiles that are partly masked: 0 * NaN would carry them into
+// rows that do not attend them.  If there are any, the unit's rows are computed again, row by row.
+//
+// What bounds it: a tile of 128 x 128 scores takes 1024 cycles of the tensor core at 128 features and
+// 1024 of the exponential unit, in a chain that the two tiles fill alternately.  So the chain is kept
+// short (the second product starts on the first half of the keys; skipped chunks where a warp's rows
+// attend nothing; packed fp32 arithmetic) and a quarter of the exponentials goes to the FMA units.
 //
 // O is rescaled only when a row's maximum grew by more than 2^8 since the last time (P then stays
 // below 2^8, which fp16 holds): the final division by the sum makes any base right.
@@ -37,35 +42,66 @@ constexpr int fwd_smem_bytes() {
 
 struct PackedFwdArgs {
   const int* first_key;
-  const int* order;  // tiles (head pairs) or pairs of tiles, most keys first
+  const int4* tiles;  // query_tiles (head pairs) or query_pairs
+  int units;          // what the blocks share out: tiles x head pairs, or pairs of tiles x heads
   int rows, valid, heads, kv_heads, dim;
-  int pitch;       // floats between the heads of lse2
-  int head_pairs;  // 1: a block takes two heads of a group; 0: two row tiles of a head
+  int pitch;       // floats between the heads of bias2
+  int head_pairs;  // 1: a unit is two heads of a group at one tile; 0: two row tiles of a head
   float scale;
   const void *q, *k, *v;  // for the exact recomputation
   long q_tok, q_head, k_tok, k_head, v_tok, v_head;
   void* o;
-  float* lse2;
+  float* bias2;
 };
 
-// Key range of the rows [r0, r0 + 128): empty where hi <= lo.
-struct KeyRange {
-  int lo, hi;
-  int last_first;  // first key of the last row: from there on every row may attend
+// The r-th unit of a block, -1 behind the last: units come most work first, so the blocks take them in
+// rounds of alternating direction, which evens out what they get.
+__device__ __forceinline__ int nth_unit(int r, int units) {
+  const int g = gridDim.x;
+  const int u = r * g + ((r & 1) ? g - 1 - int(blockIdx.x) : int(blockIdx.x));
+  return u < units ? u : -1;
+}
+
+struct QueryUnit {
+  int row0[2], head[2], last_first[2];
+  int i0[2], i1[2];  // key tiles of each, counted from `base` in steps of 128
+  int base, n, kv_head;
 };
 
-__device__ __forceinline__ KeyRange key_range(const int* first_key, int r0, int valid) {
-  KeyRange k = {0, 0, 0};
-  if (r0 < valid) {
-    k.hi = min(r0 + kTile, valid);
-    k.lo = __ldg(first_key + r0);
-    k.last_first = __ldg(first_key + k.hi - 1);
+// The tile entries of a unit (most of a trip to L2: asked for one unit ahead).
+__device__ __forceinline__ void fetch_unit(const int4* tiles, int head_pairs, int heads, int u, int4 (&e)[2]) {
+  if (u < 0) return;
+  if (head_pairs) {
+    e[0] = e[1] = __ldg(tiles + u / (heads / 2));
+  } else {
+    e[0] = __ldg(tiles + 2 * (u / heads));
+    e[1] = __ldg(tiles + 2 * (u / heads) + 1);
   }
-  return k;
+}
+
+__device__ __forceinline__ QueryUnit query_unit(const int4 (&e)[2], int head_pairs, int heads, int kv_heads, int u) {
+  QueryUnit w;
+  const int h = head_pairs ? 2 * (u % (heads / 2)) : u % heads;
+  w.head[0] = h;
+  w.head[1] = head_pairs ? h + 1 : h;
+  w.kv_head = h / (heads / kv_heads);
+  const bool some0 = e[0].w > e[0].y, some1 = e[1].w > e[1].y;
+  // The second tile never begins before the first one does, and is empty if that is.
+  w.base = e[0].y;
+  w.row0[0] = e[0].x;
+  w.row0[1] = e[1].x;
+  w.last_first[0] = e[0].z;
+  w.last_first[1] = e[1].z;
+  w.i0[0] = 0;
+  w.i1[0] = some0 ? (e[0].w - w.base + kTile - 1) / kTile : 0;
+  w.i0[1] = some1 ? (e[1].y - w.base) / kTile : 0;
+  w.i1[1] = some1 ? (e[1].w - w.base + kTile - 1) / kTile : 0;
+  w.n = max(w.i1[0], w.i1[1]);
+  return w;
 }
 
 template <int FMT, int DP>
-__device__ __noinline__ void exact_forward_row(const PackedFwdArgs& p, int row, int head, float lse2, int lane) {
+__device__ __noinline__ void exact_forward_row(const PackedFwdArgs& p, int row, int head, float bias2, int lane) {
   using T = typename Type16<FMT>::T;
   const int kv = head / (p.heads / p.kv_heads);
   const float c = p.scale * kPackedLog2e;
@@ -75,7 +111,7 @@ __device__ __noinline__ void exact_forward_row(const PackedFwdArgs& p, int row, 
     float k[DP / 32], v[DP / 32];
     load_row<FMT, DP>(k, p.k, long(j) * p.k_tok + long(kv) * p.k_head, p.dim, lane);
     load_row<FMT, DP>(v, p.v, long(j) * p.v_tok + long(kv) * p.v_head, p.dim, lane);
-    const float w = exp2f(warp_dot(q, k) * c - lse2);
+    const float w = exp2f(warp_dot(q, k) * c + (bias2 - p_shift<FMT>()));
 #pragma unroll
     for (int e = 0; e < DP / 32; ++e) o[e] = fmaf(w, v[e], o[e]);
   }
@@ -84,6 +120,108 @@ __device__ __noinline__ void exact_forward_row(const PackedFwdArgs& p, int row, 
   for (int e = 0; e < DP / 32; ++e)
     if (lane + 32 * e < p.dim) dst[lane + 32 * e] = from_float<T>(o[e]);
 }
+
+// Largest of 32 values and `top`.
+__device__ __forceinline__ float max_chunk(const uint32_t (&s)[32], float top) {
+  float a = __uint_as_float(s[0]), b = __uint_as_float(s[1]);
+#pragma unroll
+  for (int e = 2; e < 30; e += 4) {
+    a = max3(a, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+    b = max3(b, __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
+  }
+  a = max3(a, __uint_as_float(s[30]), __uint_as_float(s[31]));
+  return max3(top, a, b);
+}
+
+// P = 2^(c s - mc) of 32 columns, in 16 bits to TMEM; their sum is added to `sum`.
+template <int FMT>
+__device__ __forceinline__ void exp_chunk(uint32_t tmem, const uint32_t (&s)[32], float c, float mc, float2 (&sum)[2]) {
+  const float2 c2 = make_float2(c, c), m2 = make_float2(-mc, -mc);
+  uint32_t w[16];
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) {
+    const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, m2);
+    const float2 p = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+    sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], p);
+    w[e / 2] = pack16<FMT>(p.x, p.y);
+  }
+  tmem_st_16(tmem, w);
+}
+
+// The MMA warp of one of the two tiles.
+template <int FMT, int DP>
+struct FwdMma {
+  static_assert(kFwdStages == 2, "stages are addressed by the lowest bit of the step");
+  uint32_t tmem_s, tmem_o;
+  uint64_t q, k, v;  // descriptors; of stage 0 for k and v
+  uint64_t *k_full, *k_empty, *v_full, *v_empty, *q_full, *q_empty, *s_full, *p_full, *o_full;
+  uint32_t j = 0;  // key tiles so far
+  uint32_t steps = 0, uses = 0;
+  static constexpr uint64_t kStage = tile_bytes<DP>() >> 4;
+
+  __device__ __forceinline__ bool scores(uint32_t jj) {
+    constexpr uint32_t idesc = make_idesc_f16(kTile, kTile, FMT, 0, 0);
+    if (!warp_wait(&k_full[jj & 1], (jj >> 1) & 1)) return false;
+    tc_fence_after();
+    const uint64_t b = k + (jj & 1) * kStage;
+    if (elect_one()) {
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) {
+        const uint64_t off = uint64_t(((i / 4) * kSlabBytes + (i % 4) * 32) >> 4);
+        umma_f16(tmem_s, q + off, b + off, idesc, i > 0 ? 1u : 0u);
+      }
+      umma_commit(s_full);
+      umma_commit(&k_empty[jj & 1]);
+    }
+    __syncwarp();
+    return true;
+  }
+  __device__ __forceinline__ bool output(uint32_t jj, bool first) {
+    constexpr uint32_t idesc = make_idesc_f16(kTile, DP, FMT, 0, 1);
+    if (!warp_wait(&v_full[jj & 1], (jj >> 1) & 1)) return false;
+    const uint64_t b = v + (jj & 1) * kStage;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (!warp_wait(&p_full[half], steps & 1)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int i = 4 * half; i < 4 * half + 4; ++i)
+          umma_f16_ts(tmem_o, tmem_s + 8 * i, b + uint64_t((2048 * i) >> 4), idesc, (!first || i > 0) ? 1u : 0u);
+        if (half == 1) umma_commit(&v_empty[jj & 1]);
+      }
+      __syncwarp();
+    }
+    ++steps;
+    return true;
+  }
+  // Key tiles that only the other tile needs are handed back at once.
+  __device__ __forceinline__ bool pass(uint32_t from, uint32_t to) {
+    for (uint32_t jj = from; jj < to; ++jj) {
+      if (!warp_wait(&k_full[jj & 1], (jj >> 1) & 1)) return false;
+      if (elect_one()) mbar_arrive(&k_empty[jj & 1]);
+      if (!warp_wait(&v_full[jj & 1], (jj >> 1) & 1)) return false;
+      if (elect_one()) mbar_arrive(&v_empty[jj & 1]);
+      __syncwarp();
+    }
+    return true;
+  }
+  // S of the first key tile, then by turns O of a tile and S of the next.
+  __device__ __forceinline__ bool unit(int i0, int i1, int n) {
+    const uint32_t begin = j, end = j + n;
+    j = end;
+    if (i1 <= i0) return pass(begin, end);
+    const uint32_t a = begin + i0, z = begin + i1;
+    if (!pass(begin, a) || !warp_wait(q_full, uses & 1) || !scores(a)) return false;
+    ++uses;
+    for (uint32_t jj = a; jj + 1 < z; ++jj)
+      if (!output(jj, jj == a) || !scores(jj + 1)) return false;
+    if (elect_one()) umma_commit(q_empty);
+    if (!output(z - 1, z - 1 == a)) return false;
+    if (elect_one()) umma_commit(o_full);
+    return pass(z, end);
+  }
+};
 
 template <int FMT, int DP>
 __global__ void __launch_bounds__(kFwdThreads, 1)
@@ -96,65 +234,41 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint8_t* k_tiles = q_tiles + 2 * kTileBytes;
   uint8_t* v_tiles = k_tiles + kFwdStages * kTileBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(v_tiles + kFwdStages * kTileBytes);
-  uint64_t* q_full = bars;                     // [2]
-  uint64_t* k_full = q_full + 2;               // [stages]
+  uint64_t* q_full = bars;                  // [2] per tile
+  uint64_t* q_empty = q_full + 2;           // [2]
+  uint64_t* k_full = q_empty + 2;           // [stages]
   uint64_t* k_empty = k_full + kFwdStages;
   uint64_t* v_full = k_empty + kFwdStages;
   uint64_t* v_empty = v_full + kFwdStages;
-  uint64_t* s_full = v_empty + kFwdStages;     // [2]
-  uint64_t* p_full = s_full + 2;               // [2]
-  uint64_t* o_full = p_full + 2;               // [2]
-  uint64_t* checked = o_full + 2;              // [1]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(checked + 1);
-  int* poison = reinterpret_cast<int*>(tmem_slot + 1);
+  uint64_t* s_full = v_empty + kFwdStages;  // [2] per tile
+  uint64_t* p_full = s_full + 2;            // [2][2]: tile, half of the keys
+  uint64_t* turn_over = p_full + 4;         // [2]
+  uint64_t* o_full = turn_over + 2;         // [2]
+  uint64_t* checked = o_full + 2;           // [2]: units in turn
+  uint64_t* seen = checked + 2;             // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(seen + 2);
+  int* poison = reinterpret_cast<int*>(tmem_slot + 1);  // [2]: units in turn
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  // This block's two tiles.
-  int row0[2], head[2];
-  {
-    const int per = p.head_pairs ? p.heads / 2 : p.heads;
-    const int slot = __ldg(p.order + blockIdx.x / per), h = blockIdx.x % per;
-    if (p.head_pairs) {
-      row0[0] = row0[1] = slot * kTile;
-      head[0] = 2 * h;
-      head[1] = 2 * h + 1;
-    } else {
-      row0[0] = 2 * slot * kTile;
-      row0[1] = row0[0] + kTile;
-      head[0] = head[1] = h;
-    }
-  }
-  const int kv_head = head[0] / (p.heads / p.kv_heads);
-  KeyRange range[2] = {key_range(p.first_key, row0[0], p.valid), key_range(p.first_key, row0[1], p.valid)};
-  // Key tiles are counted from the lower of the two first keys; [i0, i1) are the ones a tile needs.
-  const bool some0 = range[0].hi > range[0].lo, some1 = range[1].hi > range[1].lo;
-  const int base = some0 ? (some1 ? min(range[0].lo, range[1].lo) : range[0].lo) : range[1].lo;
-  int i0[2], i1[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const bool some = t ? some1 : some0;
-    i0[t] = some ? (range[t].lo - base) / kTile : 0;
-    i1[t] = some ? (range[t].hi - base + kTile - 1) / kTile : 0;
-  }
-  const int n = max(i1[0], i1[1]);
-  const int begin = some0 && some1 ? min(i0[0], i0[1]) : (some0 ? i0[0] : i0[1]);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kFwdStages; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_empty[s], 2);  // the MMA warps
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 3);  // the MMA warp's commit and the two looking warps
+      mbar_init(&v_empty[s], 3);  // the MMA warps and the looking warp
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
+      mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
+      mbar_init(&p_full[2 * t], 4);
+      mbar_init(&p_full[2 * t + 1], 4);
+      mbar_init(&turn_over[t], 4);
       mbar_init(&o_full[t], 1);
+      mbar_init(&checked[t], 1);
+      mbar_init(&seen[t], 8);
     }
-    mbar_init(checked, 2);
-    *poison = 0;
     fence_barrier_init();
     tma_prefetch_desc(&map_q);
     tma_prefetch_desc(&map_k);
@@ -168,37 +282,52 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t tmem_s[2] = {tmem, tmem + 128}, tmem_o[2] = {tmem + 256, tmem + 384};
+  const uint32_t tmem_s = tmem, tmem_o = tmem + 256;  // 128 columns each per tile
+
+  // Every role goes through the block's units on its own; the barriers keep counting.
+  int4 entry[2], next[2];
+  int unit = nth_unit(0, p.units);
+  fetch_unit(p.tiles, p.head_pairs, p.heads, unit, entry);
 
   if (warp >= 8) {
-    // 168 registers a thread at launch: 3 * 168 >= 2 * 208 + 80
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == 8) {
-      if (lane == 0 && n > 0) {
+      if (lane == 0) {
         bool ok = true;
-        for (int t = 0; t < 2; ++t) {
-          if (i1[t] == 0) continue;
-          mbar_expect_tx(&q_full[t], kTileBytes);
+        int j = 0, uses[2] = {0, 0};
+        for (int r = 0; unit >= 0 && ok; ++r) {
+          const int after = nth_unit(r + 1, p.units);
+          fetch_unit(p.tiles, p.head_pairs, p.heads, after, next);
+          const QueryUnit u = query_unit(entry, p.head_pairs, p.heads, p.kv_heads, unit);
+          for (int i = 0; i < u.n && ok; ++i, ++j) {
+            const int st = j % kFwdStages;
+            const uint32_t parity = ((j / kFwdStages) & 1) ^ 1;
+            const int key = u.base + i * kTile;
+            ok = mbar_wait_bounded(&k_empty[st], parity);
+            if (!ok) break;
+            mbar_expect_tx(&k_full[st], kTileBytes);
 #pragma unroll
-          for (int s = 0; s < kSlabs; ++s)
-            tma_load_3d(q_tiles + t * kTileBytes + s * kSlabBytes, &map_q, &q_full[t], 64 * s, head[t], row0[t]);
-        }
-        for (int i = begin, j = 0; i < n && ok; ++i, ++j) {
-          const int st = j % kFwdStages;
-          const uint32_t parity = ((j / kFwdStages) & 1) ^ 1;
-          const int key = base + i * kTile;
-          ok = mbar_wait_bounded(&k_empty[st], parity);
-          if (!ok) break;
-          mbar_expect_tx(&k_full[st], kTileBytes);
+            for (int s = 0; s < kSlabs; ++s)
+              tma_load_3d(k_tiles + st * kTileBytes + s * kSlabBytes, &map_k, &k_full[st], 64 * s, u.kv_head, key);
+            for (int t = 0; t < 2 && i == 0 && ok; ++t) {
+              if (u.i1[t] == 0) continue;
+              ok = mbar_wait_bounded(&q_empty[t], (uses[t] & 1) ^ 1);
+              if (!ok) break;
+              ++uses[t];
+              mbar_expect_tx(&q_full[t], kTileBytes);
 #pragma unroll
-          for (int s = 0; s < kSlabs; ++s)
-            tma_load_3d(k_tiles + st * kTileBytes + s * kSlabBytes, &map_k, &k_full[st], 64 * s, kv_head, key);
-          ok = mbar_wait_bounded(&v_empty[st], parity);
-          if (!ok) break;
-          mbar_expect_tx(&v_full[st], kTileBytes);
+              for (int s = 0; s < kSlabs; ++s)
+                tma_load_3d(q_tiles + t * kTileBytes + s * kSlabBytes, &map_q, &q_full[t], 64 * s, u.head[t], u.row0[t]);
+            }
+            ok = ok && mbar_wait_bounded(&v_empty[st], parity);
+            if (!ok) break;
+            mbar_expect_tx(&v_full[st], kTileBytes);
 #pragma unroll
-          for (int s = 0; s < kSlabs; ++s)
-            tma_load_3d(v_tiles + st * kTileBytes + s * kSlabBytes, &map_v, &v_full[st], 64 * s, kv_head, key);
+            for (int s = 0; s < kSlabs; ++s)
+              tma_load_3d(v_tiles + st * kTileBytes + s * kSlabBytes, &map_v, &v_full[st], 64 * s, u.kv_head, key);
+          }
+          unit = after;
+          entry[0] = next[0];
+          entry[1] = next[1];
         }
         if (!ok) {
           atomicCAS(status, kStatusOk, kStatusTimeoutProducer);
@@ -206,190 +335,215 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
       }
       __syncwarp();
-    } else if (warp == 9) {
-      constexpr uint32_t idesc_s = make_idesc_f16(kTile, kTile, FMT, 0, 0);
-      constexpr uint32_t idesc_o = make_idesc_f16(kTile, DP, FMT, 0, 1);
-      if (lane == 0 && n > 0) {
-        bool ok = true;
-        // Step i: for each tile the second product of key tile i - 1, then the first product of i.
-        for (int i = begin, j = 0; i <= n && ok; ++i, ++j) {
-          const int st = j % kFwdStages, pst = (j + kFwdStages - 1) % kFwdStages;  // stages of i and i - 1
-          bool k_there = false, v_there = false;
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (i - 1 >= i0[t] && i - 1 < i1[t]) {
-              if (!v_there) {
-                ok = mbar_wait_bounded(&v_full[pst], ((j - 1) / kFwdStages) & 1);
-                v_there = true;
-              }
-              ok = ok && mbar_wait_bounded(&p_full[t], (i - 1 - i0[t]) & 1);
-              if (!ok) break;
-              tc_fence_after();
-              const uint64_t dv = make_mnmajor_sw128_desc(smem_u32(v_tiles + pst * kTileBytes), kSlabBytes);
-#pragma unroll
-              for (int k = 0; k < kTile / 16; ++k)
-                umma_f16_ts(tmem_o[t], tmem_s[t] + 8 * k, dv + uint64_t((2048 * k) >> 4), idesc_o,
-                            (i - 1 > i0[t] || k > 0) ? 1u : 0u);
-              if (i == i1[t]) umma_commit(&o_full[t]);
-            }
-            if (i >= i0[t] && i < i1[t]) {
-              if (!k_there) {
-                ok = mbar_wait_bounded(&k_full[st], (j / kFwdStages) & 1);
-                k_there = true;
-              }
-              if (i == i0[t]) ok = ok && mbar_wait_bounded(&q_full[t], 0);
-              if (!ok) break;
-              tc_fence_after();
-              const uint64_t dq = make_kmajor_sw128_desc(smem_u32(q_tiles + t * kTileBytes));
-              const uint64_t dk = make_kmajor_sw128_desc(smem_u32(k_tiles + st * kTileBytes));
-#pragma unroll
-              for (int k = 0; k < DP / 16; ++k) {
-                const uint64_t off = uint64_t(((k / 4) * kSlabBytes + (k % 4) * 32) >> 4);
-                umma_f16(tmem_s[t], dq + off, dk + off, idesc_s, k > 0 ? 1u : 0u);
-              }
-              umma_commit(&s_full[t]);
-            }
-          }
-          if (ok) {
-            // A stage that no tile needed is handed back the same way.
-            if (i < n) {
-              if (!k_there) ok = mbar_wait_bounded(&k_full[st], (j / kFwdStages) & 1);
-              umma_commit(&k_empty[st]);
-            }
-            if (i > begin) {
-              if (!v_there) ok = ok && mbar_wait_bounded(&v_full[pst], ((j - 1) / kFwdStages) & 1);
-              umma_commit(&v_empty[pst]);
-            }
-          }
+    } else if (warp < 11) {
+      const int t = warp - 9;
+      FwdMma<FMT, DP> mma;
+      mma.tmem_s = tmem_s + 128 * t;
+      mma.tmem_o = tmem_o + 128 * t;
+      mma.q = make_kmajor_sw128_desc(smem_u32(q_tiles + t * kTileBytes));
+      mma.k = make_kmajor_sw128_desc(smem_u32(k_tiles));
+      mma.v = make_mnmajor_sw128_desc(smem_u32(v_tiles), kSlabBytes);
+      mma.k_full = k_full;
+      mma.k_empty = k_empty;
+      mma.v_full = v_full;
+      mma.v_empty = v_empty;
+      mma.q_full = &q_full[t];
+      mma.q_empty = &q_empty[t];
+      mma.s_full = &s_full[t];
+      mma.p_full = &p_full[2 * t];
+      mma.o_full = &o_full[t];
+      bool ok = true;
+      for (int r = 0; unit >= 0 && ok; ++r) {
+        const int after = nth_unit(r + 1, p.units);
+        fetch_unit(p.tiles, p.head_pairs, p.heads, after, next);
+        int i0, i1, n;
+        {
+          const QueryUnit u = query_unit(entry, p.head_pairs, p.heads, p.kv_heads, unit);
+          i0 = t ? u.i0[1] : u.i0[0];
+          i1 = t ? u.i1[1] : u.i1[0];
+          n = u.n;
         }
-        if (!ok) atomicCAS(status, kStatusOk, kStatusTimeoutMma);
+        ok = mma.unit(i0, i1, n);
+        unit = after;
+        entry[0] = next[0];
+        entry[1] = next[1];
       }
-      __syncwarp();
+      if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutMma);
     } else {
-      bool bad = false, ok = true;
-      for (int i = begin, j = 0; i < n && ok; ++i, ++j) {
-        const int st = j % kFwdStages;
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&v_full[st], (j / kFwdStages) & 1));
-        const int key = base + i * kTile;
-        bool masked = false;
+      bool ok = true;
+      int j = 0, count = 0;
+      for (int r = 0; unit >= 0 && ok; ++r) {
+        const int after = nth_unit(r + 1, p.units);
+        fetch_unit(p.tiles, p.head_pairs, p.heads, after, next);
+        const QueryUnit u = query_unit(entry, p.head_pairs, p.heads, p.kv_heads, unit);
+        bool bad = false;
+        for (int i = 0; i < u.n && ok; ++i, ++j) {
+          const int st = j % kFwdStages;
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&v_full[st], (j / kFwdStages) & 1));
+          const int key = u.base + i * kTile;
+          bool masked = false;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          masked |= i >= i0[t] && i < i1[t] && (key + kTile - 1 > row0[t] || key < range[t].last_first);
-        if (masked && ok) bad |= scan_not_finite<FMT>(v_tiles + st * kTileBytes, kTileBytes, warp - 10, 2, lane);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_empty[st]);
+          for (int t = 0; t < 2; ++t)
+            masked |= i >= u.i0[t] && i < u.i1[t] && (key + kTile - 1 > u.row0[t] || key < u.last_first[t]);
+          if (masked && ok) bad |= scan_not_finite<FMT>(v_tiles + st * kTileBytes, kTileBytes, 0, 1, lane);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_empty[st]);
+        }
+        if (u.n > 0) {
+          const int slot = count & 1;
+          ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&seen[slot], ((count >> 1) & 1) ^ 1));
+          bad = __any_sync(0xffffffffu, bad);
+          if (lane == 0) {
+            poison[slot] = bad;
+            mbar_arrive(&checked[slot]);
+          }
+          ++count;
+        }
+        unit = after;
+        entry[0] = next[0];
+        entry[1] = next[1];
       }
-      if (__any_sync(0xffffffffu, bad) && lane == 0) *poison = 1;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(checked);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    using T = typename Type16<FMT>::T;
     const int t = warp >> 2, quad = warp & 3;
-    const int my_i0 = t ? i0[1] : i0[0], my_i1 = t ? i1[1] : i1[0];
-    const int r0 = t ? row0[1] : row0[0], my_head = t ? head[1] : head[0];
-    const int row = r0 + quad * 32 + lane;
-    const bool in = row < p.valid;
-    const int first = in ? __ldg(p.first_key + row) : 0x7fffffff;
-    // The warp's rows attend all of a key tile from `all_from` on, up to its first row.
-    const int warp_row0 = r0 + quad * 32;
-    const int all_from = __shfl_sync(0xffffffffu, in ? first : 0x7fffffff, 31);
     const uint32_t lane_base = uint32_t(quad * 32) << 16;
-    const uint32_t ts = (t ? tmem_s[1] : tmem_s[0]) + lane_base, to = (t ? tmem_o[1] : tmem_o[0]) + lane_base;
+    const uint32_t ts = tmem_s + 128 * t + lane_base, to = tmem_o + 128 * t + lane_base;
     const float c = p.scale * kPackedLog2e;
-    float m = -INFINITY, l = 0.f;  // m: the base in use, of the unscaled scores
     bool ok = true;
-    for (int i = my_i0; i < my_i1; ++i) {
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[t], (i - my_i0) & 1));
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) tmem_ld_32(ts + 32 * g, s[g]);
-      tmem_ld_wait();
-#pragma unroll
-      for (int g = 0; g < 4; ++g) pin_32(s[g]);
-      const int key = base + i * kTile;
-      if (key + kTile - 1 > warp_row0 || key < all_from) {
-        const int from = first - key, to_ = row - key;  // columns of the row's own range
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (32 * g + e < from || 32 * g + e > to_) s[g][e] = 0xff800000u;  // -inf
+    int steps = 0, uses = 0, count = 0, turns = 0;
+    // The two tiles take turns at the exponentials, tile 0 first: left alone they fall into step, and then
+    // nobody computes under the products.  A tile takes its turn at every key tile of the unit, needed
+    // or not, so neither is ever more than one ahead (a barrier tells only two phases apart).
+    const auto my_turn = [&](int turn) {
+      if (t == 0 && turn == 0) return true;
+      return bool(__all_sync(0xffffffffu, mbar_wait_bounded(&turn_over[1 - t], (t ? turn : turn - 1) & 1)));
+    };
+    for (int r = 0; unit >= 0 && ok; ++r) {
+      int i0, i1, warp_row0, head, base, n;
+      {
+        const QueryUnit u = query_unit(entry, p.head_pairs, p.heads, p.kv_heads, unit);
+        i0 = t ? u.i0[1] : u.i0[0];
+        i1 = t ? u.i1[1] : u.i1[0];
+        warp_row0 = (t ? u.row0[1] : u.row0[0]) + quad * 32;
+        head = t ? u.head[1] : u.head[0];
+        base = u.base;
+        n = u.n;
       }
-      float mx[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        mx[g] = __uint_as_float(s[g][0]);
-#pragma unroll
-        for (int e = 1; e < 32; ++e) mx[g] = fmaxf(mx[g], __uint_as_float(s[g][e]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      // A new base where the maximum grew by more than 2^8 (or is the row's first).
-      const bool grow = (top - m) * c > 8.f;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float alpha = grow ? fast_exp2((m - top) * c) : 1.f;
-        if (grow) m = top;
-        l *= alpha;
-        if (i > my_i0) {
+      const int row = warp_row0 + lane;
+      const bool in = row < p.valid;
+      const int first = in ? __ldg(p.first_key + row) : 0x7fffffff;
+      // The warp's rows attend all of a key tile from `all_from` on, up to its first row.
+      const int all_from = __shfl_sync(0xffffffffu, first, 31);
+      float m = -INFINITY, l = 0.f;  // m: the base in use, of the unscaled scores
+      for (int i = 0; i < n; ++i, ++turns) {
+        if (i < i0 || i >= i1) {  // only the other tile needs this key tile
+          ok = my_turn(turns);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive(&turn_over[t]);
+          continue;
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[t], steps & 1));
+        if (!ok) break;
+        tc_fence_after();
+        const int key = base + i * kTile;
+        const bool masked = key + kTile - 1 > warp_row0 || key < all_from;
+        const int from = first - key, upto = row - key;  // columns of the row's own range
+        // The scores are read twice, 32 columns at a time and one chunk ahead: small loops, whose code and
+        // values stay close.
+        uint32_t sa[32], sb[32];
+        tmem_ld_32(ts, sa);
+        float top = -INFINITY;
 #pragma unroll 1
-          for (int d = 0; d < DP; d += 32) {
-            uint32_t o[32];
-            tmem_ld_32(to + d, o);
-            tmem_ld_wait();
-            pin_32(o);
+        for (int g = 0; g < 4; g += 2) {
+          tmem_ld_wait();
+          pin_32(sa);
+          tmem_ld_32(ts + 32 * (g + 1), sb);
+          if (masked) hide(sa, bit_range(from - 32 * g, upto - 32 * g), 0xff800000u);  // -inf
+          top = max_chunk(sa, top);
+          tmem_ld_wait();
+          pin_32(sb);
+          tmem_ld_32(ts + 32 * ((g + 2) & 3), sa);
+          if (masked) hide(sb, bit_range(from - 32 * (g + 1), upto - 32 * (g + 1)), 0xff800000u);
+          top = max_chunk(sb, top);
+        }
+        // A new base where the maximum grew by more than 2^8 (or is the row's first).
+        const bool grow = (top - m) * c > 8.f;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float alpha = grow ? fast_exp2((m - top) * c) : 1.f;
+          if (grow) m = top;
+          l *= alpha;
+          if (i > i0) {
+#pragma unroll 1
+            for (int d = 0; d < DP; d += 16) {
+              float o[16];
+              uint32_t scaled[16];
+              tmem_ld_32x16(to + d, o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st_32(to + d, o);
+              for (int e = 0; e < 16; ++e) scaled[e] = __float_as_uint(o[e] * alpha);
+              tmem_st_16(to + d, scaled);
+            }
           }
         }
-      }
-      const float mc = m == -INFINITY ? 0.f : m * c;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int g = 0; g < 4; g += 2) {
-        uint32_t w[32];
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float a0 = fast_exp2(fmaf(__uint_as_float(s[g][e]), c, -mc));
-          const float a1 = fast_exp2(fmaf(__uint_as_float(s[g][e + 1]), c, -mc));
-          const float b0 = fast_exp2(fmaf(__uint_as_float(s[g + 1][e]), c, -mc));
-          const float b1 = fast_exp2(fmaf(__uint_as_float(s[g + 1][e + 1]), c, -mc));
-          sum[0] += a0;
-          sum[1] += a1;
-          sum[2] += b0;
-          sum[3] += b1;
-          w[e / 2] = pack16<FMT>(a0, a1);
-          w[16 + e / 2] = pack16<FMT>(b0, b1);
+        const float mc = m == -INFINITY ? 0.f : m * c;
+        ok = my_turn(turns);
+        if (!ok) break;
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+        for (int g = 0; g < 4; g += 2) {
+          tmem_ld_wait();
+          pin_32(sa);
+          tmem_ld_32(ts + 32 * (g + 1), sb);
+          if (masked) hide(sa, bit_range(from - 32 * g, upto - 32 * g), 0xff800000u);
+          exp_chunk<FMT>(ts + 16 * g, sa, c, mc, sum);
+          tmem_ld_wait();
+          pin_32(sb);
+          if (g == 0) tmem_ld_32(ts + 64, sa);
+          if (masked) hide(sb, bit_range(from - 32 * (g + 1), upto - 32 * (g + 1)), 0xff800000u);
+          exp_chunk<FMT>(ts + 16 * (g + 1), sb, c, mc, sum);
+          if (g == 2) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&turn_over[t]);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * t + g / 2]);
         }
-        tmem_st_32(ts + 16 * g, w);
+        ++steps;
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t]);
+      if (!ok) break;
+      // the next unit, under what is left of this one
+      unit = nth_unit(r + 1, p.units);
+      fetch_unit(p.tiles, p.head_pairs, p.heads, unit, entry);
+      const bool some = in && first <= row;
+      const float bias2 = some ? p_shift<FMT>() - fmaf(m, c, log2f(l)) : -INFINITY;
+      if (row < p.rows) p.bias2[long(head) * p.pitch + row] = bias2;
+      T* dst = static_cast<T*>(p.o) + (long(row) * p.heads + head) * p.dim;
+      if (n > 0) {
+        const int slot = count & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&checked[slot], (count >> 1) & 1));
+        const bool exact = poison[slot] != 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&seen[slot]);
+        ++count;
+        if (i1 > i0) {
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_full[t], uses & 1)) && ok;
+          ++uses;
+          tc_fence_after();
+          if (ok && !exact) store_row<FMT, DP>(to, some ? 1.f / l : 0.f, dst, p.dim, some);
+          for (int rr = 0; ok && exact && rr < 32; ++rr) {
+            const float bias_r = __shfl_sync(0xffffffffu, bias2, rr);
+            if (__shfl_sync(0xffffffffu, int(some), rr)) exact_forward_row<FMT, DP>(p, warp_row0 + rr, head, bias_r, lane);
+          }
+          tc_fence_before();
+        }
+      }
+      if (!some && row < p.rows)
+        for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
     }
-    if (ok && my_i1 > my_i0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_full[t], 0));
-    ok = __all_sync(0xffffffffu, mbar_wait_bounded(checked, 0)) && ok;
     if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutEpilogue);
-    tc_fence_after();
-    const bool some = in && first <= row;
-    const float lse2 = some ? fmaf(m, c, log2f(l)) : INFINITY;
-    if (row < p.rows) p.lse2[long(my_head) * p.pitch + row] = lse2;
-    using T = typename Type16<FMT>::T;
-    T* dst = static_cast<T*>(p.o) + (long(row) * p.heads + my_head) * p.dim;
-    const bool exact = *reinterpret_cast<volatile int*>(poison) != 0;
-    if (my_i1 > my_i0 && ok) {
-      if (!exact) store_row<FMT, DP>(to, some ? 1.f / l : 0.f, dst, p.dim, some);
-      for (int r = 0; exact && r < 32; ++r) {
-        const int row_r = warp_row0 + r;
-        const float lse_r = __shfl_sync(0xffffffffu, lse2, r);
-        if (__shfl_sync(0xffffffffu, int(some), r)) exact_forward_row<FMT, DP>(p, row_r, my_head, lse_r, lane);
-      }
-    }
-    if (!some && row < p.rows)
-      for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
   }
 
   tc_fence_before();

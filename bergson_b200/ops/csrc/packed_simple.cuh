@@ -103,7 +103,7 @@ __device__ __forceinline__ float half_warp_max(float v) {
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPackedAttention a, T* o, float* lse2) {
+__global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPackedAttention a, T* o, float* bias2) {
   extern __shared__ float smem[];
   float* qs = smem;
   float* ks = qs + DP * kSimplePitch;
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPa
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const int head = blockIdx.x % a.heads, slot = blockIdx.x / a.heads;
   const int kv_head = head / (a.heads / a.kv_heads);
-  const int q0 = (a.query_order[slot / 2] * 2 + (slot & 1)) * kSimpleTile;
+  const int q0 = a.query_tiles[4 * (slot / 2)] + (slot & 1) * kSimpleTile;
   if (q0 >= a.rows) return;
   const float c = a.scale * kLog2e;
 
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPa
     if (row >= a.rows) continue;
     const bool some = row < a.valid && first[i] <= row;
     const float inv = some ? 1.f / l[i] : 0.f;
-    if (tx == 0) lse2[long(head) * a.pitch + row] = some ? m[i] + log2f(l[i]) : INFINITY;
+    if (tx == 0) bias2[long(head) * a.pitch + row] = some ? -(m[i] + log2f(l[i])) : -INFINITY;
     T* dst = o + (long(row) * a.heads + head) * a.dim;
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPa
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kSimpleThreads)
-packed_dq_simple_kernel(BgnPackedAttention a, const T* o, const float* lse2, const T* d_o, long do_tok, long do_head,
+packed_dq_simple_kernel(BgnPackedAttention a, const T* o, const float* bias2, const T* d_o, long do_tok, long do_head,
                         float* delta, T* dq) {
   extern __shared__ float smem[];
   float* qs = smem;
@@ -193,7 +193,7 @@ packed_dq_simple_kernel(BgnPackedAttention a, const T* o, const float* lse2, con
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const int head = blockIdx.x % a.heads, slot = blockIdx.x / a.heads;
   const int kv_head = head / (a.heads / a.kv_heads);
-  const int q0 = (a.query_order[slot / 2] * 2 + (slot & 1)) * kSimpleTile;
+  const int q0 = a.query_tiles[4 * (slot / 2)] + (slot & 1) * kSimpleTile;
   if (q0 >= a.rows) return;
   const float c = a.scale * kLog2e;
 
@@ -201,13 +201,13 @@ packed_dq_simple_kernel(BgnPackedAttention a, const T* o, const float* lse2, con
   simple_load<T, DP>(gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
   __syncthreads();
   int first[4];
-  float lse[4], dl[4], out[4][DP / 16];
+  float bias[4], dl[4], out[4][DP / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = q0 + 4 * ty + i;
     const bool in = row < a.valid;
     first[i] = in ? a.first_key[row] : 0x7fffffff;
-    lse[i] = in ? lse2[long(head) * a.pitch + row] : INFINITY;
+    bias[i] = in ? bias2[long(head) * a.pitch + row] : -INFINITY;
     float sum = 0.f;
     if (in) {
       const T* orow = o + (long(row) * a.heads + head) * a.dim;
@@ -237,7 +237,7 @@ packed_dq_simple_kernel(BgnPackedAttention a, const T* o, const float* lse2, con
         const int key = k0 + 4 * tx + j;
         // A row with one key has P = 1 and no gradient through the softmax: exactly zero.
         const bool in = key >= first[i] && key <= row && first[i] < row;
-        ds[(4 * ty + i) * kSimplePitch + 4 * tx + j] = in ? exp2f(__fmul_rn(s[i][j], c) - lse[i]) * (dp[i][j] - dl[i]) : 0.f;
+        ds[(4 * ty + i) * kSimplePitch + 4 * tx + j] = in ? exp2f(__fmul_rn(s[i][j], c) + bias[i]) * (dp[i][j] - dl[i]) : 0.f;
       }
     }
     __syncthreads();
@@ -256,7 +256,7 @@ packed_dq_simple_kernel(BgnPackedAttention a, const T* o, const float* lse2, con
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kSimpleThreads)
-packed_dkv_simple_kernel(BgnPackedAttention a, const float* lse2, const T* d_o, long do_tok, long do_head,
+packed_dkv_simple_kernel(BgnPackedAttention a, const float* bias2, const T* d_o, long do_tok, long do_head,
                          const float* delta, T* dk, T* dv) {
   extern __shared__ float smem[];
   float* ks = smem;
@@ -267,7 +267,7 @@ packed_dkv_simple_kernel(BgnPackedAttention a, const float* lse2, const T* d_o, 
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const int kv_head = blockIdx.x % a.kv_heads, slot = blockIdx.x / a.kv_heads;
   const int group = a.heads / a.kv_heads;
-  const int k0 = (a.key_order[slot / 2] * 2 + (slot & 1)) * kSimpleTile;
+  const int k0 = a.key_tiles[4 * (slot / 2)] + (slot & 1) * kSimpleTile;
   if (k0 >= a.rows) return;
   const float c = a.scale * kLog2e;
 
@@ -300,13 +300,13 @@ packed_dkv_simple_kernel(BgnPackedAttention a, const float* lse2, const T* d_o, 
       for (int j = 0; j < 4; ++j) {
         const int row = q0 + 4 * tx + j;
         const bool in_row = row < a.valid;
-        const float lse = in_row ? lse2[long(head) * a.pitch + row] : INFINITY;
+        const float bias = in_row ? bias2[long(head) * a.pitch + row] : -INFINITY;
         const float dl = in_row ? delta[long(head) * a.pitch + row] : 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = k0 + 4 * ty + i;
           const bool in = row >= key && row < end[i];
-          const float p = in ? exp2f(__fmul_rn(s[i][j], c) - lse) : 0.f;
+          const float p = in ? exp2f(__fmul_rn(s[i][j], c) + bias) : 0.f;
           s[i][j] = p;
           dp[i][j] = in && own_first[i] < row ? p * (dp[i][j] - dl) : 0.f;
         }

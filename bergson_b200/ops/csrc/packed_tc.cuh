@@ -31,6 +31,27 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
       : "memory");
 }
 
+// One lane of a converged warp, the same one every time.  Code under it is known to run in one thread:
+// the MMA instructions' operands then need no detour through the vector registers, and a warp that
+// issues them next to busy arithmetic warps needs few issue slots (a branch on the lane number took
+// several times as many, and the tensor core went idle).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// All lanes of a warp wait; false if the time ran out.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
+}
+
 // 32 lanes x 32 columns without waiting; tmem_ld_wait() makes the values of all loads before it usable.
 __device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -70,6 +91,16 @@ __device__ __forceinline__ void tmem_st_32(uint32_t taddr, const uint32_t (&r)[3
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+      :
+      : "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Two values rounded to the 16-bit type, the first in the low half.
@@ -88,24 +119,28 @@ struct Type16<0> { using T = __half; };
 template <>
 struct Type16<1> { using T = __nv_bfloat16; };
 
-// Whether one of two packed 16-bit values is infinite or NaN (all exponent bits set): adding the
-// exponent's lowest bit carries into the sign bit.
+// What the forward pass hands to the backward pass: P of a row is 2^(c q.k + bias2), times 2^10 for fp16,
+// whose small values are few (see packed_bwd.cuh).
 template <int FMT>
-__device__ __forceinline__ bool not_finite2(uint32_t u) {
-  return FMT == 1 ? (((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0
-                  : (((u & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0;
+constexpr float p_shift() {
+  return FMT == 0 ? 10.f : 0.f;
 }
 
-// One warp's share of a look through `bytes` of an operand tile in shared memory.
+// One warp's share of a look through `bytes` of an operand tile in shared memory for 16-bit values that
+// are infinite or NaN (all exponent bits set): adding the exponent's lowest bit carries into the sign bit.
 template <int FMT>
 __device__ __forceinline__ bool scan_not_finite(const uint8_t* tile, int bytes, int part, int parts, int lane) {
-  bool bad = false;
-  const uint4* p = reinterpret_cast<const uint4*>(tile);
-  for (int i = part * 32 + lane; i < bytes / 16; i += parts * 32) {
-    const uint4 u = p[i];
-    bad |= not_finite2<FMT>(u.x) || not_finite2<FMT>(u.y) || not_finite2<FMT>(u.z) || not_finite2<FMT>(u.w);
+  // The carries of all values are collected and looked at once.
+  constexpr uint32_t exponent = FMT == 1 ? 0x7f807f80u : 0x7c007c00u, lowest = FMT == 1 ? 0x00800080u : 0x04000400u;
+  uint32_t carry = 0;
+  const uint4* p = reinterpret_cast<const uint4*>(tile) + part * 32 + lane;
+#pragma unroll 8
+  for (int i = 0; i < bytes / 512; i += parts) {
+    const uint4 u = p[i * 32];
+    carry |= ((u.x & exponent) + lowest) | ((u.y & exponent) + lowest) | ((u.z & exponent) + lowest) |
+             ((u.w & exponent) + lowest);
   }
-  return bad;
+  return (carry & 0x80008000u) != 0;
 }
 
 // Features of a row that a lane holds when a warp works on whole rows.
@@ -138,6 +173,47 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;"
+      : "=l"(*reinterpret_cast<uint64_t*>(&d))
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;"
+      : "=l"(*reinterpret_cast<uint64_t*>(&d))
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;"
+      : "=l"(*reinterpret_cast<uint64_t*>(&d))
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.ftz.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Bits lo .. hi (those inside 0 .. 31).
+__device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
+  const int l = lo > 0 ? lo : 0, h = hi < 31 ? hi : 31;
+  return l <= h ? (0xffffffffu << l) & (0xffffffffu >> (31 - h)) : 0u;
+}
+
+// Puts `value` where a bit of `keep` is not set.
+__device__ __forceinline__ void hide(uint32_t (&x)[32], uint32_t keep, uint32_t value) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e)
+    if (!(keep & (1u << e))) x[e] = value;
+}
+
 __device__ __forceinline__ void store_v8(void* ptr, const uint32_t* r) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(ptr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -145,12 +221,12 @@ __device__ __forceinline__ void store_v8(void* ptr, const uint32_t* r) {
 }
 
 // A thread's row of an accumulator in TMEM, scaled, rounded and stored to `dst` (dim features,
-// 16-byte aligned).
+// 16-byte aligned); with `half` 0 or 1 only that half of the features.
 template <int FMT, int DP>
-__device__ __forceinline__ void store_row(uint32_t tmem, float scale, void* dst, int dim, bool write) {
+__device__ __forceinline__ void store_row(uint32_t tmem, float scale, void* dst, int dim, bool write, int half = -1) {
   const bool wide = (dim & 15) == 0;  // every row begins on a 32-byte boundary then
 #pragma unroll 1
-  for (int c = 0; c < DP; c += 32) {
+  for (int c = half == 1 ? DP / 2 : 0; c < (half == 0 ? DP / 2 : DP); c += 32) {
     if (c >= dim) break;
     uint32_t r[32];
     tmem_ld_32(tmem + c, r);

@@ -61,28 +61,42 @@ class PackedSequences:
         first_key[:valid] = np.repeat(begins, lens)
         end_query[:valid] = np.repeat(ends, lens)
         position[:valid] = at[:valid] - first_key[:valid]
-        # Tiles by their work, most first: blocks are dealt in this order, and a long tile that starts
-        # last would be waited for.
-        head = np.arange(0, rows, _TILE)
-        last = np.minimum(head + _TILE, rows) - 1
-        query_work = np.minimum(last + 1, valid) - first_key[head] if rows else head
-        key_work = np.minimum(end_query[last], valid) - head if rows else head
-        query_order = np.argsort(-query_work, kind="stable")
-        key_order = np.argsort(-key_work, kind="stable")
-        pair = np.maximum(np.append(query_work, -1)[1::2], query_work[::2])[: -(-len(head) // 2)]
-        query_pair_order = np.argsort(-pair, kind="stable")
-        parts = [first_key, end_query, position, query_order, query_pair_order, key_order, np.concatenate([[0], ends])]
-        table = torch.from_numpy(np.concatenate(parts).astype(np.int32)).to(device)
+        # Tiles of 128 rows with what their blocks need to know, by their work, most first: blocks are dealt
+        # in this order, and a long tile that starts last would be waited for.
+        row0 = np.arange(0, rows, _TILE)
+        end = np.minimum(row0 + _TILE, valid)
+        some = end > row0
+        first = np.minimum(row0, max(valid - 1, 0))
+        last = np.maximum(end - 1, 0)
+        query = np.zeros((len(row0), 4), np.int64)  # first row, first key of it, first key of the last row, last key + 1
+        query[:, 0] = row0
+        key = np.zeros((len(row0), 4), np.int64)  # first key, last query + 1, the same of the first key alone
+        key[:, 0] = key[:, 1] = row0
+        if valid:
+            query[some, 1:] = np.stack([first_key[first], first_key[last], end], 1)[some]
+            key[some, 1:3] = np.stack([end_query[last], end_query[first]], 1)[some]
+        work = query[:, 3] - query[:, 1]
+        if len(row0) % 2:  # pairs of neighbouring tiles: the last one alone has an empty second
+            query = np.concatenate([query, [[rows + _TILE, 0, 0, 0]]])
+            pair_work = np.append(work, 0)
+        else:
+            pair_work = work
+        pairs = query.reshape(-1, 8)[np.argsort(-pair_work.reshape(-1, 2).max(1), kind="stable")]
+        query = query[np.argsort(-work, kind="stable")]
+        key = key[np.argsort(-(key[:, 1] - key[:, 0]), kind="stable")]
+        parts = [query, pairs, key, first_key, end_query, position, np.concatenate([[0], ends])]
+        flat = np.concatenate([x.reshape(-1) for x in parts]).astype(np.int32)
+        table = torch.from_numpy(flat).to(device)
         self.device = table.device
-        (self.first_key, self.end_query, self.position, self.query_order, self.query_pair_order,
-         self.key_order, self.cu_seqlens) = table.split([len(p) for p in parts])
+        (self.query_tiles, self.query_pairs, self.key_tiles, self.first_key, self.end_query, self.position,
+         self.cu_seqlens) = table.split([x.size for x in parts])
 
     def __repr__(self) -> str:
         return f"PackedSequences({len(self.lengths)} documents, {self.num_tokens} tokens, {self.rows} rows)"
 
     def tables(self):
         """What the attention kernels read of the plan."""
-        return self.first_key, self.end_query, self.query_order, self.query_pair_order, self.key_order
+        return self.first_key, self.end_query, self.query_tiles, self.query_pairs, self.key_tiles
 
     def spans(self):
         """(begin, end) of each document that has tokens."""
@@ -141,8 +155,8 @@ class _PackedAttentionFn(torch.autograd.Function):
         from . import native
 
         p = packing
-        o, lse2 = native.packed_attention_fwd(q, k, v, *p.tables(), p.num_tokens, scale)
-        ctx.save_for_backward(q, k, v, o, lse2)
+        o, bias2 = native.packed_attention_fwd(q, k, v, *p.tables(), p.num_tokens, scale)
+        ctx.save_for_backward(q, k, v, o, bias2)
         ctx.packing, ctx.scale = packing, scale
         return o
 
@@ -151,9 +165,9 @@ class _PackedAttentionFn(torch.autograd.Function):
     def backward(ctx, d_o):
         from . import native
 
-        q, k, v, o, lse2 = ctx.saved_tensors
+        q, k, v, o, bias2 = ctx.saved_tensors
         p = ctx.packing
-        dq, dk, dv = native.packed_attention_bwd(d_o, q, k, v, o, lse2, *p.tables(), p.num_tokens, ctx.scale)
+        dq, dk, dv = native.packed_attention_bwd(d_o, q, k, v, o, bias2, *p.tables(), p.num_tokens, ctx.scale)
         return dq, dk, dv, None, None
 
 

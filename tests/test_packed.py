@@ -24,15 +24,28 @@ def test_plan_describes_every_row(lens, total):
         t += n
     for r in range(t, rows):
         assert p.first_key[r] == r + 1 and p.end_query[r] == r and p.position[r] == 0
-    tiles = -(-rows // 128)
-    assert sorted(p.query_order.tolist()) == list(range(tiles)) == sorted(p.key_order.tolist())
-    assert all(x.dtype == torch.int32 for x in (p.first_key, p.end_query, p.position, p.query_order, p.key_order))
+    valid = sum(lens)
+    queries, keys = {}, {}
+    for row0 in range(0, rows, 128):
+        own = range(row0, min(row0 + 128, valid))
+        some = len(own) > 0
+        queries[row0] = [row0] + ([int(p.first_key[own[0]]), int(p.first_key[own[-1]]), own[-1] + 1] if some else [0, 0, 0])
+        keys[row0] = [row0] + ([int(p.end_query[own[-1]]), int(p.end_query[own[0]]), 0] if some else [row0, 0, 0])
+    assert {e[0]: e for e in p.query_tiles.view(-1, 4).tolist()} == queries
+    assert {e[0]: e for e in p.key_tiles.view(-1, 4).tolist()} == keys
+    pairs = p.query_pairs.view(-1, 8).tolist()
+    assert sorted(e[0] for e in pairs) == list(range(0, rows, 256))
+    for e in pairs:
+        assert e[:4] == queries[e[0]]
+        assert e[4:] == queries[e[0] + 128] if e[0] + 128 in queries else e[4] >= rows and e[5:] == [0, 0, 0]
+    assert all(x.dtype == torch.int32 for x in (p.first_key, p.end_query, p.position, p.query_tiles))
 
 
 def test_plan_orders_tiles_by_work():
     p = ops.PackedSequences([1000, 24])  # one long document, then a short one in the last tile
-    assert p.query_order.tolist()[0] == 7 and p.query_order.tolist()[-1] == 0
-    assert p.key_order.tolist() == list(range(8))
+    assert p.query_tiles.view(-1, 4)[:, 0].tolist() == list(range(896, -1, -128))
+    assert p.query_pairs.view(-1, 8)[:, 0].tolist() == [768, 512, 256, 0]
+    assert p.key_tiles.view(-1, 4)[:, 0].tolist() == list(range(0, 1024, 128))
 
 
 def test_plan_accepts_arrays_and_tensors():
