@@ -97,7 +97,7 @@ BgnPackedAttention packed_args(const at::Tensor& q, const at::Tensor& k, const a
 
 std::vector<at::Tensor> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor first_key,
                                              at::Tensor end_query, at::Tensor query_tiles, at::Tensor query_pairs, at::Tensor key_tiles,
-                                             int64_t valid, double scale) {
+                                             int64_t valid, double scale, bool backward) {
   c10::cuda::CUDAGuard guard(q.device());
   check_packed(q, k);
   q = readable(q);
@@ -106,13 +106,17 @@ std::vector<at::Tensor> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Ten
   const auto a = packed_args(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale);
   auto o = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
   auto bias2 = at::empty({q.size(1), a.pitch}, q.options().dtype(at::kFloat));
-  ran(bgn_packed_attention_fwd(&a, o.data_ptr(), bias2.data_ptr<float>(), bgn_status_word(q), current()),
+  at::Tensor rest;
+  if (backward && a.type != 2) rest = at::empty_like(o);
+  ran(bgn_packed_attention_fwd(&a, o.data_ptr(), rest.defined() ? rest.data_ptr() : nullptr, bias2.data_ptr<float>(),
+                               bgn_status_word(q), current()),
       "packed_attention_fwd");
+  if (rest.defined()) return {o, bias2, rest};
   return {o, bias2};
 }
 
 std::vector<at::Tensor> packed_attention_bwd(at::Tensor d_o, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o,
-                                             at::Tensor bias2, at::Tensor first_key, at::Tensor end_query,
+                                             at::Tensor bias2, c10::optional<at::Tensor> rest, at::Tensor first_key, at::Tensor end_query,
                                              at::Tensor query_tiles, at::Tensor query_pairs, at::Tensor key_tiles, int64_t valid, double scale) {
   c10::cuda::CUDAGuard guard(q.device());
   check_packed(q, k);
@@ -123,6 +127,9 @@ std::vector<at::Tensor> packed_attention_bwd(at::Tensor d_o, at::Tensor q, at::T
                   o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type() && o.is_contiguous() &&
                   bias2.scalar_type() == at::kFloat && bias2.is_contiguous() && bias2.numel() == (q.size(0) + 127) / 128 * 128 * q.size(1),
               "bergson_b200: the output's gradient does not fit the operands");
+  TORCH_CHECK(!rest.has_value() || (rest->sizes() == o.sizes() && rest->scalar_type() == o.scalar_type() &&
+                                    rest->is_contiguous() && rest->device() == o.device()),
+              "bergson_b200: the output's rest does not fit the output");
   d_o = readable(d_o);
   const auto a = packed_args(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale);
   auto delta = at::empty_like(bias2);
@@ -131,7 +138,7 @@ std::vector<at::Tensor> packed_attention_bwd(at::Tensor d_o, at::Tensor q, at::T
   auto dk = at::empty({k.size(0), k.size(1), k.size(2)}, k.options());
   auto dv = at::empty_like(dk);
   const auto [tok, head] = strides_of(d_o);
-  ran(bgn_packed_attention_bwd(&a, o.data_ptr(), bias2.data_ptr<float>(), d_o.data_ptr(), tok, head,
+  ran(bgn_packed_attention_bwd(&a, o.data_ptr(), rest.has_value() ? rest->data_ptr() : nullptr, bias2.data_ptr<float>(), d_o.data_ptr(), tok, head,
                                delta.data_ptr<float>(), do_max.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                bgn_status_word(q), current()),
       "packed_attention_bwd");

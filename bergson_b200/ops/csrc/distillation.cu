@@ -12,12 +12,14 @@
 
 #include "common.cuh"
 #include "kernels_distill.h"
+#include "packed_tc.cuh"
 
 namespace bgn {
 
 namespace cg = cooperative_groups;
 
-constexpr int kDistillThreads = 512;
+constexpr int kDistillThreads = 256;
+constexpr int kDistillUnroll = 4;  // packets a thread has in flight, and as many at work
 constexpr int kDistillWarps = kDistillThreads / 32;
 constexpr float kDistillLog2e = 1.4426950408889634f;
 constexpr float kDistillLn2 = 0.6931471805599453f;
@@ -69,10 +71,63 @@ __device__ __forceinline__ int lead_of(const T* p, int n) {
   return lead < n ? lead : n;
 }
 
+// work(packet, index) for the packets of one part of a row, kDistillUnroll of them in flight for a thread;
+// the first ones are asked for by fetch().  Many small blocks on an SM keep the memory busy while one of
+// them computes or joins its sums.
+template <typename T>
+struct DistillStream {
+  static constexpr int U = kDistillUnroll;
+  const DistillPacket<T>* from;
+  int packets;
+  DistillPacket<T> held[U];
+
+  __device__ __forceinline__ void fetch(int base) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (base + u * kDistillThreads < packets) held[u] = from[base + u * kDistillThreads];
+  }
+  template <typename F>
+  __device__ __forceinline__ void run(F work) {
+    for (int i = threadIdx.x; i < packets;) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * kDistillThreads < packets) work(held[u], i + u * kDistillThreads);
+      i += U * kDistillThreads;
+      fetch(i);
+    }
+  }
+};
+
+// A packet's values in fp32, and the largest of them (NaN does not count).
+template <typename T>
+__device__ __forceinline__ float unpack_max(const DistillPacket<T>& p, float2 (&f)[DistillPacket<T>::N / 2]);
+template <>
+__device__ __forceinline__ float unpack_max<float>(const DistillPacket<float>& p, float2 (&f)[2]) {
+  f[0] = make_float2(p.v[0], p.v[1]);
+  f[1] = make_float2(p.v[2], p.v[3]);
+  return fmaxf(fmaxf(p.v[0], p.v[1]), fmaxf(p.v[2], p.v[3]));
+}
+template <>
+__device__ __forceinline__ float unpack_max<__nv_bfloat16>(const DistillPacket<__nv_bfloat16>& p, float2 (&f)[4]) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(p.v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = __bfloat1622float2(h[e]);
+  const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+template <>
+__device__ __forceinline__ float unpack_max<__half>(const DistillPacket<__half>& p, float2 (&f)[4]) {
+  const __half2* h = reinterpret_cast<const __half2*>(p.v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = __half22float2(h[e]);
+  const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+
 // A cluster of blocks shares one row: block r of it sweeps the r-th part of the columns, the first
 // block joins the parts in rank order.
 template <typename T>
-__global__ void __launch_bounds__(kDistillThreads) distill_fwd_kernel(BgnDistill a, float* loss, float* stats) {
+__global__ void __launch_bounds__(kDistillThreads, 5) distill_fwd_kernel(BgnDistill a, float* loss, float* stats) {
   constexpr int V = DistillPacket<T>::N;
   __shared__ float red[3 * kDistillWarps];
   __shared__ float part[2];
@@ -85,8 +140,24 @@ __global__ void __launch_bounds__(kDistillThreads) distill_fwd_kernel(BgnDistill
   const int per = ((a.vocab + parts - 1) / parts + V - 1) / V * V;
   const int begin = min(rank * per, a.vocab), n = min(begin + per, a.vocab) - begin;
   const T* x = z + begin;
-  float m = -INFINITY, s = 0.f;
+  const int lead = lead_of(x, n);
+  DistillStream<T> stream = {reinterpret_cast<const DistillPacket<T>*>(x + lead), (n - lead) / V};
+  stream.fetch(threadIdx.x);
+
+  // Teacher entries of the row and the student's logits there, while the first packets are on their way.
+  __shared__ float t_of[kDistillMaxTop], z_of[kDistillMaxTop];
+  float t_max = -INFINITY;
+  if (rank == 0)
+    for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
+      float t;
+      const int id = load_entry(a, row * a.top + k, &t);
+      t_of[k] = id >= 0 ? t : -INFINITY;
+      z_of[k] = id >= 0 ? to_float<T>(z[id]) : 0.f;
+      t_max = fmaxf(t_max, t_of[k]);
+    }
+
   // The difference to the maximum is taken before the factor, which could overflow a type's lowest value.
+  float m = -INFINITY, s = 0.f;
   const auto one = [&](float v) {
     if (v > m) {
       s *= exp2f((m - v) * c);
@@ -95,124 +166,83 @@ __global__ void __launch_bounds__(kDistillThreads) distill_fwd_kernel(BgnDistill
     // an entry of -inf adds nothing, and there may be no finite maximum yet
     if (v != -INFINITY) s += exp2f((v - m) * c);
   };
-  const int lead = lead_of(x, n), packets = (n - lead) / V;
   if (int(threadIdx.x) < lead) one(to_float<T>(x[threadIdx.x]));
-  const DistillPacket<T>* xp = reinterpret_cast<const DistillPacket<T>*>(x + lead);
-  constexpr int U = 4;  // packets in flight for a thread
-  for (int i = threadIdx.x; i < packets; i += kDistillThreads * U) {
-    DistillPacket<T> p[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u * kDistillThreads < packets) p[u] = xp[i + u * kDistillThreads];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u * kDistillThreads >= packets) break;
-      float f[V], mx = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        f[e] = to_float<T>(p[u].v[e]);
-        mx = fmaxf(mx, f[e]);
-      }
-      if (mx > m) {
-        s *= exp2f((m - mx) * c);
-        m = mx;
-      }
-      if (mx != -INFINITY) {
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) sum += exp2f((f[e] - m) * c);
-        s += sum;
-      }
+  stream.run([&](const DistillPacket<T>& p, int) {
+    float2 f[V / 2];
+    const float mx = unpack_max<T>(p, f);
+    if (mx > m) {
+      s *= exp2f((m - mx) * c);
+      m = mx;
     }
-  }
-  for (int i = lead + packets * V + threadIdx.x; i < n; i += kDistillThreads) one(to_float<T>(x[i]));
+    if (mx != -INFINITY) {
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int e = 0; e < V / 2; ++e) {
+        const float2 d = mul2(add2(f[e], make_float2(-m, -m)), make_float2(c, c));
+        sum = add2(sum, make_float2(fast_exp2(d.x), fast_exp2(d.y)));
+      }
+      s += sum.x + sum.y;
+    }
+  });
+  for (int i = lead + stream.packets * V + threadIdx.x; i < n; i += kDistillThreads) one(to_float<T>(x[i]));
 
-  // Teacher entries of the row: only the first block needs them.
-  const long k0 = row * a.top;
-  float t_max = -INFINITY;
-  if (rank == 0)
-    for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
-      float t;
-      if (load_entry(a, k0 + k, &t) >= 0) t_max = fmaxf(t_max, t);
-    }
   float mx[2] = {m, t_max};
   block_reduce<2, true>(mx, red);
-  float sums[1] = {m == -INFINITY ? s : s * exp2f((m - mx[0]) * c)};
-  block_reduce<1, false>(sums, red);
-  float row_m = mx[0], row_s = sums[0];
+  float row_m = mx[0];
+  if (m != -INFINITY) s *= exp2f((m - row_m) * c);
   if (parts > 1) {
+    float sum[1] = {s};
+    block_reduce<1, false>(sum, red);
     if (threadIdx.x == 0) {
       part[0] = row_m;
-      part[1] = row_s;
+      part[1] = sum[0];
     }
     cluster.sync();
+    s = 0.f;
     if (rank == 0) {
       for (int r = 1; r < parts; ++r) row_m = fmaxf(row_m, *cluster.map_shared_rank(&part[0], r));
-      row_s = 0.f;
-      for (int r = 0; r < parts; ++r) {
-        const float pm = *cluster.map_shared_rank(&part[0], r), ps = *cluster.map_shared_rank(&part[1], r);
-        row_s += pm == -INFINITY ? ps : ps * exp2f((pm - row_m) * c);
-      }
+      if (threadIdx.x == 0)
+        for (int r = 0; r < parts; ++r) {
+          const float pm = *cluster.map_shared_rank(&part[0], r), ps = *cluster.map_shared_rank(&part[1], r);
+          s += pm == -INFINITY ? ps : ps * exp2f((pm - row_m) * c);
+        }
     }
     cluster.sync();  // the parts stay until they are read
     if (rank != 0) return;
   }
-  float w_sum[2] = {0.f, 0.f};  // W, sum of w (log2 w - log2 of the student's unnormalised value)
-  int any = 0;
-  for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
-    float t;
-    const int id = load_entry(a, k0 + k, &t);
-    if (id < 0) continue;
-    any = 1;
-    t = (t - mx[1]) * c;
-    const float w = exp2f(t);
-    w_sum[0] += w;
-    if (w != 0.f) w_sum[1] += w * (t - (to_float<T>(z[id]) - row_m) * c);
-  }
-  any = __syncthreads_or(any);
-  block_reduce<2, false>(w_sum, red);
+  // s; W; sum of w (log2 w - log2 of the student's unnormalised value)
+  float sums[3] = {s, 0.f, 0.f};
+  if (rank == 0)
+    for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
+      if (t_of[k] == -INFINITY) continue;
+      const float d = (t_of[k] - mx[1]) * c, w = exp2f(d);
+      sums[1] += w;
+      if (w != 0.f) sums[2] += w * (d - (z_of[k] - row_m) * c);
+    }
+  block_reduce<3, false>(sums, red);
   if (threadIdx.x == 0) {
-    const float l2 = log2f(row_s);
+    const float l2 = log2f(sums[0]);
     stats[2 * row] = row_m;
     stats[2 * row + 1] = l2;
-    loss[row] = any ? a.temperature * a.temperature * kDistillLn2 * (w_sum[1] / w_sum[0] - log2f(w_sum[0]) + l2) : 0.f;
+    const float loss2 = sums[2] / sums[1] - log2f(sums[1]) + l2;
+    // the largest entry has w = 1: no sum, no entry
+    loss[row] = sums[1] == 0.f ? 0.f : a.temperature * a.temperature * kDistillLn2 * loss2;
   }
 }
 
-// grid (parts, tokens): a block rewrites one part of a row's columns and puts its teacher entries right
+// Blocks parts * row ...: a block rewrites one part of a row's columns and puts its teacher entries right
 // afterwards, each from the logit itself, so that every value is rounded once.
 template <typename T>
-__global__ void __launch_bounds__(kDistillThreads)
+__global__ void __launch_bounds__(kDistillThreads, 5)
 distill_bwd_kernel(BgnDistill a, const float* stats, const float* dloss, T* dlogits, long d_pitch, int parts) {
   constexpr int V = DistillPacket<T>::N;
   __shared__ float red[kDistillWarps];
-  __shared__ float p_of[kDistillMaxTop];
-  __shared__ int id_of[kDistillMaxTop];
+  __shared__ alignas(16) float p_of[kDistillMaxTop];
+  __shared__ alignas(16) int id_of[kDistillMaxTop];
   const long row = blockIdx.x / parts;
   const int rank = int(blockIdx.x % parts);
   const float c = kDistillLog2e / a.temperature;
   const long k0 = row * a.top;
-
-  float t_max[1] = {-INFINITY};
-  int any = 0;
-  for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
-    id_of[k] = load_entry(a, k0 + k, &p_of[k]);
-    if (id_of[k] >= 0) {
-      any = 1;
-      t_max[0] = fmaxf(t_max[0], p_of[k]);
-    }
-  }
-  any = __syncthreads_or(any);
-  block_reduce<1, true>(t_max, red);
-  float w_sum[1] = {0.f};
-  for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
-    p_of[k] = id_of[k] >= 0 ? exp2f((p_of[k] - t_max[0]) * c) : 0.f;
-    w_sum[0] += p_of[k];
-  }
-  block_reduce<1, false>(w_sum, red);
-  const float inv_w = any ? 1.f / w_sum[0] : 0.f;
-  const float g = any ? dloss[row] * a.temperature : 0.f;
-  const float m = stats[2 * row], l2 = stats[2 * row + 1];
   const T* z = static_cast<const T*>(a.logits) + row * a.pitch;
   T* dz = dlogits + row * d_pitch;
 
@@ -220,27 +250,48 @@ distill_bwd_kernel(BgnDistill a, const float* stats, const float* dloss, T* dlog
   const int begin = min(rank * per, a.vocab), n = min(begin + per, a.vocab) - begin;
   const T* x = z + begin;
   T* y = dz + begin;
-  const auto value = [&](float v) { return g == 0.f ? 0.f : g * exp2f((v - m) * c - l2); };
+  // Packets need the same alignment on both sides.
   const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0;
-  const int lead = same ? lead_of(x, n) : n, packets = (n - lead) / V;
-  for (int i = threadIdx.x; i < lead; i += kDistillThreads) y[i] = from_float<T>(value(to_float<T>(x[i])));
-  const DistillPacket<T>* xp = reinterpret_cast<const DistillPacket<T>*>(x + lead);
-  DistillPacket<T>* yp = reinterpret_cast<DistillPacket<T>*>(y + lead);
-  constexpr int U = 4;
-  for (int i = threadIdx.x; i < packets; i += kDistillThreads * U) {
-    DistillPacket<T> p[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u * kDistillThreads < packets) p[u] = xp[i + u * kDistillThreads];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u * kDistillThreads >= packets) break;
-#pragma unroll
-      for (int e = 0; e < V; ++e) p[u].v[e] = from_float<T>(value(to_float<T>(p[u].v[e])));
-      yp[i + u * kDistillThreads] = p[u];
-    }
+  const int lead = same ? lead_of(x, n) : n;
+  DistillStream<T> stream = {reinterpret_cast<const DistillPacket<T>*>(x + lead), (n - lead) / V};
+  stream.fetch(threadIdx.x);
+
+  float t_max[1] = {-INFINITY};
+  for (int k = threadIdx.x; k < (a.top + 3) / 4 * 4; k += kDistillThreads) {
+    float t = 0.f;
+    id_of[k] = k < a.top ? load_entry(a, k0 + k, &t) : -1;
+    p_of[k] = t;
+    if (id_of[k] >= 0) t_max[0] = fmaxf(t_max[0], t);
   }
-  for (int i = lead + packets * V + threadIdx.x; i < n; i += kDistillThreads) y[i] = from_float<T>(value(to_float<T>(x[i])));
+  block_reduce<1, true>(t_max, red);
+  float w_sum[1] = {0.f};
+  for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
+    p_of[k] = id_of[k] >= 0 ? exp2f((p_of[k] - t_max[0]) * c) : 0.f;
+    w_sum[0] += p_of[k];
+  }
+  block_reduce<1, false>(w_sum, red);
+  const bool any = w_sum[0] != 0.f;
+  const float inv_w = any ? 1.f / w_sum[0] : 0.f;
+  const float g = any ? dloss[row] * a.temperature : 0.f;
+  const float m = stats[2 * row], l2 = stats[2 * row + 1];
+  const auto value = [&](float v) { return g == 0.f ? 0.f : g * exp2f((v - m) * c - l2); };
+
+  for (int i = threadIdx.x; i < lead; i += kDistillThreads) y[i] = from_float<T>(value(to_float<T>(x[i])));
+  DistillPacket<T>* to = reinterpret_cast<DistillPacket<T>*>(y + lead);
+  stream.run([&](const DistillPacket<T>& p, int i) {
+    DistillPacket<T> o;
+    float2 f[V / 2];
+    unpack_max<T>(p, f);
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) {
+      const float2 d = fma2(add2(f[e], make_float2(-m, -m)), make_float2(c, c), make_float2(-l2, -l2));
+      const float2 q = mul2(make_float2(fast_exp2(d.x), fast_exp2(d.y)), make_float2(g, g));
+      o.v[2 * e] = from_float<T>(g == 0.f ? 0.f : q.x);
+      o.v[2 * e + 1] = from_float<T>(g == 0.f ? 0.f : q.y);
+    }
+    to[i] = o;
+  });
+  for (int i = lead + stream.packets * V + threadIdx.x; i < n; i += kDistillThreads) y[i] = from_float<T>(value(to_float<T>(x[i])));
   __syncthreads();
   // The teacher's entries: the first of equal ids takes the sum of all of them, in their order.
   for (int k = threadIdx.x; k < a.top; k += kDistillThreads) {
@@ -248,13 +299,15 @@ distill_bwd_kernel(BgnDistill a, const float* stats, const float* dloss, T* dlog
     if (id < begin || id >= begin + n) continue;
     bool first = true;
     float p = 0.f;
-    for (int j = 0; j < a.top; ++j) {
-      if (id_of[j] != id) continue;
-      if (j < k) {
-        first = false;
-        break;
-      }
-      p += p_of[j];
+    for (int j = 0; j < a.top; j += 4) {  // the arrays are filled up to a multiple of four
+      const int4 ids = *reinterpret_cast<const int4*>(id_of + j);
+      const float4 ps = *reinterpret_cast<const float4*>(p_of + j);
+      if (ids.x == id) p += ps.x;
+      if (ids.y == id) p += ps.y;
+      if (ids.z == id) p += ps.z;
+      if (ids.w == id) p += ps.w;
+      first = first && !((ids.x == id && j < k) || (ids.y == id && j + 1 < k) || (ids.z == id && j + 2 < k) ||
+                         (ids.w == id && j + 3 < k));
     }
     if (first) dz[id] = from_float<T>(g == 0.f ? 0.f : g * (exp2f((to_float<T>(z[id]) - m) * c - l2) - p * inv_w));
   }
@@ -275,12 +328,12 @@ static cudaError_t launch_distill_fwd(const BgnDistill& a, float* loss, float* s
   return cudaLaunchKernelEx(&cfg, distill_fwd_kernel<T>, a, loss, stats);
 }
 
-// Blocks to a row: with few rows a row is shared, so that some two blocks per SM are at work, as
-// long as each has at least four packets a thread.
+// Blocks to a row: with few rows a row is shared, so that some four blocks per SM are at work, as
+// long as each has a full group of packets for its threads.
 static int row_parts(const BgnDistill& a, int most) {
-  const int per_block = kDistillThreads * 4 * (a.type == 2 ? 4 : 8);
+  const int per_block = kDistillThreads * kDistillUnroll * (a.type == 2 ? 4 : 8);
   int parts = 1;
-  while (parts < most && a.tokens * parts < 2 * 148 && a.vocab / (2 * parts) >= per_block) parts *= 2;
+  while (parts < most && a.tokens * parts < 4 * 148 && a.vocab / (2 * parts) >= per_block) parts *= 2;
   return parts;
 }
 

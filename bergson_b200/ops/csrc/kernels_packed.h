@@ -30,12 +30,13 @@ typedef struct {
 // o [rows, heads, dim] contiguous and bias2 [heads, pitch]: minus the base-2 logarithm of the softmax
 // denominator of scale * log2(e) * q.k (for fp16 with 10 added); -inf where a row attends nothing,
 // unset from `rows` on.  The backward pass reads it.
-int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, float* bias2, int* status, cudaStream_t stream);
+// o_rest, like o: what rounding to 16 bits took from o; null where no backward pass follows, and for fp32.
+int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, void* o_rest, float* bias2, int* status, cudaStream_t stream);
 
 // Gradients of the operands (contiguous) from the output's gradient d_o [rows, heads, dim] (strides in
-// elements), the forward's o and bias2.  Scratch: delta [heads, pitch], do_max [heads, pitch / 32].
-int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const float* bias2, const void* d_o, long do_tok,
-                             long do_head, float* delta, float* do_max, void* dq, void* dk, void* dv, int* status,
+// elements), the forward's o, o_rest and bias2.  Scratch: delta [heads, pitch], do_max [heads, pitch / 32].
+int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const void* o_rest, const float* bias2,
+                             const void* d_o, long do_tok, long do_head, float* delta, float* do_max, void* dq, void* dk, void* dv, int* status,
                              cudaStream_t stream);
 
 typedef struct {

@@ -9,15 +9,16 @@ using namespace bgn;
 
 namespace {
 
-// cudaFuncSetAttribute holds for the current device only.
-cudaError_t allow_smem(const void* kernel, int bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
+// What a launch has to know of the current device.
 cudaError_t sm_count(int* n) {
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   return e == cudaSuccess ? cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, device) : e;
+}
+
+// cudaFuncSetAttribute holds for the current device only.
+cudaError_t allow_smem(const void* kernel, int bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
 template <typename T, int DP>
@@ -85,7 +86,7 @@ bool operand_map(CUtensorMap* map, const void* base, int fmt, int dim, int heads
 }
 
 template <int FMT, int DP>
-cudaError_t tensor_fwd(const BgnPackedAttention& a, void* o, float* bias2, int* status, cudaStream_t stream) {
+cudaError_t tensor_fwd(const BgnPackedAttention& a, void* o, void* o_rest, float* bias2, int* status, cudaStream_t stream) {
   ensure_context_bound();
   CUtensorMap mq, mk, mv;
   if (!operand_map(&mq, a.q, FMT, a.dim, a.heads, a.valid, a.q_head, a.q_tok) ||
@@ -116,6 +117,7 @@ cudaError_t tensor_fwd(const BgnPackedAttention& a, void* o, float* bias2, int* 
   p.v_tok = a.v_tok;
   p.v_head = a.v_head;
   p.o = o;
+  p.o_rest = o_rest;
   p.bias2 = bias2;
   constexpr int smem = fwd_smem_bytes<DP>();
   auto kern = packed_fwd_kernel<FMT, DP>;
@@ -129,7 +131,7 @@ cudaError_t tensor_fwd(const BgnPackedAttention& a, void* o, float* bias2, int* 
 }
 
 template <int FMT, int DP>
-cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const float* bias2, const void* d_o, long do_tok,
+cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const void* o_rest, const float* bias2, const void* d_o, long do_tok,
                        long do_head, float* delta, float* do_max, void* dq, void* dk, void* dv, int* status,
                        cudaStream_t stream) {
   ensure_context_bound();
@@ -153,6 +155,7 @@ cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const float* 
   p.k = a.k;
   p.v = a.v;
   p.o = o;
+  p.o_rest = o_rest;
   p.d_o = d_o;
   p.q_tok = a.q_tok;
   p.q_head = a.q_head;
@@ -196,17 +199,18 @@ bool sound(const BgnPackedAttention* a) {
 
 }  // namespace
 
-extern "C" int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, float* bias2, int* status,
+extern "C" int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, void* o_rest, float* bias2, int* status,
                                         cudaStream_t stream) {
   if (!sound(a)) return int(cudaErrorInvalidValue);
   const bool narrow = a->dim <= 64;
   if (a->type == 2) return int(narrow ? simple_fwd<float, 64>(*a, o, bias2, stream) : simple_fwd<float, 128>(*a, o, bias2, stream));
   if (a->type == 1)
-    return int(narrow ? tensor_fwd<1, 64>(*a, o, bias2, status, stream) : tensor_fwd<1, 128>(*a, o, bias2, status, stream));
-  return int(narrow ? tensor_fwd<0, 64>(*a, o, bias2, status, stream) : tensor_fwd<0, 128>(*a, o, bias2, status, stream));
+    return int(narrow ? tensor_fwd<1, 64>(*a, o, o_rest, bias2, status, stream) : tensor_fwd<1, 128>(*a, o, o_rest, bias2, status, stream));
+  return int(narrow ? tensor_fwd<0, 64>(*a, o, o_rest, bias2, status, stream) : tensor_fwd<0, 128>(*a, o, o_rest, bias2, status, stream));
 }
 
-extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const float* bias2, const void* d_o,
+extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const void* o_rest,
+                                        const float* bias2, const void* d_o,
                                         long do_tok, long do_head, float* delta, float* do_max, void* dq, void* dk,
                                         void* dv, int* status, cudaStream_t stream) {
   if (!sound(a)) return int(cudaErrorInvalidValue);
@@ -216,5 +220,6 @@ extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void*
                       : simple_bwd<float, 128>(*a, o, bias2, d_o, do_tok, do_head, delta, dq, dk, dv, stream));
   auto run = a->type == 1 ? (narrow ? tensor_bwd<1, 64> : tensor_bwd<1, 128>)
                           : (narrow ? tensor_bwd<0, 64> : tensor_bwd<0, 128>);
-  return int(run(*a, o, bias2, d_o, do_tok, do_head, delta, do_max, dq, dk, dv, status, stream));
+  if (o_rest == nullptr) return int(cudaErrorInvalidValue);
+  return int(run(*a, o, o_rest, bias2, d_o, do_tok, do_head, delta, do_max, dq, dk, dv, status, stream));
 }

@@ -12,15 +12,14 @@
 // few small values, so there P carries a factor 2^10 and dS the power of two that brings the largest
 // |do| of the rows concerned to [1/2, 1): both are taken out of the fp32 sums at the end.
 //
-// Blocks look for infinities and NaN in operand tiles that are partly masked and then compute their
-// rows again, row by row, as the forward pass does.
+// Rows whose results are not finite are computed again over what they attend alone, as in the forward pass.
 #pragma once
 
 #include "packed_fwd.cuh"
 
 namespace bgn {
 
-constexpr int kBwdThreads = 384;
+constexpr int kBwdThreads = 320;
 
 struct PackedBwdArgs {
   const int* first_key;
@@ -30,7 +29,7 @@ struct PackedBwdArgs {
   int rows, valid, heads, kv_heads, dim;
   int pitch;  // floats between the heads of bias2 and neg_delta, a multiple of 128
   float scale;
-  const void *q, *k, *v, *o, *d_o;
+  const void *q, *k, *v, *o, *o_rest, *d_o;
   long q_tok, q_head, k_tok, k_head, v_tok, v_head, do_tok, do_head;
   const float* bias2;
   float* neg_delta;
@@ -77,18 +76,20 @@ __device__ __forceinline__ float2 score_gradient(uint32_t p0, uint32_t p1, uint3
 //
 // TMEM: dQ, S, dP twice (128 columns each; dS in 16 bits over its dP).  Shared memory: q, do, three
 // key and two value tiles (7 tiles of 32 KB at 128 features).  Warps 0-7: softmax, warps 0-3 on the first 64 keys of a tile, 4-7 on the rest;
-// two threads share a row.  8 TMA, 9 MMA, 10-11 look through partly masked key tiles.
+// two threads share a row.  8 TMA, 9 MMA.
 
 constexpr int kDqKStages = 3;  // a key tile stays until dQ of its step, which comes after S and dP of the next
 constexpr int kDqVStages = 2;
 
 template <int DP>
 constexpr int dq_smem_bytes() {
-  return (2 + kDqKStages + kDqVStages) * tile_bytes<DP>() + 1024 + 256;
+  return (2 + kDqKStages + kDqVStages) * tile_bytes<DP>() + 4 * kTile * 4 + 256;
 }
 
+// One half of the features of a row of dQ.
 template <int FMT, int DP>
-__device__ __noinline__ void exact_dq_row(const PackedBwdArgs& p, int row, int head, float bias2, float neg_delta, int lane) {
+__device__ __noinline__ void exact_dq_row(const PackedBwdArgs& p, int row, int head, float bias2, float neg_delta, int half,
+                                          int lane) {
   using T = typename Type16<FMT>::T;
   const int kv = head / (p.heads / p.kv_heads), first = p.first_key[row];
   const float c = p.scale * kPackedLog2e;
@@ -106,7 +107,7 @@ __device__ __noinline__ void exact_dq_row(const PackedBwdArgs& p, int row, int h
   T* dst = static_cast<T*>(p.dq) + (long(row) * p.heads + head) * p.dim;
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e)
-    if (lane + 32 * e < p.dim) dst[lane + 32 * e] = from_float<T>(dq[e] * p.scale);
+    if (lane + 32 * e < p.dim && (lane + 32 * e >= DP / 2) == (half != 0)) dst[lane + 32 * e] = from_float<T>(dq[e] * p.scale);
 }
 
 template <int FMT, int DP>
@@ -116,12 +117,18 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                  const __grid_constant__ PackedBwdArgs p, int* status) {
   constexpr int kTileBytes = tile_bytes<DP>();
   constexpr int kSlabs = DP / 64;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* q_tile = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  // Nearly all of the shared memory is in use at 128 features: there is no room for moving up to a boundary.
+  if ((smem_u32(smem_raw) & 1023u) != 0) {
+    if (threadIdx.x == 0) atomicCAS(status, kStatusOk, kStatusTimeoutProducer);
+    return;
+  }
+  uint8_t* q_tile = smem_raw;
   uint8_t* g_tile = q_tile + kTileBytes;
   uint8_t* k_tiles = g_tile + kTileBytes;
   uint8_t* v_tiles = k_tiles + kDqKStages * kTileBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(v_tiles + kDqVStages * kTileBytes);
+  float* halves = reinterpret_cast<float*>(v_tiles + kDqVStages * kTileBytes);  // [half][-delta, |do|][row]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(halves + 4 * kTile);
   uint64_t* q_full = bars;  // q and do
   uint64_t* q_empty = q_full + 1;
   uint64_t* k_full = q_empty + 1;  // [3]
@@ -133,10 +140,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   uint64_t* dp_full = s_read + 1;   // [2]
   uint64_t* ds_full = dp_full + 2;  // [2]
   uint64_t* dq_full = ds_full + 2;
-  uint64_t* checked = dq_full + 1;  // [2]: units in turn
-  uint64_t* seen = checked + 2;     // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(seen + 2);
-  int* poison = reinterpret_cast<int*>(tmem_slot + 1);  // [2][2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dq_full + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = p.heads / p.kv_heads;
@@ -146,15 +150,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     mbar_init(q_empty, 9);  // the MMA warp's commit and the softmax warps, which read do
     for (int s = 0; s < kDqKStages; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 3);  // commit and the two looking warps
+      mbar_init(&k_empty[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&v_full[t], 1);
       mbar_init(&v_empty[t], 1);
       mbar_init(&dp_full[t], 1);
       mbar_init(&ds_full[t], 8);
-      mbar_init(&checked[t], 2);
-      mbar_init(&seen[t], 8);
     }
     mbar_init(s_full, 1);
     mbar_init(s_read, 8);
@@ -296,35 +298,6 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       entry = next;
     }
     if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutMma);
-  } else if (warp >= 10) {
-    bool ok = true;
-    int j = 0, count = 0;
-    for (int r = 0; unit >= 0 && ok; ++r) {
-      const int after = nth_unit(r + 1, p.units);
-      const int4 next = after >= 0 ? __ldg(p.tiles + after / p.heads) : entry;
-      const int n = steps_of(entry);
-      bool bad = false;
-      for (int i = 0; i < n && ok; ++i, ++j) {
-        const int st = j % kDqKStages, key = entry.y + i * kTile;
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&k_full[st], (j / kDqKStages) & 1));
-        const bool masked = key + kTile - 1 > entry.x || key < entry.z;
-        if (masked && ok) bad |= scan_not_finite<FMT>(k_tiles + st * kTileBytes, kTileBytes, warp - 10, 2, lane);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&k_empty[st]);
-      }
-      if (n > 0) {
-        const int slot = count & 1;
-        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&seen[slot], ((count >> 1) & 1) ^ 1));
-        bad = __any_sync(0xffffffffu, bad);
-        if (lane == 0) {
-          poison[2 * slot + warp - 10] = bad;
-          mbar_arrive(&checked[slot]);
-        }
-        ++count;
-      }
-      unit = after;
-      entry = next;
-    }
   } else {
     using T = typename Type16<FMT>::T;
     const int half = warp >> 2, quad = warp & 3;
@@ -335,6 +308,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     bool ok = true;
     int j = 0, count = 0;
     for (int r = 0; unit >= 0 && ok; ++r) {
+      const int after = nth_unit(r + 1, p.units);
+      const int4 next = after >= 0 ? __ldg(p.tiles + after / p.heads) : entry;
       const int head = unit % p.heads, n = steps_of(entry);
       const int warp_row0 = entry.x + quad * 32, row = warp_row0 + lane;
       const bool in = row < p.valid;
@@ -343,35 +318,51 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const float bias2 = in ? p.bias2[long(head) * p.pitch + row] : -INFINITY;
       const int all_from = __shfl_sync(0xffffffffu, first, 31);
 
-      // delta = do . o: o from memory, asked for before do arrives in shared memory (swizzled rows of
-      // 128 bytes).  Both threads of a row compute it.
+      // delta = do . o, with what rounding took from o: dS is a difference against delta, and for rows with few
+      // keys that rounding would be its largest error.  o comes from memory, asked for before do arrives in
+      // shared memory (swizzled rows of 128 bytes).  Each of the two threads of a row takes half of the
+      // features.
       float neg_delta = 0.f, factor = 1.f;
       if (n > 0) {
-        uint4 o_row[DP / 8];
+        constexpr int kPackets = DP / 16;
+        uint4 o_row[kPackets], r_row[kPackets];
         const T* orow = static_cast<const T*>(p.o) + at;
+        const T* rrow = static_cast<const T*>(p.o_rest) + at;
 #pragma unroll
-        for (int d = 0; d < DP / 8; ++d)
-          o_row[d] = in && 8 * d < p.dim ? __ldg(reinterpret_cast<const uint4*>(orow + 8 * d)) : make_uint4(0, 0, 0, 0);
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(q_full, count & 1));
+        for (int d = 0; d < kPackets; ++d) {
+          const int f = 8 * (d + half * kPackets);
+          const bool there = in && f < p.dim;
+          o_row[d] = there ? __ldg(reinterpret_cast<const uint4*>(orow + f)) : make_uint4(0, 0, 0, 0);
+          r_row[d] = there ? __ldg(reinterpret_cast<const uint4*>(rrow + f)) : make_uint4(0, 0, 0, 0);
+        }
+        ok = warp_wait(q_full, count & 1);
         if (!ok) break;
         float top = 0.f;
         if (in) {
           const uint8_t* g = g_tile + tile_row * 128;
 #pragma unroll
-          for (int d = 0; d < DP / 8; ++d) {
-            union { uint4 u; T h[8]; } a, b;
+          for (int d = 0; d < kPackets; ++d) {
+            const int k = d + half * kPackets;
+            if (8 * k >= p.dim) continue;
+            union { uint4 u; T h[8]; } a, b, c;
             a.u = o_row[d];
-            b.u = *reinterpret_cast<const uint4*>(g + (d / 8) * kSlabBytes + (((d % 8) ^ (tile_row & 7)) << 4));
-            if (8 * d < p.dim) {
+            b.u = *reinterpret_cast<const uint4*>(g + (k / 8) * kSlabBytes + (((k % 8) ^ (tile_row & 7)) << 4));
+            c.u = r_row[d];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float x = to_float<T>(b.h[e]);
-                neg_delta = fmaf(-to_float<T>(a.h[e]), x, neg_delta);
-                top = fmaxf(top, fabsf(x));
-              }
+            for (int e = 0; e < 8; ++e) {
+              const float x = to_float<T>(b.h[e]);
+              neg_delta = fmaf(-to_float<T>(a.h[e]) - to_float<T>(c.h[e]), x, neg_delta);
+              top = fmaxf(top, fabsf(x));
             }
           }
         }
+        // Read again only after dQ of this unit, for which every softmax warp is done with them.
+        halves[half * 2 * kTile + tile_row] = neg_delta;
+        if (FMT == 0) halves[half * 2 * kTile + kTile + tile_row] = top;
+        named_barrier_sync(1, 256);
+        const float* other = halves + (1 - half) * 2 * kTile + tile_row;
+        neg_delta = half ? other[0] + neg_delta : neg_delta + other[0];
+        if (FMT == 0) top = fmaxf(top, other[kTile]);
         __syncwarp();
         if (lane == 0) mbar_arrive(q_empty);
         if (FMT == 0) {
@@ -437,27 +428,21 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (lane == 0) mbar_arrive(&ds_full[j & 1]);
       }
       if (!ok) break;
-      // the next unit, under what is left of this one
-      unit = nth_unit(r + 1, p.units);
-      if (unit >= 0) entry = __ldg(p.tiles + unit / p.heads);
       const bool some = in && first <= row;
+      unit = after;
+      entry = next;
       T* dst = static_cast<T*>(p.dq) + at;
       if (n > 0) {
-        const int slot = count & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&checked[slot], (count >> 1) & 1));
-        const bool exact = (poison[2 * slot] | poison[2 * slot + 1]) != 0;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&seen[slot]);
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(dq_full, count & 1)) && ok;
+        ok = warp_wait(dq_full, count & 1);
         ++count;
         if (!ok) break;
         tc_fence_after();
         // each of the two threads of a row stores one half of the features
-        if (!exact) store_row<FMT, DP>(tmem_dq + lane_base, p.scale / factor, dst, p.dim, some, half);
-        for (int rr = half; exact && rr < 32; rr += 2) {
-          const float bias_r = __shfl_sync(0xffffffffu, bias2, rr), delta_r = __shfl_sync(0xffffffffu, neg_delta, rr);
-          if (__shfl_sync(0xffffffffu, int(some), rr))
-            exact_dq_row<FMT, DP>(p, warp_row0 + rr, head, bias_r, delta_r, lane);
+        const bool bad = store_row<FMT, DP>(tmem_dq + lane_base, p.scale / factor, dst, p.dim, some, half);
+        for (uint32_t again = __ballot_sync(0xffffffffu, bad); again != 0; again &= again - 1) {
+          const int rr = __ffs(again) - 1;
+          exact_dq_row<FMT, DP>(p, warp_row0 + rr, head, __shfl_sync(0xffffffffu, bias2, rr),
+                                __shfl_sync(0xffffffffu, neg_delta, rr), half, lane);
         }
         tc_fence_before();
       }
@@ -485,8 +470,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 //
 // TMEM: dV, dK (up to 128 columns each), S^T, dP^T (128 each).  Shared memory: k, v, three query tiles,
 // two tiles of do with the rows' bias2 and delta.  Warps 0-7: softmax, warps 0-3 on the first 64
-// queries of a tile, 4-7 on the rest; two threads share a key.  8 TMA, 9 MMA, 10-11 look through
-// partly masked tiles of q and do.
+// queries of a tile, 4-7 on the rest; two threads share a key.  8 TMA, 9 MMA.
 
 constexpr int kDkvQStages = 3;
 constexpr int kDkvGStages = 2;
@@ -497,8 +481,9 @@ constexpr int dkv_smem_bytes() {
   return (2 + kDkvQStages + kDkvGStages) * tile_bytes<DP>() + kDkvGStages * kDkvRowBytes + 512;
 }
 
+// A row of dV (half 0) or of dK.
 template <int FMT, int DP>
-__device__ __noinline__ void exact_dkv_row(const PackedBwdArgs& p, int key, int kv, int lane) {
+__device__ __noinline__ void exact_dkv_row(const PackedBwdArgs& p, int key, int kv, int half, int lane) {
   using T = typename Type16<FMT>::T;
   const int group = p.heads / p.kv_heads, end = p.end_query[key], first = p.first_key[key];
   const float c = p.scale * kPackedLog2e;
@@ -523,8 +508,8 @@ __device__ __noinline__ void exact_dkv_row(const PackedBwdArgs& p, int key, int 
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e)
     if (lane + 32 * e < p.dim) {
-      static_cast<T*>(p.dk)[at + lane + 32 * e] = from_float<T>(dk[e] * p.scale);
-      static_cast<T*>(p.dv)[at + lane + 32 * e] = from_float<T>(dv[e]);
+      if (half) static_cast<T*>(p.dk)[at + lane + 32 * e] = from_float<T>(dk[e] * p.scale);
+      else static_cast<T*>(p.dv)[at + lane + 32 * e] = from_float<T>(dv[e]);
     }
 }
 
@@ -560,10 +545,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint64_t* dp_full = p_full + 1;
   uint64_t* ds_full = dp_full + 1;
   uint64_t* done = ds_full + 1;
-  uint64_t* checked = done + 1;  // [2]: units in turn
-  uint64_t* seen = checked + 2;  // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(seen + 2);
-  int* poison = reinterpret_cast<int*>(tmem_slot + 1);  // [2][2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = p.heads / p.kv_heads;
@@ -575,21 +557,17 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     mbar_init(v_empty, 1);
     for (int s = 0; s < kDkvQStages; ++s) {
       mbar_init(&q_full[s], 1);
-      mbar_init(&q_empty[s], 3);  // commit, 2 looking warps
+      mbar_init(&q_empty[s], 1);
     }
     for (int s = 0; s < kDkvGStages; ++s) {
       mbar_init(&g_full[s], 1);
-      mbar_init(&g_empty[s], 11);  // commit, 8 softmax warps, 2 looking warps
+      mbar_init(&g_empty[s], 9);  // commit and 8 softmax warps
     }
     mbar_init(s_full, 1);
     mbar_init(p_full, 8);
     mbar_init(dp_full, 1);
     mbar_init(ds_full, 8);
     mbar_init(done, 1);
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(&checked[t], 2);
-      mbar_init(&seen[t], 8);
-    }
     fence_barrier_init();
     tma_prefetch_desc(&map_q);
     tma_prefetch_desc(&map_do);
@@ -752,40 +730,6 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       entry = next;
     }
     if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutMma);
-  } else if (warp >= 10) {
-    bool ok = true;
-    int j = 0, count = 0;
-    for (int r = 0; unit >= 0 && ok; ++r) {
-      const int after = nth_unit(r + 1, p.units);
-      const int4 next = after >= 0 ? __ldg(p.tiles + after / p.kv_heads) : entry;
-      const int per_head = tiles_of(entry), n = per_head * group;
-      bool bad = false;
-      for (int i = 0; i < n && ok; ++i, ++j) {
-        const int q0 = entry.x + (i % per_head) * kTile;
-        const int qs = j % kDkvQStages, gs = j % kDkvGStages;
-        const bool masked = q0 < entry.x + kTile || q0 + kTile > entry.z;
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&q_full[qs], (j / kDkvQStages) & 1));
-        if (masked && ok) bad |= scan_not_finite<FMT>(q_tiles + qs * kTileBytes, kTileBytes, warp - 10, 2, lane);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_empty[qs]);
-        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&g_full[gs], (j / kDkvGStages) & 1));
-        if (masked && ok) bad |= scan_not_finite<FMT>(g_tiles + gs * kTileBytes, kTileBytes, warp - 10, 2, lane);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&g_empty[gs]);
-      }
-      if (n > 0) {
-        const int slot = count & 1;
-        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&seen[slot], ((count >> 1) & 1) ^ 1));
-        bad = __any_sync(0xffffffffu, bad);
-        if (lane == 0) {
-          poison[2 * slot + warp - 10] = bad;
-          mbar_arrive(&checked[slot]);
-        }
-        ++count;
-      }
-      unit = after;
-      entry = next;
-    }
   } else {
     using T = typename Type16<FMT>::T;
     const int half = warp >> 2, quad = warp & 3;
@@ -796,6 +740,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     bool ok = true;
     int j = 0, count = 0;
     for (int r = 0; unit >= 0 && ok; ++r) {
+      const int after = nth_unit(r + 1, p.units);
+      const int4 next = after >= 0 ? __ldg(p.tiles + after / p.kv_heads) : entry;
       const int kv_head = unit % p.kv_heads, per_head = tiles_of(entry), n = per_head * group;
       const int warp_key0 = entry.x + quad * 32, key = warp_key0 + lane;
       const bool in = key < p.valid;
@@ -887,25 +833,18 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
       }
       if (!ok) break;
-      // the next unit, under what is left of this one
-      unit = nth_unit(r + 1, p.units);
-      if (unit >= 0) entry = __ldg(p.tiles + unit / p.kv_heads);
+      unit = after;
+      entry = next;
       T* dst = static_cast<T*>(half ? p.dk : p.dv) + (long(key) * p.kv_heads + kv_head) * p.dim;
       if (n > 0) {
-        const int slot = count & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&checked[slot], (count >> 1) & 1));
-        const bool exact = (poison[2 * slot] | poison[2 * slot + 1]) != 0;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&seen[slot]);
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(done, count & 1)) && ok;
+        ok = warp_wait(done, count & 1);
         ++count;
         if (!ok) break;
         tc_fence_after();
         const float out = half ? p.scale / factor : (FMT == 0 ? 1.f / 1024.f : 1.f);
-        if (!exact) store_row<FMT, DP>((half ? tmem_dk : tmem_dv) + lane_base, out, dst, p.dim, in);
-        // both halves share the rows: even ones here, odd ones there
-        for (int rr = half; exact && rr < 32; rr += 2)
-          if (warp_key0 + rr < p.valid) exact_dkv_row<FMT, DP>(p, warp_key0 + rr, kv_head, lane);
+        const bool bad = store_row<FMT, DP>((half ? tmem_dk : tmem_dv) + lane_base, out, dst, p.dim, in);
+        for (uint32_t again = __ballot_sync(0xffffffffu, bad); again != 0; again &= again - 1)
+          exact_dkv_row<FMT, DP>(p, warp_key0 + __ffs(again) - 1, kv_head, half, lane);
         tc_fence_before();
       }
       if (!in && key < p.rows)

@@ -12,14 +12,18 @@
 // TMEM (512 columns): S of the two tiles (128 each, P in 16 bits over the first half of the same
 // columns: the A operand of the second product) and O of the two (up to 128 each).
 //
-// Warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread has a row), 8 TMA, 9 and 10 MMA of tile 0 and 1,
-// 11 looks for infinities and NaN in value tiles that are partly masked: 0 * NaN would carry them into
-// rows that do not attend them.  If there are any, the unit's rows are computed again, row by row.
+// Warps: 0-3 and 4-7 softmax of tile 0 and 1 (a thread has a row), 8 TMA, 9 and 10 MMA of tile 0 and 1.
+//
+// An infinity or NaN in a value row that some rows of a tile do not attend reaches them all the same, as
+// 0 * NaN of the second product.  It shows as a NaN of the result: a row whose result is not finite is
+// computed again, over its own keys alone.  (Looking through the tiles in shared memory instead held up
+// the pipeline: other reads wait long while the tensor core takes its operands from there.)
 //
 // What bounds it: a tile of 128 x 128 scores takes 1024 cycles of the tensor core at 128 features and
-// 1024 of the exponential unit, in a chain that the two tiles fill alternately.  So the chain is kept
-// short (the second product starts on the first half of the keys; skipped chunks where a warp's rows
-// attend nothing; packed fp32 arithmetic) and a quarter of the exponentials goes to the FMA units.
+// 1024 of the exponential unit (twice that of the tensor core at 64), in a chain that the two tiles
+// fill alternately.  The chain is kept short: a row's scores stay in registers, the second product starts
+// on the first three quarters of the keys, fp32 arithmetic is packed in pairs.  Moving a quarter of the
+// exponentials to a polynomial on the FMA units was slower (2.0 against 1.9 ms at 16384 tokens).
 //
 // O is rescaled only when a row's maximum grew by more than 2^8 since the last time (P then stays
 // below 2^8, which fp16 holds): the final division by the sum makes any base right.
@@ -51,6 +55,7 @@ struct PackedFwdArgs {
   const void *q, *k, *v;  // for the exact recomputation
   long q_tok, q_head, k_tok, k_head, v_tok, v_head;
   void* o;
+  void* o_rest;  // what rounding took from o, for the backward pass (may be null)
   float* bias2;
 };
 
@@ -63,7 +68,7 @@ __device__ __forceinline__ int nth_unit(int r, int units) {
 }
 
 struct QueryUnit {
-  int row0[2], head[2], last_first[2];
+  int row0[2], head[2];
   int i0[2], i1[2];  // key tiles of each, counted from `base` in steps of 128
   int base, n, kv_head;
 };
@@ -90,8 +95,6 @@ __device__ __forceinline__ QueryUnit query_unit(const int4 (&e)[2], int head_pai
   w.base = e[0].y;
   w.row0[0] = e[0].x;
   w.row0[1] = e[1].x;
-  w.last_first[0] = e[0].z;
-  w.last_first[1] = e[1].z;
   w.i0[0] = 0;
   w.i1[0] = some0 ? (e[0].w - w.base + kTile - 1) / kTile : 0;
   w.i0[1] = some1 ? (e[1].y - w.base) / kTile : 0;
@@ -115,10 +118,14 @@ __device__ __noinline__ void exact_forward_row(const PackedFwdArgs& p, int row, 
 #pragma unroll
     for (int e = 0; e < DP / 32; ++e) o[e] = fmaf(w, v[e], o[e]);
   }
-  T* dst = static_cast<T*>(p.o) + (long(row) * p.heads + head) * p.dim;
+  const long at = (long(row) * p.heads + head) * p.dim + lane;
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e)
-    if (lane + 32 * e < p.dim) dst[lane + 32 * e] = from_float<T>(o[e]);
+    if (lane + 32 * e < p.dim) {
+      const T kept = from_float<T>(o[e]);
+      static_cast<T*>(p.o)[at + 32 * e] = kept;
+      if (p.o_rest != nullptr) static_cast<T*>(p.o_rest)[at + 32 * e] = from_float<T>(o[e] - to_float<T>(kept));
+    }
 }
 
 // Largest of 32 values and `top`.
@@ -181,14 +188,14 @@ struct FwdMma {
     if (!warp_wait(&v_full[jj & 1], (jj >> 1) & 1)) return false;
     const uint64_t b = v + (jj & 1) * kStage;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (!warp_wait(&p_full[half], steps & 1)) return false;
+    for (int part = 0; part < 2; ++part) {
+      if (!warp_wait(&p_full[part], steps & 1)) return false;
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll
-        for (int i = 4 * half; i < 4 * half + 4; ++i)
+        for (int i = part ? 6 : 0; i < (part ? 8 : 6); ++i)
           umma_f16_ts(tmem_o, tmem_s + 8 * i, b + uint64_t((2048 * i) >> 4), idesc, (!first || i > 0) ? 1u : 0u);
-        if (half == 1) umma_commit(&v_empty[jj & 1]);
+        if (part == 1) umma_commit(&v_empty[jj & 1]);
       }
       __syncwarp();
     }
@@ -241,13 +248,10 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   uint64_t* v_full = k_empty + kFwdStages;
   uint64_t* v_empty = v_full + kFwdStages;
   uint64_t* s_full = v_empty + kFwdStages;  // [2] per tile
-  uint64_t* p_full = s_full + 2;            // [2][2]: tile, half of the keys
+  uint64_t* p_full = s_full + 2;            // [2][2]: tile, first 96 and last 32 keys
   uint64_t* turn_over = p_full + 4;         // [2]
   uint64_t* o_full = turn_over + 2;         // [2]
-  uint64_t* checked = o_full + 2;           // [2]: units in turn
-  uint64_t* seen = checked + 2;             // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(seen + 2);
-  int* poison = reinterpret_cast<int*>(tmem_slot + 1);  // [2]: units in turn
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -256,7 +260,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 2);  // the MMA warps
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 3);  // the MMA warps and the looking warp
+      mbar_init(&v_empty[s], 2);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
@@ -266,8 +270,6 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       mbar_init(&p_full[2 * t + 1], 4);
       mbar_init(&turn_over[t], 4);
       mbar_init(&o_full[t], 1);
-      mbar_init(&checked[t], 1);
-      mbar_init(&seen[t], 8);
     }
     fence_barrier_init();
     tma_prefetch_desc(&map_q);
@@ -290,6 +292,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   fetch_unit(p.tiles, p.head_pairs, p.heads, unit, entry);
 
   if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");  // 168 a thread at launch: 3 * 168 = 2 * 208 + 88
     if (warp == 8) {
       if (lane == 0) {
         bool ok = true;
@@ -369,49 +372,16 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         entry[1] = next[1];
       }
       if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutMma);
-    } else {
-      bool ok = true;
-      int j = 0, count = 0;
-      for (int r = 0; unit >= 0 && ok; ++r) {
-        const int after = nth_unit(r + 1, p.units);
-        fetch_unit(p.tiles, p.head_pairs, p.heads, after, next);
-        const QueryUnit u = query_unit(entry, p.head_pairs, p.heads, p.kv_heads, unit);
-        bool bad = false;
-        for (int i = 0; i < u.n && ok; ++i, ++j) {
-          const int st = j % kFwdStages;
-          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&v_full[st], (j / kFwdStages) & 1));
-          const int key = u.base + i * kTile;
-          bool masked = false;
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            masked |= i >= u.i0[t] && i < u.i1[t] && (key + kTile - 1 > u.row0[t] || key < u.last_first[t]);
-          if (masked && ok) bad |= scan_not_finite<FMT>(v_tiles + st * kTileBytes, kTileBytes, 0, 1, lane);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&v_empty[st]);
-        }
-        if (u.n > 0) {
-          const int slot = count & 1;
-          ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&seen[slot], ((count >> 1) & 1) ^ 1));
-          bad = __any_sync(0xffffffffu, bad);
-          if (lane == 0) {
-            poison[slot] = bad;
-            mbar_arrive(&checked[slot]);
-          }
-          ++count;
-        }
-        unit = after;
-        entry[0] = next[0];
-        entry[1] = next[1];
-      }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     using T = typename Type16<FMT>::T;
     const int t = warp >> 2, quad = warp & 3;
     const uint32_t lane_base = uint32_t(quad * 32) << 16;
     const uint32_t ts = tmem_s + 128 * t + lane_base, to = tmem_o + 128 * t + lane_base;
     const float c = p.scale * kPackedLog2e;
     bool ok = true;
-    int steps = 0, uses = 0, count = 0, turns = 0;
+    int steps = 0, uses = 0, turns = 0;
     // The two tiles take turns at the exponentials, tile 0 first: left alone they fall into step, and then
     // nobody computes under the products.  A tile takes its turn at every key tile of the unit, needed
     // or not, so neither is ever more than one ahead (a barrier tells only two phases apart).
@@ -449,24 +419,19 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         const int key = base + i * kTile;
         const bool masked = key + kTile - 1 > warp_row0 || key < all_from;
         const int from = first - key, upto = row - key;  // columns of the row's own range
-        // The scores are read twice, 32 columns at a time and one chunk ahead: small loops, whose code and
-        // values stay close.
-        uint32_t sa[32], sb[32];
-        tmem_ld_32(ts, sa);
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int g = 0; g < 4; g += 2) {
-          tmem_ld_wait();
-          pin_32(sa);
-          tmem_ld_32(ts + 32 * (g + 1), sb);
-          if (masked) hide(sa, bit_range(from - 32 * g, upto - 32 * g), 0xff800000u);  // -inf
-          top = max_chunk(sa, top);
-          tmem_ld_wait();
-          pin_32(sb);
-          tmem_ld_32(ts + 32 * ((g + 2) & 3), sa);
-          if (masked) hide(sb, bit_range(from - 32 * (g + 1), upto - 32 * (g + 1)), 0xff800000u);
-          top = max_chunk(sb, top);
+        uint32_t s[4][32];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) tmem_ld_32(ts + 32 * g, s[g]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int g = 0; g < 4; ++g) pin_32(s[g]);
+        if (masked) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) hide(s[g], bit_range(from - 32 * g, upto - 32 * g), 0xff800000u);  // -inf
         }
+        float top = max_chunk(s[0], -INFINITY);
+#pragma unroll
+        for (int g = 1; g < 4; ++g) top = max_chunk(s[g], top);
         // A new base where the maximum grew by more than 2^8 (or is the row's first).
         const bool grow = (top - m) * c > 8.f;
         if (__any_sync(0xffffffffu, grow)) {
@@ -489,26 +454,19 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ok = my_turn(turns);
         if (!ok) break;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
-        for (int g = 0; g < 4; g += 2) {
-          tmem_ld_wait();
-          pin_32(sa);
-          tmem_ld_32(ts + 32 * (g + 1), sb);
-          if (masked) hide(sa, bit_range(from - 32 * g, upto - 32 * g), 0xff800000u);
-          exp_chunk<FMT>(ts + 16 * g, sa, c, mc, sum);
-          tmem_ld_wait();
-          pin_32(sb);
-          if (g == 0) tmem_ld_32(ts + 64, sa);
-          if (masked) hide(sb, bit_range(from - 32 * (g + 1), upto - 32 * (g + 1)), 0xff800000u);
-          exp_chunk<FMT>(ts + 16 * (g + 1), sb, c, mc, sum);
-          if (g == 2) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          exp_chunk<FMT>(ts + 16 * g, s[g], c, mc, sum);
+          if (g == 1) {  // early: the handover takes about as long as the other half
             __syncwarp();
             if (lane == 0) mbar_arrive(&turn_over[t]);
           }
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[2 * t + g / 2]);
+          if (g >= 2) {  // the second product starts on three quarters of the keys
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * t + g - 2]);
+          }
         }
         ++steps;
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
@@ -520,25 +478,20 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const bool some = in && first <= row;
       const float bias2 = some ? p_shift<FMT>() - fmaf(m, c, log2f(l)) : -INFINITY;
       if (row < p.rows) p.bias2[long(head) * p.pitch + row] = bias2;
-      T* dst = static_cast<T*>(p.o) + (long(row) * p.heads + head) * p.dim;
-      if (n > 0) {
-        const int slot = count & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&checked[slot], (count >> 1) & 1));
-        const bool exact = poison[slot] != 0;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&seen[slot]);
-        ++count;
-        if (i1 > i0) {
-          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_full[t], uses & 1)) && ok;
-          ++uses;
-          tc_fence_after();
-          if (ok && !exact) store_row<FMT, DP>(to, some ? 1.f / l : 0.f, dst, p.dim, some);
-          for (int rr = 0; ok && exact && rr < 32; ++rr) {
-            const float bias_r = __shfl_sync(0xffffffffu, bias2, rr);
-            if (__shfl_sync(0xffffffffu, int(some), rr)) exact_forward_row<FMT, DP>(p, warp_row0 + rr, head, bias_r, lane);
-          }
-          tc_fence_before();
+      const long at = (long(row) * p.heads + head) * p.dim;
+      T* dst = static_cast<T*>(p.o) + at;
+      T* rest = p.o_rest != nullptr ? static_cast<T*>(p.o_rest) + at : nullptr;
+      if (i1 > i0) {
+        ok = warp_wait(&o_full[t], uses & 1);
+        ++uses;
+        if (!ok) break;
+        tc_fence_after();
+        const bool bad = store_row<FMT, DP>(to, some ? 1.f / l : 0.f, dst, p.dim, some, -1, rest);
+        for (uint32_t again = __ballot_sync(0xffffffffu, bad); again != 0; again &= again - 1) {
+          const int rr = __ffs(again) - 1;
+          exact_forward_row<FMT, DP>(p, warp_row0 + rr, head, __shfl_sync(0xffffffffu, bias2, rr), lane);
         }
+        tc_fence_before();
       }
       if (!some && row < p.rows)
         for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);

@@ -113,6 +113,12 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 }
 
 template <int FMT>
+__device__ __forceinline__ float2 unpack16(uint32_t h) {
+  if (FMT == 1) return make_float2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+template <int FMT>
 struct Type16;
 template <>
 struct Type16<0> { using T = __half; };
@@ -124,23 +130,6 @@ struct Type16<1> { using T = __nv_bfloat16; };
 template <int FMT>
 constexpr float p_shift() {
   return FMT == 0 ? 10.f : 0.f;
-}
-
-// One warp's share of a look through `bytes` of an operand tile in shared memory for 16-bit values that
-// are infinite or NaN (all exponent bits set): adding the exponent's lowest bit carries into the sign bit.
-template <int FMT>
-__device__ __forceinline__ bool scan_not_finite(const uint8_t* tile, int bytes, int part, int parts, int lane) {
-  // The carries of all values are collected and looked at once.
-  constexpr uint32_t exponent = FMT == 1 ? 0x7f807f80u : 0x7c007c00u, lowest = FMT == 1 ? 0x00800080u : 0x04000400u;
-  uint32_t carry = 0;
-  const uint4* p = reinterpret_cast<const uint4*>(tile) + part * 32 + lane;
-#pragma unroll 8
-  for (int i = 0; i < bytes / 512; i += parts) {
-    const uint4 u = p[i * 32];
-    carry |= ((u.x & exponent) + lowest) | ((u.y & exponent) + lowest) | ((u.z & exponent) + lowest) |
-             ((u.w & exponent) + lowest);
-  }
-  return (carry & 0x80008000u) != 0;
 }
 
 // Features of a row that a lane holds when a warp works on whole rows.
@@ -221,10 +210,13 @@ __device__ __forceinline__ void store_v8(void* ptr, const uint32_t* r) {
 }
 
 // A thread's row of an accumulator in TMEM, scaled, rounded and stored to `dst` (dim features,
-// 16-byte aligned); with `half` 0 or 1 only that half of the features.
+// 16-byte aligned); with `half` 0 or 1 only that half of the features.  `rest`, if any, gets what the
+// rounding took away, rounded in its turn.  Returns whether some value is infinite or NaN.
 template <int FMT, int DP>
-__device__ __forceinline__ void store_row(uint32_t tmem, float scale, void* dst, int dim, bool write, int half = -1) {
+__device__ __forceinline__ bool store_row(uint32_t tmem, float scale, void* dst, int dim, bool write, int half = -1,
+                                          void* rest = nullptr) {
   const bool wide = (dim & 15) == 0;  // every row begins on a 32-byte boundary then
+  bool bad = false;
 #pragma unroll 1
   for (int c = half == 1 ? DP / 2 : 0; c < (half == 0 ? DP / 2 : DP); c += 32) {
     if (c >= dim) break;
@@ -234,22 +226,41 @@ __device__ __forceinline__ void store_row(uint32_t tmem, float scale, void* dst,
     pin_32(r);
     if (write) {
       uint32_t h[16];
+      const auto store = [&](void* to) {
+        uint8_t* at = static_cast<uint8_t*>(to) + c * 2;
+        if (wide) {
+          store_v8(at, h);
+          if (c + 16 < dim) store_v8(at + 32, h + 8);
+        } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        h[i] = pack16<FMT>(__uint_as_float(r[2 * i]) * scale, __uint_as_float(r[2 * i + 1]) * scale);
-      uint8_t* at = static_cast<uint8_t*>(dst) + c * 2;
-      if (wide) {
-        store_v8(at, h);
-        if (c + 16 < dim) store_v8(at + 32, h + 8);
-      } else {
+          for (int i = 0; i < 4; ++i)
+            if (c + 8 * i < dim)
+              *reinterpret_cast<uint4*>(at + 16 * i) = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+        }
+      };
+      float largest = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (c + 8 * i < dim)
-            *reinterpret_cast<uint4*>(at + 16 * i) = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+      for (int i = 0; i < 16; ++i) {
+        const float x = __uint_as_float(r[2 * i]) * scale, y = __uint_as_float(r[2 * i + 1]) * scale;
+        asm("max.NaN.ftz.f32 %0, %0, %1;" : "+f"(largest) : "f"(fabsf(x)));
+        asm("max.NaN.ftz.f32 %0, %0, %1;" : "+f"(largest) : "f"(fabsf(y)));
+        h[i] = pack16<FMT>(x, y);
+      }
+      bad |= !(largest < INFINITY);
+      store(dst);
+      if (rest != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 kept = unpack16<FMT>(h[i]);
+          h[i] = pack16<FMT>(fmaf(__uint_as_float(r[2 * i]), scale, -kept.x),
+                             fmaf(__uint_as_float(r[2 * i + 1]), scale, -kept.y));
+        }
+        store(rest);
       }
     }
     __syncwarp();
   }
+  return bad;
 }
 
 }  // namespace bgn

@@ -596,5 +596,9 @@ def token_distillation(
     kernels = (torch.bfloat16, torch.float16, torch.float32)
     if (logits.dtype in kernels and teacher_logits.dtype in kernels and logits.shape[0] > 0
             and use_fused(logits, teacher_ids, teacher_logits)):
-        return _TokenDistillationFn.apply(logits, teacher_ids, teacher_logits, temperature)
+        if torch.is_grad_enabled() and logits.requires_grad:
+            return _TokenDistillationFn.apply(logits, teacher_ids, teacher_logits, temperature)
+        from . import native
+
+        return native.distill_fwd(logits, teacher_ids.contiguous(), teacher_logits.contiguous(), temperature)[0]
     return token_distillation_ref(logits, teacher_ids, teacher_logits, temperature)

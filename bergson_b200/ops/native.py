@@ -18,6 +18,7 @@ _BUILD_DIR = Path(__file__).resolve().parent / "_build"
 _EXT_NAME = "bergson_b200_C"
 _mod = None
 _load_error: Exception | None = None
+_found_device = False
 
 
 def extension_path() -> Path:
@@ -46,10 +47,14 @@ def _load():
 
 def available() -> bool:
     """Whether the fused kernels can run in this process."""
-    if not torch.cuda.is_available():
-        return False
+    global _found_device
     if os.environ.get("BERGSON_B200_DISABLE_NATIVE") == "1":
         return False
+    if _found_device and _mod is not None:  # every operator asks: the rest holds once it held
+        return True
+    if not torch.cuda.is_available():
+        return False
+    _found_device = True
     mod = _load()
     if mod is None:
         if os.environ.get("BERGSON_B200_ALLOW_FALLBACK") == "1":

@@ -90,13 +90,14 @@ class PackedSequences:
         self.device = table.device
         (self.query_tiles, self.query_pairs, self.key_tiles, self.first_key, self.end_query, self.position,
          self.cu_seqlens) = table.split([x.size for x in parts])
+        self._tables = (self.first_key, self.end_query, self.query_tiles, self.query_pairs, self.key_tiles)
 
     def __repr__(self) -> str:
         return f"PackedSequences({len(self.lengths)} documents, {self.num_tokens} tokens, {self.rows} rows)"
 
     def tables(self):
         """What the attention kernels read of the plan."""
-        return self.first_key, self.end_query, self.query_tiles, self.query_pairs, self.key_tiles
+        return self._tables
 
     def spans(self):
         """(begin, end) of each document that has tokens."""
@@ -115,21 +116,26 @@ class PackedSequences:
         return labels.masked_fill(~own.to(labels.device), ignore_index)
 
 
-def _check(name: str, packing: PackedSequences, *tensors: Tensor) -> None:
-    if not isinstance(packing, PackedSequences):
+def _check(name: str, packing: PackedSequences, q: Tensor, *others: Tensor) -> None:
+    if type(packing) is not PackedSequences and not isinstance(packing, PackedSequences):
         raise TypeError(f"{name}: packing must be a PackedSequences, got {type(packing).__name__}")
-    q = tensors[0]
-    for t in tensors:
+    for t in (q, *others):
         if t.ndim != 3:
             raise ValueError(f"{name}: [tokens, heads, features] expected, got shape {tuple(t.shape)}")
         if t.dtype != q.dtype or t.device != q.device or not t.is_floating_point():
             raise ValueError(f"{name}: operands of one floating-point dtype and one device expected")
-        if t.shape[0] != packing.rows:
-            raise ValueError(f"{name}: {t.shape[0]} rows for a packing of {packing.rows}")
-        if t.shape[2] != q.shape[2] or t.shape[2] == 0:
-            raise ValueError(f"{name}: head sizes {q.shape[2]} and {t.shape[2]}")
+        rows, _, dim = t.shape
+        if rows != packing.rows:
+            raise ValueError(f"{name}: {rows} rows for a packing of {packing.rows}")
+        if dim != q.shape[2] or dim == 0:
+            raise ValueError(f"{name}: head sizes {q.shape[2]} and {dim}")
     if q.is_cuda and packing.device != q.device:
         raise ValueError(f"{name}: packing on {packing.device}, operands on {q.device}")
+
+
+def _tracked(*tensors: Tensor) -> bool:
+    """Whether a graph is being built through these operands."""
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
 # --------------------------------------------------------------------------- #
@@ -155,8 +161,8 @@ class _PackedAttentionFn(torch.autograd.Function):
         from . import native
 
         p = packing
-        o, bias2 = native.packed_attention_fwd(q, k, v, *p.tables(), p.num_tokens, scale)
-        ctx.save_for_backward(q, k, v, o, bias2)
+        o, bias2, *rest = native.packed_attention_fwd(q, k, v, *p.tables(), p.num_tokens, scale, True)
+        ctx.save_for_backward(q, k, v, o, bias2, *rest)
         ctx.packing, ctx.scale = packing, scale
         return o
 
@@ -165,9 +171,10 @@ class _PackedAttentionFn(torch.autograd.Function):
     def backward(ctx, d_o):
         from . import native
 
-        q, k, v, o, bias2 = ctx.saved_tensors
+        q, k, v, o, bias2, *rest = ctx.saved_tensors
         p = ctx.packing
-        dq, dk, dv = native.packed_attention_bwd(d_o, q, k, v, o, bias2, *p.tables(), p.num_tokens, ctx.scale)
+        dq, dk, dv = native.packed_attention_bwd(d_o, q, k, v, o, bias2, rest[0] if rest else None, *p.tables(),
+                                                 p.num_tokens, ctx.scale)
         return dq, dk, dv, None, None
 
 
@@ -193,7 +200,11 @@ def packed_causal_attention(q: Tensor, k: Tensor, v: Tensor, packing: PackedSequ
     if q.dtype in _KERNEL_DTYPES and q.shape[2] % 8 == 0 and q.shape[2] <= 128 and use_fused(q, k, v):
         if q.numel() == 0:
             return q * 1.0  # no rows or no heads: nothing to launch
-        return _PackedAttentionFn.apply(q, k, v, packing, scale)
+        if _tracked(q, k, v):
+            return _PackedAttentionFn.apply(q, k, v, packing, scale)
+        from . import native
+
+        return native.packed_attention_fwd(q, k, v, *packing.tables(), packing.num_tokens, scale, False)[0]
     return packed_causal_attention_ref(q, k, v, packing, scale)
 
 
@@ -242,7 +253,12 @@ def packed_rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, rot_dim: int,
     if cos.requires_grad or sin.requires_grad:
         raise ValueError("packed_rotary: the tables get no gradient")
     if q.dtype in _KERNEL_DTYPES and q.shape[2] <= 256 and use_fused(q, k) and q.numel() and k.numel():
-        return _PackedRotaryFn.apply(q, k, cos.float().contiguous(), sin.float().contiguous(), packing.position, rot_dim)
+        cos, sin = cos.float().contiguous(), sin.float().contiguous()
+        if _tracked(q, k):
+            return _PackedRotaryFn.apply(q, k, cos, sin, packing.position, rot_dim)
+        from . import native
+
+        return tuple(native.packed_rotary(q, k, cos, sin, packing.position, rot_dim, False))
     at = packing.position.to(q.device, torch.int64)
     c, s = cos[at][:, None].to(q.dtype), sin[at][:, None].to(q.dtype)
     return rotary_pairs(q, c, s, rot_dim), rotary_pairs(k, c, s, rot_dim)
