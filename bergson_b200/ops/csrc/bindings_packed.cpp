@@ -64,7 +64,7 @@ BgnPackedAttention packed_args(const at::Tensor& q, const at::Tensor& k, const a
   TORCH_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device(),
               "bergson_b200: k and v must be alike");
   TORCH_CHECK(rows < (int64_t(1) << 30) && valid >= 0 && valid <= rows, "bergson_b200: row count out of range");
-  TORCH_CHECK(2 * tiles * q.size(1) < (int64_t(1) << 31), "bergson_b200: too many tiles for one launch");
+  TORCH_CHECK(4 * tiles * q.size(1) < (int64_t(1) << 31), "bergson_b200: too many tiles for one launch");
   check_index(first_key, rows, q);
   check_index(end_query, rows, q);
   check_index(query_tiles, 4 * tiles, q);

@@ -180,6 +180,10 @@ cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const void* o
   e = sm_count(&sms);
   if (e != cudaSuccess) return e;
   const int tiles = (a.rows + kTile - 1) / kTile;
+  constexpr int kLanes = DP / 8;
+  packed_delta_kernel<FMT, kLanes><<<unsigned(4 * tiles) * unsigned(a.heads), 32 * kLanes, 0, stream>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
   p.tiles = reinterpret_cast<const int4*>(a.query_tiles);
   p.units = tiles * a.heads;
   kq<<<unsigned(p.units < sms ? p.units : sms), kBwdThreads, dq_smem_bytes<DP>(), stream>>>(mq, mg, mk, mv, p, status);

@@ -3,7 +3,7 @@
 //   P = 2^(c q.k + bias2),  delta_t = do_t . o_t,  dS = P (do.v - delta)
 //   dQ = scale dS k,   dK = scale dS^T q,   dV = P^T do      (dK, dV summed over the heads of a group)
 //
-// Two kernels, each of which keeps its sums in TMEM from the first to the last tile: one block for the
+// After a small one for delta, two kernels, each of which keeps its sums in TMEM from the first to the last tile: one block for the
 // rows of dQ, one for the rows of dK and dV.  P is computed in both: that is seven products for the
 // five of the mathematics, and buys sums in one order (the results are the same in every run) without
 // a fp32 copy of dQ in memory.  Tiles are cut from the packed axis as in the forward pass.
@@ -68,6 +68,47 @@ __device__ __forceinline__ float2 score_gradient(uint32_t p0, uint32_t p1, uint3
   return FMT == 0 ? mul2(x, factor) : x;
 }
 
+// ---- delta ----------------------------------------------------------------------------
+//
+// delta = do . o, with what rounding took from o: dS is a difference against delta, and for rows with few
+// keys that rounding would be its largest error.  A block has 32 rows of a head, LANES lanes to a row.
+// HBM bounds it: o, its rest and do are read once.
+
+template <int FMT, int LANES>
+__global__ void __launch_bounds__(32 * LANES) packed_delta_kernel(const __grid_constant__ PackedBwdArgs p) {
+  using T = typename Type16<FMT>::T;
+  __shared__ float tops[LANES];
+  const int head = blockIdx.x % p.heads, row0 = blockIdx.x / p.heads * 32;
+  const int lane = threadIdx.x % LANES, row = row0 + threadIdx.x / LANES, f = 8 * lane;
+  float sum = 0.f, top = 0.f;
+  if (row < p.valid && f < p.dim) {
+    const long from = (long(row) * p.heads + head) * p.dim + f;
+    union { uint4 u; T h[8]; } o, rest, g;
+    o.u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.o) + from));
+    rest.u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.o_rest) + from));
+    g.u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.d_o) + long(row) * p.do_tok + long(head) * p.do_head + f));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = to_float<T>(g.h[e]);
+      sum = fmaf(-to_float<T>(o.h[e]) - to_float<T>(rest.h[e]), x, sum);
+      top = fmaxf(top, fabsf(x));
+    }
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const long at = long(head) * p.pitch + row;
+  if (lane == 0) p.neg_delta[at] = sum;  // zero where there is no row
+  if (FMT == 0) {
+    top = warp_max(top);
+    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < LANES; ++w) top = fmaxf(top, tops[w]);
+      p.do_max[at / 32] = top;
+    }
+  }
+}
+
 // ---- dQ -------------------------------------------------------------------------------
 //
 // A unit is one tile of 128 query rows of a head.  Per key tile: S = q k^T and dP = do v^T, the softmax
@@ -77,13 +118,17 @@ __device__ __forceinline__ float2 score_gradient(uint32_t p0, uint32_t p1, uint3
 // TMEM: dQ, S, dP twice (128 columns each; dS in 16 bits over its dP).  Shared memory: q, do, three
 // key and two value tiles (7 tiles of 32 KB at 128 features).  Warps 0-7: softmax, warps 0-3 on the first 64 keys of a tile, 4-7 on the rest;
 // two threads share a row.  8 TMA, 9 MMA.
+//
+// Delta comes from a kernel of its own: read here, by softmax warps or by others, o and do took as long as
+// two to four key tiles, as loads through the first-level cache wait for the tensor core's operands.
 
 constexpr int kDqKStages = 3;  // a key tile stays until dQ of its step, which comes after S and dP of the next
 constexpr int kDqVStages = 2;
+constexpr int kDqRowFloats = 2 * kTile;  // of a unit: -delta, bias2
 
 template <int DP>
 constexpr int dq_smem_bytes() {
-  return (2 + kDqKStages + kDqVStages) * tile_bytes<DP>() + 4 * kTile * 4 + 256;
+  return (2 + kDqKStages + kDqVStages) * tile_bytes<DP>() + kDqRowFloats * 4 + 256;
 }
 
 // One half of the features of a row of dQ.
@@ -127,9 +172,9 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   uint8_t* g_tile = q_tile + kTileBytes;
   uint8_t* k_tiles = g_tile + kTileBytes;
   uint8_t* v_tiles = k_tiles + kDqKStages * kTileBytes;
-  float* halves = reinterpret_cast<float*>(v_tiles + kDqVStages * kTileBytes);  // [half][-delta, |do|][row]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(halves + 4 * kTile);
-  uint64_t* q_full = bars;  // q and do
+  float* row_values = reinterpret_cast<float*>(v_tiles + kDqVStages * kTileBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(row_values + kDqRowFloats);
+  uint64_t* q_full = bars;  // q, do and the row values
   uint64_t* q_empty = q_full + 1;
   uint64_t* k_full = q_empty + 1;  // [3]
   uint64_t* k_empty = k_full + kDqKStages;
@@ -147,7 +192,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 9);  // the MMA warp's commit and the softmax warps, which read do
+    mbar_init(q_empty, 9);  // the MMA warp's commit and the softmax warps, which read the row values
     for (int s = 0; s < kDqKStages; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
@@ -195,15 +240,18 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           ok = mbar_wait_bounded(&k_empty[st], ((j / kDqKStages) & 1) ^ 1);
           if (!ok) break;
           mbar_expect_tx(&k_full[st], kTileBytes);
-#pragma unroll
+  #pragma unroll
           for (int s = 0; s < kSlabs; ++s)
             tma_load_3d(k_tiles + st * kTileBytes + s * kSlabBytes, &map_k, &k_full[st], 64 * s, kv_head, key);
           if (i == 0) {
             ok = mbar_wait_bounded(q_empty, (uses & 1) ^ 1);
             if (!ok) break;
             ++uses;
-            mbar_expect_tx(q_full, 2 * kTileBytes);
-#pragma unroll
+            mbar_expect_tx(q_full, 2 * kTileBytes + 4 * kDqRowFloats);
+            // whole tiles of rows to a head, so the copies stay inside
+            bulk_load(row_values, p.neg_delta + long(head) * p.pitch + entry.x, 4 * kTile, q_full);
+            bulk_load(row_values + kTile, p.bias2 + long(head) * p.pitch + entry.x, 4 * kTile, q_full);
+  #pragma unroll
             for (int s = 0; s < kSlabs; ++s) {
               tma_load_3d(q_tile + s * kSlabBytes, &map_q, q_full, 64 * s, head, entry.x);
               tma_load_3d(g_tile + s * kSlabBytes, &map_do, q_full, 64 * s, head, entry.x);
@@ -212,7 +260,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           ok = mbar_wait_bounded(&v_empty[vst], ((j / kDqVStages) & 1) ^ 1);
           if (!ok) break;
           mbar_expect_tx(&v_full[vst], kTileBytes);
-#pragma unroll
+  #pragma unroll
           for (int s = 0; s < kSlabs; ++s)
             tma_load_3d(v_tiles + vst * kTileBytes + s * kSlabBytes, &map_v, &v_full[vst], 64 * s, kv_head, key);
         }
@@ -235,7 +283,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const uint64_t dk_mn = make_mnmajor_sw128_desc(smem_u32(k_tiles), kSlabBytes);
     constexpr uint64_t kStage = kTileBytes >> 4;
     const auto scores = [&](uint32_t tmem_d, uint64_t a, uint64_t b) {  // one thread
-#pragma unroll
+  #pragma unroll
       for (int k = 0; k < DP / 16; ++k) {
         const uint64_t off = uint64_t(((k / 4) * kSlabBytes + (k % 4) * 32) >> 4);
         umma_f16(tmem_d, a + off, b + off, idesc_s, k > 0 ? 1u : 0u);
@@ -250,7 +298,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const uint64_t b = dk_mn + st * kStage;
       const uint32_t a = tmem_dp + 128 * (jj & 1);
       if (elect_one()) {
-#pragma unroll
+  #pragma unroll
         for (int k = 0; k < kTile / 16; ++k)
           umma_f16_ts(tmem_dq, a + (k / 4) * 64 + (k % 4) * 8, b + uint64_t((2048 * k) >> 4), idesc_dq,
                       (!first || k > 0) ? 1u : 0u);
@@ -315,65 +363,18 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const bool in = row < p.valid;
       const long at = (long(row) * p.heads + head) * p.dim;
       const int first = in ? __ldg(p.first_key + row) : 0x7fffffff;
-      const float bias2 = in ? p.bias2[long(head) * p.pitch + row] : -INFINITY;
       const int all_from = __shfl_sync(0xffffffffu, first, 31);
 
-      // delta = do . o, with what rounding took from o: dS is a difference against delta, and for rows with few
-      // keys that rounding would be its largest error.  o comes from memory, asked for before do arrives in
-      // shared memory (swizzled rows of 128 bytes).  Each of the two threads of a row takes half of the
-      // features.
-      float neg_delta = 0.f, factor = 1.f;
+      float neg_delta = 0.f, bias2 = -INFINITY, factor = 1.f;
       if (n > 0) {
-        constexpr int kPackets = DP / 16;
-        uint4 o_row[kPackets], r_row[kPackets];
-        const T* orow = static_cast<const T*>(p.o) + at;
-        const T* rrow = static_cast<const T*>(p.o_rest) + at;
-#pragma unroll
-        for (int d = 0; d < kPackets; ++d) {
-          const int f = 8 * (d + half * kPackets);
-          const bool there = in && f < p.dim;
-          o_row[d] = there ? __ldg(reinterpret_cast<const uint4*>(orow + f)) : make_uint4(0, 0, 0, 0);
-          r_row[d] = there ? __ldg(reinterpret_cast<const uint4*>(rrow + f)) : make_uint4(0, 0, 0, 0);
-        }
         ok = warp_wait(q_full, count & 1);
         if (!ok) break;
-        float top = 0.f;
-        if (in) {
-          const uint8_t* g = g_tile + tile_row * 128;
-#pragma unroll
-          for (int d = 0; d < kPackets; ++d) {
-            const int k = d + half * kPackets;
-            if (8 * k >= p.dim) continue;
-            union { uint4 u; T h[8]; } a, b, c;
-            a.u = o_row[d];
-            b.u = *reinterpret_cast<const uint4*>(g + (k / 8) * kSlabBytes + (((k % 8) ^ (tile_row & 7)) << 4));
-            c.u = r_row[d];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float x = to_float<T>(b.h[e]);
-              neg_delta = fmaf(-to_float<T>(a.h[e]) - to_float<T>(c.h[e]), x, neg_delta);
-              top = fmaxf(top, fabsf(x));
-            }
-          }
-        }
-        // Read again only after dQ of this unit, for which every softmax warp is done with them.
-        halves[half * 2 * kTile + tile_row] = neg_delta;
-        if (FMT == 0) halves[half * 2 * kTile + kTile + tile_row] = top;
-        named_barrier_sync(1, 256);
-        const float* other = halves + (1 - half) * 2 * kTile + tile_row;
-        neg_delta = half ? other[0] + neg_delta : neg_delta + other[0];
-        if (FMT == 0) top = fmaxf(top, other[kTile]);
+        neg_delta = row_values[tile_row];
+        bias2 = in ? row_values[kTile + tile_row] : -INFINITY;
+        if (FMT == 0) factor = power_below_one(p.do_max[(long(head) * p.pitch + warp_row0) / 32]);
         __syncwarp();
         if (lane == 0) mbar_arrive(q_empty);
-        if (FMT == 0) {
-          top = warp_max(top);
-          factor = power_below_one(top);
-          if (half == 0 && lane == 0) p.do_max[(long(head) * p.pitch + warp_row0) / 32] = top;
-        }
-      } else if (FMT == 0 && half == 0 && lane == 0) {
-        p.do_max[(long(head) * p.pitch + warp_row0) / 32] = 0.f;
       }
-      if (half == 0 && row < p.rows) p.neg_delta[long(head) * p.pitch + row] = neg_delta;
       const float ds_factor = FMT == 0 ? factor * (1.f / 1024.f) : 1.f;
       const bool lone = first == row;  // one key: P = 1, and nothing goes through the softmax
       const float2 c2 = make_float2(c, c), b2 = make_float2(bias2, bias2), d2 = make_float2(neg_delta, neg_delta);
