@@ -15,6 +15,7 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
+from ..ops.packed import PackedSequences
 from ..utils.math import weighted_causal_lm_ce
 
 
@@ -134,12 +135,19 @@ class NativeCausalLM(nn.Module):
     def gradient_checkpointing_enable(self, **_):
         self.gradient_checkpointing = True
 
-    def hidden(self, input_ids: Tensor) -> Tensor:
-        """Final-norm hidden states ``[B, S, d]``."""
+    def hidden(self, input_ids: Tensor, packing: PackedSequences | None = None) -> Tensor:
+        """Final-norm hidden states ``[B, S, d]``.  With ``packing`` the one row of ``input_ids`` holds
+        documents that lie one behind the other: each starts at position 0 and attends itself alone."""
         raise NotImplementedError
 
-    def forward(self, input_ids: Tensor, labels: Tensor | None = None, **kwargs) -> CausalLMOutput:
-        h = self.hidden(input_ids)
+    def forward(self, input_ids: Tensor, labels: Tensor | None = None, packing: PackedSequences | None = None,
+                **kwargs) -> CausalLMOutput:
+        if packing is None:
+            h = self.hidden(input_ids)
+        else:
+            h = self.hidden(input_ids, packing)
+            if labels is not None:  # no token predicts the first one of the next document
+                labels = packing.mask_labels(labels)
         head = self.get_output_embeddings()
         V = self.config.vocab_size
         ours = getattr(self.loss_function, "func", self.loss_function) is weighted_causal_lm_ce
@@ -214,6 +222,15 @@ class Conv1D(nn.Module):
 
     def extra_repr(self) -> str:
         return f"nf={self.nf}, nx={self.nx}"
+
+
+def positions_needed(input_ids: Tensor, packing: PackedSequences | None) -> int:
+    """Positions that the tokens of a batch take: the row length, or the longest document's."""
+    if packing is None:
+        return input_ids.shape[1]
+    if input_ids.ndim != 2 or tuple(input_ids.shape) != (1, packing.rows):
+        raise ValueError(f"packed documents come as one row of {packing.rows} tokens, got {tuple(input_ids.shape)}")
+    return max(1, packing.max_length)
 
 
 def maybe_checkpoint(module: NativeCausalLM, fn, *args):

@@ -8,7 +8,7 @@ import torch.nn as nn
 from torch import Tensor
 
 from .. import ops
-from .common import Backbone, Conv1D, ModelArgs, NativeCausalLM, maybe_checkpoint
+from .common import Backbone, Conv1D, ModelArgs, NativeCausalLM, maybe_checkpoint, positions_needed
 
 
 class _LN(nn.LayerNorm):
@@ -24,10 +24,13 @@ class GPT2Attention(nn.Module):
         self.c_attn = Conv1D(3 * d, d)
         self.c_proj = Conv1D(d, d)
 
-    def forward(self, x: Tensor) -> Tensor:
+    def forward(self, x: Tensor, packing: ops.PackedSequences | None = None) -> Tensor:
         B, S, d = x.shape
         q, k, v = self.c_attn(x).split(d, dim=2)
         shape = (B, S, self.num_heads, self.head_dim)
+        if packing is not None:
+            o = ops.packed_causal_attention(q.view(shape)[0], k.view(shape)[0], v.view(shape)[0], packing)
+            return self.c_proj(o.reshape(B, S, d))
         o = ops.causal_attention(
             q.view(shape).transpose(1, 2), k.view(shape).transpose(1, 2), v.view(shape).transpose(1, 2)
         )
@@ -52,8 +55,8 @@ class GPT2Block(nn.Module):
         self.ln_2 = _LN(cfg.hidden_size, eps=cfg.layer_norm_eps)
         self.mlp = GPT2MLP(cfg)
 
-    def forward(self, x: Tensor) -> Tensor:
-        x = x + self.attn(self.ln_1(x))
+    def forward(self, x: Tensor, packing: ops.PackedSequences | None = None) -> Tensor:
+        x = x + self.attn(self.ln_1(x), packing)
         return x + self.mlp(self.ln_2(x))
 
 
@@ -82,10 +85,16 @@ class GPT2LMHeadModel(NativeCausalLM):
     def get_output_embeddings(self):
         return self.lm_head
 
-    def hidden(self, input_ids: Tensor) -> Tensor:
+    def hidden(self, input_ids: Tensor, packing: ops.PackedSequences | None = None) -> Tensor:
         t = self.transformer
-        pos = torch.arange(input_ids.shape[1], device=input_ids.device)
+        needed = positions_needed(input_ids, packing)
+        if packing is None:
+            pos = torch.arange(needed, device=input_ids.device)
+        else:
+            if needed > t.wpe.num_embeddings:
+                raise ValueError(f"documents of up to {needed} tokens, {t.wpe.num_embeddings} learned positions")
+            pos = packing.position.to(input_ids.device)
         x = t.wte(input_ids) + t.wpe(pos)[None]
         for block in t.h:
-            x = maybe_checkpoint(self, block, x)
+            x = maybe_checkpoint(self, block, x, packing)
         return t.ln_f(x)

@@ -8,7 +8,7 @@ import torch.nn as nn
 from torch import Tensor
 
 from .. import ops
-from .common import Backbone, ModelArgs, NativeCausalLM, maybe_checkpoint
+from .common import Backbone, ModelArgs, NativeCausalLM, maybe_checkpoint, positions_needed
 
 
 class _LN(nn.LayerNorm):
@@ -27,10 +27,13 @@ class NeoXAttention(nn.Module):
         self.query_key_value = ops.Linear(d, 3 * d, bias=True)
         self.dense = ops.Linear(d, d, bias=True)
 
-    def forward(self, x: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
+    def forward(self, x: Tensor, cos: Tensor, sin: Tensor, packing: ops.PackedSequences | None = None) -> Tensor:
         B, S, _ = x.shape
         qkv = self.query_key_value(x).view(B, S, self.num_heads, 3 * self.head_dim)
         q, k, v = qkv.split(self.head_dim, dim=-1)  # each [B, S, H, D]
+        if packing is not None:
+            q, k = ops.packed_rotary(q[0], k[0], cos, sin, self.rot_dim, packing)
+            return self.dense(ops.packed_causal_attention(q, k, v[0], packing).reshape(B, S, -1))
         q = ops.rotary(q, cos, sin, self.rot_dim)
         k = ops.rotary(k, cos, sin, self.rot_dim)
         o = ops.causal_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
@@ -56,8 +59,8 @@ class NeoXLayer(nn.Module):
         self.attention = NeoXAttention(cfg)
         self.mlp = NeoXMLP(cfg)
 
-    def forward(self, x: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
-        a = self.attention(self.input_layernorm(x), cos, sin)
+    def forward(self, x: Tensor, cos: Tensor, sin: Tensor, packing: ops.PackedSequences | None = None) -> Tensor:
+        a = self.attention(self.input_layernorm(x), cos, sin, packing)
         if self.parallel:
             return x + a + self.mlp(self.post_attention_layernorm(x))
         x = x + a
@@ -87,11 +90,11 @@ class GPTNeoXForCausalLM(NativeCausalLM):
     def get_output_embeddings(self):
         return self.embed_out
 
-    def hidden(self, input_ids: Tensor) -> Tensor:
+    def hidden(self, input_ids: Tensor, packing: ops.PackedSequences | None = None) -> Tensor:
         m = self.gpt_neox
         x = m.embed_in(input_ids)
         rot = m.layers[0].attention.rot_dim
-        cos, sin = ops.rotary_tables(input_ids.shape[1], rot, self.config.rope_theta, x.device)
+        cos, sin = ops.rotary_tables(positions_needed(input_ids, packing), rot, self.config.rope_theta, x.device)
         for layer in m.layers:
-            x = maybe_checkpoint(self, layer, x, cos, sin)
+            x = maybe_checkpoint(self, layer, x, cos, sin, packing)
         return m.final_layer_norm(x)

@@ -7,7 +7,7 @@ import torch.nn as nn
 from torch import Tensor
 
 from .. import ops
-from .common import Backbone, ModelArgs, NativeCausalLM, maybe_checkpoint
+from .common import Backbone, ModelArgs, NativeCausalLM, maybe_checkpoint, positions_needed
 
 
 class LlamaRMSNorm(nn.Module):
@@ -31,7 +31,7 @@ class LlamaAttention(nn.Module):
         self.o_proj = ops.Linear(self.num_heads * hd, d, bias=cfg.attention_bias)
         self.tp_group = None  # set by parallel.tensor_parallel.apply_tensor_parallel
 
-    def forward(self, x: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
+    def forward(self, x: Tensor, cos: Tensor, sin: Tensor, packing: ops.PackedSequences | None = None) -> Tensor:
         B, S, _ = x.shape
         if self.tp_group is not None:
             from ..parallel.tensor_parallel import copy_to_group, reduce_from_group
@@ -40,6 +40,10 @@ class LlamaAttention(nn.Module):
         q = self.q_proj(x).view(B, S, self.num_heads, self.head_dim)
         k = self.k_proj(x).view(B, S, self.kv_heads, self.head_dim)
         v = self.v_proj(x).view(B, S, self.kv_heads, self.head_dim)
+        if packing is not None:
+            q, k = ops.packed_rotary(q[0], k[0], cos, sin, self.head_dim, packing)
+            out = self.o_proj(ops.packed_causal_attention(q, k, v[0], packing).reshape(B, S, -1))
+            return reduce_from_group(out, self.tp_group) if self.tp_group is not None else out
         q = ops.rotary(q, cos, sin, self.head_dim)
         k = ops.rotary(k, cos, sin, self.head_dim)
         o = ops.causal_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
@@ -97,8 +101,8 @@ class LlamaDecoderLayer(nn.Module):
         self.input_layernorm = LlamaRMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
         self.post_attention_layernorm = LlamaRMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
 
-    def forward(self, x: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
-        x = x + self.self_attn(self.input_layernorm(x), cos, sin)
+    def forward(self, x: Tensor, cos: Tensor, sin: Tensor, packing: ops.PackedSequences | None = None) -> Tensor:
+        x = x + self.self_attn(self.input_layernorm(x), cos, sin, packing)
         return x + self.mlp(self.post_attention_layernorm(x))
 
     def forward_seq_parallel(self, x: Tensor, cos: Tensor, sin: Tensor, sp, lead) -> Tensor:
@@ -132,17 +136,17 @@ class LlamaForCausalLM(NativeCausalLM):
     def get_output_embeddings(self):
         return self.lm_head
 
-    def hidden(self, input_ids: Tensor) -> Tensor:
+    def hidden(self, input_ids: Tensor, packing: ops.PackedSequences | None = None) -> Tensor:
         m = self.model
-        sp = self._seq_parallel_for(input_ids)
+        sp = self._seq_parallel_for(input_ids) if packing is None else None
         if sp is not None:
             return self._hidden_seq_parallel(input_ids, sp)
         x = m.embed_tokens(input_ids)
         cos, sin = ops.rotary_tables(
-            input_ids.shape[1], self.config.head_dim, self.config.rope_theta, x.device
+            positions_needed(input_ids, packing), self.config.head_dim, self.config.rope_theta, x.device
         )
         for layer in m.layers:
-            x = maybe_checkpoint(self, layer, x, cos, sin)
+            x = maybe_checkpoint(self, layer, x, cos, sin, packing)
         return m.norm(x)
 
     def _seq_parallel_for(self, input_ids: Tensor):

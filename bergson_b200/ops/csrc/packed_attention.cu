@@ -1,5 +1,7 @@
 // Host side of the attention over packed documents.
 #include <mutex>
+#include <set>
+#include <utility>
 
 #include "packed_bwd.cuh"
 #include "packed_fwd.cuh"
@@ -16,9 +18,18 @@ cudaError_t sm_count(int* n) {
   return e == cudaSuccess ? cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, device) : e;
 }
 
-// cudaFuncSetAttribute holds for the current device only.
+// cudaFuncSetAttribute holds for the current device only; it is asked for once per kernel and device.
 cudaError_t allow_smem(const void* kernel, int bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({kernel, device})) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.insert({kernel, device});
+  return e;
 }
 
 template <typename T, int DP>
@@ -207,7 +218,10 @@ extern "C" int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, vo
                                         cudaStream_t stream) {
   if (!sound(a)) return int(cudaErrorInvalidValue);
   const bool narrow = a->dim <= 64;
-  if (a->type == 2) return int(narrow ? simple_fwd<float, 64>(*a, o, bias2, stream) : simple_fwd<float, 128>(*a, o, bias2, stream));
+  if (a->type == 2) {
+    auto run = a->dim <= 32 ? simple_fwd<float, 32> : (narrow ? simple_fwd<float, 64> : simple_fwd<float, 128>);
+    return int(run(*a, o, bias2, stream));
+  }
   if (a->type == 1)
     return int(narrow ? tensor_fwd<1, 64>(*a, o, o_rest, bias2, status, stream) : tensor_fwd<1, 128>(*a, o, o_rest, bias2, status, stream));
   return int(narrow ? tensor_fwd<0, 64>(*a, o, o_rest, bias2, status, stream) : tensor_fwd<0, 128>(*a, o, o_rest, bias2, status, stream));
@@ -219,9 +233,10 @@ extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void*
                                         void* dv, int* status, cudaStream_t stream) {
   if (!sound(a)) return int(cudaErrorInvalidValue);
   const bool narrow = a->dim <= 64;
-  if (a->type == 2)
-    return int(narrow ? simple_bwd<float, 64>(*a, o, bias2, d_o, do_tok, do_head, delta, dq, dk, dv, stream)
-                      : simple_bwd<float, 128>(*a, o, bias2, d_o, do_tok, do_head, delta, dq, dk, dv, stream));
+  if (a->type == 2) {
+    auto run = a->dim <= 32 ? simple_bwd<float, 32> : (narrow ? simple_bwd<float, 64> : simple_bwd<float, 128>);
+    return int(run(*a, o, bias2, d_o, do_tok, do_head, delta, dq, dk, dv, stream));
+  }
   auto run = a->type == 1 ? (narrow ? tensor_bwd<1, 64> : tensor_bwd<1, 128>)
                           : (narrow ? tensor_bwd<0, 64> : tensor_bwd<0, 128>);
   if (o_rest == nullptr) return int(cudaErrorInvalidValue);

@@ -17,6 +17,7 @@ import numpy as np
 import torch
 from torch import Tensor
 
+from . import native
 from .functional import causal_attention_ref, rotary_pairs, use_fused
 
 _TILE = 128  # rows of the kernels' tiles
@@ -119,16 +120,16 @@ class PackedSequences:
 def _check(name: str, packing: PackedSequences, q: Tensor, *others: Tensor) -> None:
     if type(packing) is not PackedSequences and not isinstance(packing, PackedSequences):
         raise TypeError(f"{name}: packing must be a PackedSequences, got {type(packing).__name__}")
+    dtype, device, rows = q.dtype, q.device, packing.rows
     for t in (q, *others):
         if t.ndim != 3:
             raise ValueError(f"{name}: [tokens, heads, features] expected, got shape {tuple(t.shape)}")
-        if t.dtype != q.dtype or t.device != q.device or not t.is_floating_point():
+        if t.dtype != dtype or t.device != device or not dtype.is_floating_point:
             raise ValueError(f"{name}: operands of one floating-point dtype and one device expected")
-        rows, _, dim = t.shape
-        if rows != packing.rows:
-            raise ValueError(f"{name}: {rows} rows for a packing of {packing.rows}")
-        if dim != q.shape[2] or dim == 0:
-            raise ValueError(f"{name}: head sizes {q.shape[2]} and {dim}")
+        if t.shape[0] != rows:
+            raise ValueError(f"{name}: {t.shape[0]} rows for a packing of {rows}")
+        if t.shape[2] != q.shape[2] or t.shape[2] == 0:
+            raise ValueError(f"{name}: head sizes {q.shape[2]} and {t.shape[2]}")
     if q.is_cuda and packing.device != q.device:
         raise ValueError(f"{name}: packing on {packing.device}, operands on {q.device}")
 
@@ -158,8 +159,6 @@ def packed_causal_attention_ref(q: Tensor, k: Tensor, v: Tensor, packing: Packed
 class _PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, packing, scale):
-        from . import native
-
         p = packing
         o, bias2, *rest = native.packed_attention_fwd(q, k, v, *p.tables(), p.num_tokens, scale, True)
         ctx.save_for_backward(q, k, v, o, bias2, *rest)
@@ -169,8 +168,6 @@ class _PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o):
-        from . import native
-
         q, k, v, o, bias2, *rest = ctx.saved_tensors
         p = ctx.packing
         dq, dk, dv = native.packed_attention_bwd(d_o, q, k, v, o, bias2, rest[0] if rest else None, *p.tables(),
@@ -197,13 +194,11 @@ def packed_causal_attention(q: Tensor, k: Tensor, v: Tensor, packing: PackedSequ
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"packed_causal_attention: scale must be positive, got {scale}")
-    if q.dtype in _KERNEL_DTYPES and q.shape[2] % 8 == 0 and q.shape[2] <= 128 and use_fused(q, k, v):
+    if q.dtype in _KERNEL_DTYPES and q.shape[2] % 8 == 0 and q.shape[2] <= 128 and use_fused(q):
         if q.numel() == 0:
             return q * 1.0  # no rows or no heads: nothing to launch
         if _tracked(q, k, v):
             return _PackedAttentionFn.apply(q, k, v, packing, scale)
-        from . import native
-
         return native.packed_attention_fwd(q, k, v, *packing.tables(), packing.num_tokens, scale, False)[0]
     return packed_causal_attention_ref(q, k, v, packing, scale)
 
@@ -216,8 +211,6 @@ def packed_causal_attention(q: Tensor, k: Tensor, v: Tensor, packing: PackedSequ
 class _PackedRotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, cos, sin, position, rot_dim):
-        from . import native
-
         ctx.save_for_backward(cos, sin, position)
         ctx.rot_dim = rot_dim
         return tuple(native.packed_rotary(q, k, cos, sin, position, rot_dim, False))
@@ -225,8 +218,6 @@ class _PackedRotaryFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
-        from . import native
-
         cos, sin, position = ctx.saved_tensors
         dq, dk = native.packed_rotary(dq, dk, cos, sin, position, ctx.rot_dim, True)
         return dq, dk, None, None, None, None
@@ -252,12 +243,10 @@ def packed_rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, rot_dim: int,
         raise ValueError(f"packed_rotary: tables on {cos.device}, operands on {q.device}")
     if cos.requires_grad or sin.requires_grad:
         raise ValueError("packed_rotary: the tables get no gradient")
-    if q.dtype in _KERNEL_DTYPES and q.shape[2] <= 256 and use_fused(q, k) and q.numel() and k.numel():
+    if q.dtype in _KERNEL_DTYPES and q.shape[2] <= 256 and use_fused(q) and q.numel() and k.numel():
         cos, sin = cos.float().contiguous(), sin.float().contiguous()
         if _tracked(q, k):
             return _PackedRotaryFn.apply(q, k, cos, sin, packing.position, rot_dim)
-        from . import native
-
         return tuple(native.packed_rotary(q, k, cos, sin, packing.position, rot_dim, False))
     at = packing.position.to(q.device, torch.int64)
     c, s = cos[at][:, None].to(q.dtype), sin[at][:, None].to(q.dtype)
