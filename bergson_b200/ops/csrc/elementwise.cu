@@ -1075,6 +1075,14 @@ extern "C" int bgn_rmsnorm_bwd(const void* dy, const void* x, const void* w, con
   return int(cudaGetLastError());
 }
 
+extern "C" int bgn_rmsnorm_bwd_load(void) {
+  cudaFuncAttributes a;
+  cudaError_t e = cudaFuncGetAttributes(&a, rmsnorm_bwd_kernel<__half>);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, rmsnorm_bwd_kernel<__nv_bfloat16>);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, rmsnorm_bwd_kernel<float>);
+  return int(e);
+}
+
 extern "C" int bgn_rmsnorm_bwd_bwd(const void* U, const float* Vw, const void* dy, const void* x, const void* w,
                                    const float* rstd, void* d_dy, void* d_x, float* dw_partial, int n_partial,
                                    long rows, int d, int type, cudaStream_t st) {

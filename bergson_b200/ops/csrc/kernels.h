@@ -55,6 +55,9 @@ int bgn_finalize_rows(const float* acc, void* out, const long* row_index, int N,
 
 int bgn_rmsnorm_fwd(const void* x, const void* w, void* y, float* rstd, long rows, int d, float eps,
                     int type, cudaStream_t stream);
+// Loads the kernels of bgn_rmsnorm_bwd on the current device: the first launch of a kernel may need device
+// memory for its code.
+int bgn_rmsnorm_bwd_load(void);
 int bgn_rmsnorm_bwd(const void* dy, const void* x, const void* w, const float* rstd, void* dx,
                     float* dw_partial, int n_partial, long rows, int d, int type,
                     cudaStream_t stream);

@@ -38,7 +38,8 @@ __global__ void sum_partials_kernel(const float* __restrict__ partials, int n_pa
   dw[c] = s;
 }
 
-// Device address of the scratch array on the current device (resolved on first use).
+// Device address of the scratch array on the current device (resolved on first use, when the code of
+// every variant is loaded too: left to their first launches, that could take device memory later).
 int scratch_for_current_device(float** out) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -50,6 +51,10 @@ int scratch_for_current_device(float** out) {
     e = cudaGetSymbolAddress(reinterpret_cast<void**>(&ptr), g_dw_partials);
     if (e != cudaSuccess || ptr == nullptr)
       return fail(int(e == cudaSuccess ? cudaErrorInvalidSymbol : e), "cudaGetSymbolAddress failed (%ld)", long(e));
+    cudaFuncAttributes a;
+    if (int rc = bgn_rmsnorm_bwd_load()) return fail_cuda(rc, "loading the rmsnorm backward failed");
+    if ((e = cudaFuncGetAttributes(&a, sum_partials_kernel)) != cudaSuccess)
+      return fail_cuda(int(e), "loading the partial-sum kernel failed");
     g_scratch_ptr[dev] = ptr;
   }
   *out = g_scratch_ptr[dev];
