@@ -2,6 +2,7 @@
 // allocation of outputs, current-stream lookup.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include "bindings.h"
@@ -145,8 +146,8 @@ std::vector<at::Tensor> packed_attention_bwd(at::Tensor d_o, at::Tensor q, at::T
   return {dq, dk, dv};
 }
 
-std::vector<at::Tensor> packed_rotary(at::Tensor q, at::Tensor k, at::Tensor cos, at::Tensor sin, at::Tensor position,
-                                      int64_t rot, bool inverse) {
+std::vector<at::Tensor> packed_rotary_turn(at::Tensor q, at::Tensor k, at::Tensor cos, at::Tensor sin,
+                                           at::Tensor position, int64_t rot, bool inverse) {
   c10::cuda::CUDAGuard guard(q.device());
   check_packed(q, k);
   check_index(position, q.size(0), q);
@@ -239,12 +240,122 @@ at::Tensor distill_bwd(at::Tensor logits, at::Tensor ids, at::Tensor teacher, at
   return dlogits;
 }
 
+// ---- autograd -------------------------------------------------------------------------
+//
+// The graph nodes are here and not in Python: for small batches their calls cost more than the kernels.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool tracked(std::initializer_list<const at::Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const auto* t : inputs)
+    if (t->requires_grad()) return true;
+  return false;
+}
+
+// Gradients that refuse to be differentiated: the backward kernels have none of their own.
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  auto refuse = std::make_shared<torch::autograd::DelayedError>(
+      std::string("bergson_b200: the gradient of ") + what + " on the kernels cannot be differentiated again; use ops.composable()",
+      int64_t(grads.size()));
+  return (*refuse)(std::move(grads));
+}
+
+struct PackedAttentionFn : torch::autograd::Function<PackedAttentionFn> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor first_key,
+                            at::Tensor end_query, at::Tensor query_tiles, at::Tensor query_pairs, at::Tensor key_tiles,
+                            int64_t valid, double scale) {
+    auto out = packed_attention_fwd(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale, true);
+    if (out.size() < 3) out.emplace_back();
+    ctx->save_for_backward({q, k, v, out[0], out[1], out[2], first_key, end_query, query_tiles, query_pairs, key_tiles});
+    ctx->saved_data["valid"] = valid;
+    ctx->saved_data["scale"] = scale;
+    return out[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    variable_list out(3);
+    {
+      at::AutoGradMode off(false);
+      c10::optional<at::Tensor> rest;
+      if (s[5].defined()) rest = s[5];
+      out = packed_attention_bwd(grads[0], s[0], s[1], s[2], s[3], s[4], rest, s[6], s[7], s[8], s[9], s[10],
+                                 ctx->saved_data["valid"].toInt(), ctx->saved_data["scale"].toDouble());
+    }
+    out = once(std::move(out), "packed_causal_attention");
+    out.resize(10);
+    return out;
+  }
+};
+
+at::Tensor packed_attention(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor first_key, at::Tensor end_query,
+                            at::Tensor query_tiles, at::Tensor query_pairs, at::Tensor key_tiles, int64_t valid,
+                            double scale) {
+  if (tracked({&q, &k, &v}))
+    return PackedAttentionFn::apply(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale);
+  return packed_attention_fwd(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale, false)[0];
+}
+
+struct PackedRotaryFn : torch::autograd::Function<PackedRotaryFn> {
+  static variable_list forward(AutogradContext* ctx, at::Tensor q, at::Tensor k, at::Tensor cos, at::Tensor sin,
+                               at::Tensor position, int64_t rot) {
+    ctx->save_for_backward({cos, sin, position});
+    ctx->saved_data["rot"] = rot;
+    return packed_rotary_turn(q, k, cos, sin, position, rot, false);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    variable_list out(2);
+    {
+      at::AutoGradMode off(false);
+      out = packed_rotary_turn(grads[0], grads[1], s[0], s[1], s[2], ctx->saved_data["rot"].toInt(), true);
+    }
+    out = once(std::move(out), "packed_rotary");
+    out.resize(6);
+    return out;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> packed_rotary(at::Tensor q, at::Tensor k, at::Tensor cos, at::Tensor sin,
+                                                 at::Tensor position, int64_t rot) {
+  auto out = tracked({&q, &k}) ? PackedRotaryFn::apply(q, k, cos, sin, position, rot)
+                               : packed_rotary_turn(q, k, cos, sin, position, rot, false);
+  return {out[0], out[1]};
+}
+
+struct DistillFn : torch::autograd::Function<DistillFn> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor logits, at::Tensor ids, at::Tensor teacher, double temperature) {
+    auto out = distill_fwd(logits, ids, teacher, temperature);
+    ctx->save_for_backward({logits, ids, teacher, out[1]});
+    ctx->saved_data["temperature"] = temperature;
+    return out[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    variable_list out(1);
+    {
+      at::AutoGradMode off(false);
+      out[0] = distill_bwd(s[0], s[1], s[2], s[3], grads[0].contiguous(), ctx->saved_data["temperature"].toDouble());
+    }
+    out = once(std::move(out), "token_distillation");
+    out.resize(4);
+    return out;
+  }
+};
+
+at::Tensor distill(at::Tensor logits, at::Tensor ids, at::Tensor teacher, double temperature) {
+  ids = ids.contiguous();
+  teacher = teacher.contiguous();
+  if (tracked({&logits})) return DistillFn::apply(logits, ids, teacher, temperature);
+  return distill_fwd(logits, ids, teacher, temperature)[0];
+}
+
 }  // namespace
 
 void bgn_register_packed(pybind11::module& m) {
-  m.def("packed_attention_fwd", &packed_attention_fwd);
-  m.def("packed_attention_bwd", &packed_attention_bwd);
+  m.def("packed_attention", &packed_attention);
   m.def("packed_rotary", &packed_rotary);
-  m.def("distill_fwd", &distill_fwd);
-  m.def("distill_bwd", &distill_bwd);
+  m.def("distill", &distill);
 }

@@ -542,27 +542,6 @@ def token_distillation_ref(logits: Tensor, teacher_ids: Tensor, teacher_logits: 
     return term.sum(1) * temperature**2
 
 
-class _TokenDistillationFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, teacher_ids, teacher_logits, temperature):
-        from . import native
-
-        teacher_ids, teacher_logits = teacher_ids.contiguous(), teacher_logits.contiguous()
-        loss, stats = native.distill_fwd(logits, teacher_ids, teacher_logits, temperature)
-        ctx.save_for_backward(logits, teacher_ids, teacher_logits, stats)
-        ctx.temperature = temperature
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dloss):
-        from . import native
-
-        logits, ids, teacher, stats = ctx.saved_tensors
-        dloss = dloss.float().contiguous()
-        return native.distill_bwd(logits, ids, teacher, stats, dloss, ctx.temperature), None, None, None
-
-
 def token_distillation(
     logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor, temperature: float = 1.0
 ) -> Tensor:
@@ -595,10 +574,8 @@ def token_distillation(
         raise ValueError(f"token_distillation: temperature must be positive, got {temperature}")
     kernels = (torch.bfloat16, torch.float16, torch.float32)
     if (logits.dtype in kernels and teacher_logits.dtype in kernels and logits.shape[0] > 0
-            and use_fused(logits, teacher_ids, teacher_logits)):
-        if torch.is_grad_enabled() and logits.requires_grad:
-            return _TokenDistillationFn.apply(logits, teacher_ids, teacher_logits, temperature)
+            and use_fused(logits)):
         from . import native
 
-        return native.distill_fwd(logits, teacher_ids.contiguous(), teacher_logits.contiguous(), temperature)[0]
+        return native.distill(logits, teacher_ids, teacher_logits, temperature)
     return token_distillation_ref(logits, teacher_ids, teacher_logits, temperature)

@@ -4,8 +4,8 @@
 layer and in both directions.  ``packed_causal_attention`` attends inside each document,
 ``packed_rotary`` turns q and k by the positions inside each document; both stand beside
 ``causal_attention`` and ``rotary`` of the rectangular batches and pick their path the same way: the
-sm_100a kernels on CUDA, differentiable torch expressions on the CPU and inside ``ops.composable()``.
-The kernels' backward passes cannot be differentiated again.
+sm_100a kernels on CUDA (their graph nodes are in the extension), differentiable torch expressions on the
+CPU and inside ``ops.composable()``.  The kernels' backward passes cannot be differentiated again.
 """
 
 from __future__ import annotations
@@ -134,11 +134,6 @@ def _check(name: str, packing: PackedSequences, q: Tensor, *others: Tensor) -> N
         raise ValueError(f"{name}: packing on {packing.device}, operands on {q.device}")
 
 
-def _tracked(*tensors: Tensor) -> bool:
-    """Whether a graph is being built through these operands."""
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
-
-
 # --------------------------------------------------------------------------- #
 # attention
 # --------------------------------------------------------------------------- #
@@ -156,33 +151,14 @@ def packed_causal_attention_ref(q: Tensor, k: Tensor, v: Tensor, packing: Packed
     return torch.cat(parts)
 
 
-class _PackedAttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, packing, scale):
-        p = packing
-        o, bias2, *rest = native.packed_attention_fwd(q, k, v, *p.tables(), p.num_tokens, scale, True)
-        ctx.save_for_backward(q, k, v, o, bias2, *rest)
-        ctx.packing, ctx.scale = packing, scale
-        return o
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_o):
-        q, k, v, o, bias2, *rest = ctx.saved_tensors
-        p = ctx.packing
-        dq, dk, dv = native.packed_attention_bwd(d_o, q, k, v, o, bias2, rest[0] if rest else None, *p.tables(),
-                                                 p.num_tokens, ctx.scale)
-        return dq, dk, dv, None, None
-
-
 def packed_causal_attention(q: Tensor, k: Tensor, v: Tensor, packing: PackedSequences,
                             scale: float | None = None) -> Tensor:
     """Causal attention inside each document of a packed batch.
 
     q: ``[rows, Hq, D]``; k, v: ``[rows, Hkv, D]`` (Hq a multiple of Hkv); returns ``[rows, Hq, D]``.
     Row t attends the rows of its own document up to t; nothing that stands in other documents or behind
-    the last one, not even an infinity or NaN, reaches it.  Rows behind the last document give zeros and get zero gradients.
-    ``scale`` (default ``1 / sqrt(D)``) must be positive.  The kernels take bf16, fp16 and fp32 with D a
+    the last one, not even an infinity or NaN, reaches it.  Rows behind the last document give zeros and
+    get zero gradients.  ``scale`` (default ``1 / sqrt(D)``) must be positive.  The kernels take bf16, fp16 and fp32 with D a
     multiple of 8 up to 128; views of a fused projection are read in place.  Other dtypes and head sizes
     run document by document on torch operations.
     """
@@ -197,9 +173,7 @@ def packed_causal_attention(q: Tensor, k: Tensor, v: Tensor, packing: PackedSequ
     if q.dtype in _KERNEL_DTYPES and q.shape[2] % 8 == 0 and q.shape[2] <= 128 and use_fused(q):
         if q.numel() == 0:
             return q * 1.0  # no rows or no heads: nothing to launch
-        if _tracked(q, k, v):
-            return _PackedAttentionFn.apply(q, k, v, packing, scale)
-        return native.packed_attention_fwd(q, k, v, *packing.tables(), packing.num_tokens, scale, False)[0]
+        return native.packed_attention(q, k, v, *packing.tables(), packing.num_tokens, scale)
     return packed_causal_attention_ref(q, k, v, packing, scale)
 
 
@@ -208,29 +182,14 @@ def packed_causal_attention(q: Tensor, k: Tensor, v: Tensor, packing: PackedSequ
 # --------------------------------------------------------------------------- #
 
 
-class _PackedRotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, cos, sin, position, rot_dim):
-        ctx.save_for_backward(cos, sin, position)
-        ctx.rot_dim = rot_dim
-        return tuple(native.packed_rotary(q, k, cos, sin, position, rot_dim, False))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq, dk):
-        cos, sin, position = ctx.saved_tensors
-        dq, dk = native.packed_rotary(dq, dk, cos, sin, position, ctx.rot_dim, True)
-        return dq, dk, None, None, None, None
-
-
 def packed_rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, rot_dim: int,
                   packing: PackedSequences) -> tuple[Tensor, Tensor]:
     """Rotary embedding of q ``[rows, Hq, D]`` and k ``[rows, Hkv, D]`` at each document's own positions.
 
     ``cos``, ``sin``: ``[positions, rot_dim / 2]`` as ``rotary_tables`` gives them, at least as many
     positions as the longest document has tokens.  The first ``rot_dim`` features of a head turn in pairs
-    ``(i, i + rot_dim / 2)``; the rest, and rows behind the last document, are copied.  The tables get no
-    gradient.
+    ``(i, i + rot_dim / 2)``; the rest are copied.  Rows behind the last document count as position 0.  The
+    tables get no gradient.
     """
     _check("packed_rotary", packing, q, k)
     if rot_dim % 2 or not 0 < rot_dim <= q.shape[2]:
@@ -245,9 +204,7 @@ def packed_rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, rot_dim: int,
         raise ValueError("packed_rotary: the tables get no gradient")
     if q.dtype in _KERNEL_DTYPES and q.shape[2] <= 256 and use_fused(q) and q.numel() and k.numel():
         cos, sin = cos.float().contiguous(), sin.float().contiguous()
-        if _tracked(q, k):
-            return _PackedRotaryFn.apply(q, k, cos, sin, packing.position, rot_dim)
-        return tuple(native.packed_rotary(q, k, cos, sin, packing.position, rot_dim, False))
+        return native.packed_rotary(q, k, cos, sin, packing.position, rot_dim)
     at = packing.position.to(q.device, torch.int64)
     c, s = cos[at][:, None].to(q.dtype), sin[at][:, None].to(q.dtype)
     return rotary_pairs(q, c, s, rot_dim), rotary_pairs(k, c, s, rot_dim)
