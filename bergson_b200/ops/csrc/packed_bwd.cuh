@@ -363,7 +363,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const bool in = row < p.valid;
       const long at = (long(row) * p.heads + head) * p.dim;
       const int first = in ? __ldg(p.first_key + row) : 0x7fffffff;
-      const int all_from = __shfl_sync(0xffffffffu, first, 31);
+      const int all_from = __shfl_sync(0xffffffffu, first, 31), any_from = __shfl_sync(0xffffffffu, first, 0);
 
       float neg_delta = 0.f, bias2 = -INFINITY, factor = 1.f;
       if (n > 0) {
@@ -395,10 +395,14 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (lane == 0) mbar_arrive(s_read);
         const int key = entry.y + i * kTile + 64 * half;  // first key of this half
         const bool masked = key + 63 > warp_row0 || key < all_from;
+        // Chunks of 32 keys that some row of the warp attends: [g0, g1).  With short documents they are few.
+        const int g0 = masked ? max(any_from - key, 0) >> 5 : 0, g1 = masked ? ((warp_row0 + 31 - key) >> 5) + 1 : 2;
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+        for (int g = 0; g < 2; ++g) {
+          if (g < g0 || g >= g1) continue;
 #pragma unroll
           for (int e = 0; e < 32; e += 2) prob_pair(s[g][e], s[g][e + 1], c2, b2);
+        }
         const uint32_t tp = tmem_dp + 128 * (j & 1) + lane_base + 64 * half;
         ok = __all_sync(0xffffffffu, mbar_wait_bounded(&dp_full[j & 1], (j >> 1) & 1));
         if (!ok) break;
@@ -411,6 +415,10 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           pin_32(d[g]);
+          if (g < g0 || g >= g1) {
+            tmem_st_zero_16(tp + 16 * g);
+            continue;
+          }
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const float2 x = score_gradient<FMT>(s[g][e], s[g][e + 1], d[g][e], d[g][e + 1], d2, f2);
@@ -748,7 +756,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const bool in = key < p.valid;
       const int end = in ? __ldg(p.end_query + key) : 0;
       const bool opens = in && __ldg(p.first_key + key) == key;  // its own row attends nothing else
-      const int min_end = __reduce_min_sync(0xffffffffu, end);
+      const int min_end = __reduce_min_sync(0xffffffffu, end), max_end = __reduce_max_sync(0xffffffffu, end);
       // fp16: the largest |do| among the rows of all steps sets the factor of dS.
       float factor = 1.f;
       if (FMT == 0) {
@@ -771,6 +779,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         tc_fence_after();
         const bool masked = q0 < warp_key0 + 31 || q0 + 64 > min_end;
         const int from = key - q0, upto = end - 1 - q0;  // columns that attend this key
+        // Chunks of 32 queries of which some attend some key of the warp: [g0, g1).
+        const int g0 = masked ? max(warp_key0 - q0, 0) >> 5 : 0, g1 = masked ? ((max_end - 1 - q0) >> 5) + 1 : 2;
         const float4* bias = reinterpret_cast<const float4*>(row_values + gs * 2 * kTile + 64 * half);
         uint32_t s[2][32];
         tmem_ld_32(ts, s[0]);
@@ -780,6 +790,10 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         pin_32(s[1]);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
+          if (g < g0 || g >= g1) {
+            tmem_st_zero_16(ts + 16 * g);
+            continue;
+          }
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
             const float4 x = bias[g * 8 + e / 4];
@@ -808,6 +822,10 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           pin_32(d[g]);
+          if (g < g0 || g >= g1) {
+            tmem_st_zero_16(tp + 16 * g);
+            continue;
+          }
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
             const float4 y = dl[g * 8 + e / 4];

@@ -32,6 +32,8 @@
 // values in fp32, and O is rounded once.
 #pragma once
 
+#include <type_traits>
+
 #include "packed_tc.cuh"
 
 namespace bgn {
@@ -403,8 +405,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const int row = warp_row0 + lane;
       const bool in = row < p.valid;
       const int first = in ? __ldg(p.first_key + row) : 0x7fffffff;
-      // The warp's rows attend all of a key tile from `all_from` on, up to its first row.
-      const int all_from = __shfl_sync(0xffffffffu, first, 31);
+      // The warp's rows attend all of a key tile from `all_from` on, up to its first row, and nothing of it
+      // in front of `any_from`.
+      const int all_from = __shfl_sync(0xffffffffu, first, 31), any_from = __shfl_sync(0xffffffffu, first, 0);
       float m = -INFINITY, l = 0.f;  // m: the base in use, of the unscaled scores
       for (int i = 0; i < n; ++i, ++turns) {
         if (i < i0 || i >= i1) {  // only the other tile needs this key tile
@@ -425,13 +428,20 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         tmem_ld_wait();
 #pragma unroll
         for (int g = 0; g < 4; ++g) pin_32(s[g]);
+        // Chunks of 32 keys that some row of the warp attends: [g0, g1).  With short documents they are few.
+        const int g0 = masked ? max(any_from - key, 0) >> 5 : 0, g1 = masked ? ((warp_row0 + 31 - key) >> 5) + 1 : 4;
+        float top = -INFINITY;
         if (masked) {
 #pragma unroll
-          for (int g = 0; g < 4; ++g) hide(s[g], bit_range(from - 32 * g, upto - 32 * g), 0xff800000u);  // -inf
-        }
-        float top = max_chunk(s[0], -INFINITY);
+          for (int g = 0; g < 4; ++g) {
+            if (g < g0 || g >= g1) continue;
+            hide(s[g], bit_range(from - 32 * g, upto - 32 * g), 0xff800000u);  // -inf
+            top = max_chunk(s[g], top);
+          }
+        } else {
 #pragma unroll
-        for (int g = 1; g < 4; ++g) top = max_chunk(s[g], top);
+          for (int g = 0; g < 4; ++g) top = max_chunk(s[g], top);
+        }
         // A new base where the maximum grew by more than 2^8 (or is the row's first).
         const bool grow = (top - m) * c > 8.f;
         if (__any_sync(0xffffffffu, grow)) {
@@ -454,9 +464,12 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ok = my_turn(turns);
         if (!ok) break;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // Two copies of the code: tests between the chunks keep the whole tiles' exponentials from overlapping.
+        const auto exps = [&](auto part) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          exp_chunk<FMT>(ts + 16 * g, s[g], c, mc, sum);
+          if (!decltype(part)::value || (g >= g0 && g < g1)) exp_chunk<FMT>(ts + 16 * g, s[g], c, mc, sum);
+          else tmem_st_zero_16(ts + 16 * g);
           if (g == 1) {  // early: the handover takes about as long as the other half
             __syncwarp();
             if (lane == 0) mbar_arrive(&turn_over[t]);
@@ -468,6 +481,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             if (lane == 0) mbar_arrive(&p_full[2 * t + g - 2]);
           }
         }
+        };
+        if (masked) exps(std::true_type());
+        else exps(std::false_type());
         ++steps;
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }

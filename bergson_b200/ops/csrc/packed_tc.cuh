@@ -196,6 +196,11 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
   return l <= h ? (0xffffffffu << l) & (0xffffffffu >> (31 - h)) : 0u;
 }
 
+__device__ __forceinline__ void tmem_st_zero_16(uint32_t taddr) {
+  const uint32_t zeros[16] = {};
+  tmem_st_16(taddr, zeros);
+}
+
 // Puts `value` where a bit of `keep` is not set.
 __device__ __forceinline__ void hide(uint32_t (&x)[32], uint32_t keep, uint32_t value) {
 #pragma unroll
