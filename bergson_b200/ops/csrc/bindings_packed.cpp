@@ -1,8 +1,10 @@
 // Python bindings of the operators on packed documents and of the distillation loss: checks,
 // allocation of outputs, current-stream lookup.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
 
 #include "bindings.h"
@@ -232,10 +234,13 @@ at::Tensor distill_bwd(at::Tensor logits, at::Tensor ids, at::Tensor teacher, at
                   dloss.scalar_type() == at::kFloat && dloss.is_contiguous() && dloss.numel() == logits.size(0) &&
                   stats.device() == logits.device() && dloss.device() == logits.device(),
               "bergson_b200: distill_bwd: stats [T, 2] and dloss [T] in fp32 expected");
-  // The gradient has the logits' row pitch, so that both have the same alignment.
-  auto wide = at::empty({logits.size(0), logits.stride(0)}, logits.options());
-  auto dlogits = wide.narrow(1, 0, logits.size(1));
-  ran(bgn_distill_bwd(&a, stats.data_ptr<float>(), dloss.data_ptr<float>(), dlogits.data_ptr(), wide.size(1), current()),
+  // The gradient's rows are aligned like the logits', so that both take the same packets.
+  const int64_t packet = 16 / logits.element_size();
+  const int64_t pitch = logits.size(1) + (logits.stride(0) - logits.size(1)) % packet;
+  const int64_t shift = reinterpret_cast<uintptr_t>(logits.data_ptr()) % 16 / logits.element_size();
+  auto dlogits = at::empty({logits.size(0) * pitch + shift}, logits.options())
+                     .as_strided({logits.size(0), logits.size(1)}, {pitch, 1}, shift);
+  ran(bgn_distill_bwd(&a, stats.data_ptr<float>(), dloss.data_ptr<float>(), dlogits.data_ptr(), pitch, current()),
       "distill_bwd");
   return dlogits;
 }
@@ -247,11 +252,22 @@ at::Tensor distill_bwd(at::Tensor logits, at::Tensor ids, at::Tensor teacher, at
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-bool tracked(std::initializer_list<const at::Tensor*> inputs) {
+bool tracked(std::initializer_list<const at::Tensor*> inputs, const char* what) {
   if (!at::GradMode::is_enabled()) return false;
-  for (const auto* t : inputs)
-    if (t->requires_grad()) return true;
-  return false;
+  bool any = false;
+  for (const auto* t : inputs) any = any || t->requires_grad();
+  if (!any || at::cuda::currentStreamCaptureStatus() == at::cuda::CaptureStatus::None) return any;
+  // While an eager graph of a leaf lives, so does the leaf's accumulation node, bound to that graph's stream;
+  // a captured backward pass would wait for the stream, which ends the process.
+  const auto here = at::cuda::getCurrentCUDAStream().unwrap();
+  for (const auto* t : inputs) {
+    if (!t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : c10::nullopt;
+    TORCH_CHECK(!stream || *stream == here, "bergson_b200: ", what,
+                ": capturing a graph over a leaf whose eager graph on another stream is still alive; drop that graph first");
+  }
+  return true;
 }
 
 // Gradients that refuse to be differentiated: the backward kernels have none of their own.
@@ -293,7 +309,7 @@ struct PackedAttentionFn : torch::autograd::Function<PackedAttentionFn> {
 at::Tensor packed_attention(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor first_key, at::Tensor end_query,
                             at::Tensor query_tiles, at::Tensor query_pairs, at::Tensor key_tiles, int64_t valid,
                             double scale) {
-  if (tracked({&q, &k, &v}))
+  if (tracked({&q, &k, &v}, "packed_causal_attention"))
     return PackedAttentionFn::apply(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale);
   return packed_attention_fwd(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale, false)[0];
 }
@@ -320,7 +336,7 @@ struct PackedRotaryFn : torch::autograd::Function<PackedRotaryFn> {
 
 std::tuple<at::Tensor, at::Tensor> packed_rotary(at::Tensor q, at::Tensor k, at::Tensor cos, at::Tensor sin,
                                                  at::Tensor position, int64_t rot) {
-  auto out = tracked({&q, &k}) ? PackedRotaryFn::apply(q, k, cos, sin, position, rot)
+  auto out = tracked({&q, &k}, "packed_rotary") ? PackedRotaryFn::apply(q, k, cos, sin, position, rot)
                                : packed_rotary_turn(q, k, cos, sin, position, rot, false);
   return {out[0], out[1]};
 }
@@ -348,7 +364,7 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
 at::Tensor distill(at::Tensor logits, at::Tensor ids, at::Tensor teacher, double temperature) {
   ids = ids.contiguous();
   teacher = teacher.contiguous();
-  if (tracked({&logits})) return DistillFn::apply(logits, ids, teacher, temperature);
+  if (tracked({&logits}, "token_distillation")) return DistillFn::apply(logits, ids, teacher, temperature);
   return distill_fwd(logits, ids, teacher, temperature)[0];
 }
 

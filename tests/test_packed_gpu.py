@@ -419,6 +419,43 @@ def test_distillation_views(native, dtype):
         _check_distill(native, z, ids, t, 1.0)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_distillation_rows_without_a_loss(native, dtype):
+    """Rows whose entries are all unused and rows whose loss gets no gradient: zeros, whatever stands there."""
+    T, V = 700, 1003  # more rows than share out to several blocks each
+    z = _rand((T, V), dtype, 30)
+    ids = torch.randint(0, V, (T, 5), device="cuda")
+    t = _rand((T, 5), torch.float32, 31)
+    ids[::3] = -1
+    z[::3] = float("nan")
+    up = torch.ones(T, device="cuda")
+    up[1::3] = 0.0
+    leaf = z.detach().requires_grad_()
+    loss = ops.token_distillation(leaf, ids, t)
+    (g,) = torch.autograd.grad(loss, leaf, up)
+    assert (loss[::3] == 0).all() and torch.isfinite(loss).all()
+    assert (g[::3] == 0).all() and (g[1::3] == 0).all()
+    kept = slice(2, None, 3)
+    _check_distill(native, z[kept], ids[kept], t[kept], 1.0)
+    alone = z[kept].contiguous().requires_grad_()
+    one = ops.token_distillation(alone, ids[kept], t[kept])
+    want = torch.autograd.grad(one, alone, up[kept])[0]
+    torch.testing.assert_close(loss[kept], one, rtol=2e-6, atol=2e-6)  # sums of other parts
+    assert_within(g[kept], want.double(), (torch.finfo(dtype).eps + 4e-6) * want.double().abs(), floor=1e-6)
+
+
+def test_distillation_gradient_of_far_apart_rows(native):
+    """One position of each sequence: the gradient takes no more memory than its own rows."""
+    z = _rand((4, 64, 1000), torch.bfloat16, 32)
+    ids, t = torch.randint(0, 1000, (4, 6), device="cuda"), _rand((4, 6), torch.float32, 33)
+    for rows in (z[:, -1], z[:, 5, 3:900], z[:, 5, 8:901]):
+        ids_in = ids % rows.shape[1]
+        _check_distill(native, rows, ids_in, t, 1.0)
+        leaf = rows.detach().requires_grad_()
+        (g,) = torch.autograd.grad(ops.token_distillation(leaf, ids_in, t).sum(), leaf)
+        assert g.untyped_storage().nbytes() <= rows.numel() * 2 + 256
+
+
 def test_distillation_is_reproducible(native):
     z = _rand((5, 50257), torch.float32, 16).requires_grad_()
     ids, t = torch.randint(0, 9, (5, 100), device="cuda"), _rand((5, 100), torch.float32, 17)
@@ -493,3 +530,31 @@ def test_captured_and_replayed(native):
         for x, (loss, grads) in zip(steps, outs):
             l2, g2 = _step(*x)
             assert torch.equal(loss, l2.detach()) and all(torch.equal(a, b) for a, b in zip(grads, g2))
+
+
+def test_capture_over_a_leaf_of_a_living_eager_graph_is_refused(native):
+    x = _step_inputs(600)
+    q, k, v, cos, sin, p, w, ids, t = x
+    alive = ops.packed_causal_attention(q, k, v, p)
+    turned = ops.packed_rotary(q, k, cos, sin, 64, p)
+    z = _rand((257, 1000), torch.bfloat16, 601).requires_grad_()
+    loss = ops.token_distillation(z, ids, t)
+    torch.cuda.synchronize()
+    calls = (lambda: ops.packed_causal_attention(q, k, v, p), lambda: ops.packed_rotary(q, k, cos, sin, 64, p),
+             lambda: ops.token_distillation(z, ids, t))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    torch.cuda.synchronize()
+    del alive, turned, loss
+    want = _step(*x)
+    want = (want[0].detach(), want[1])
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        loss, grads = _step(*x)
+        loss = loss.detach()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(loss, want[0]) and all(torch.equal(a, b) for a, b in zip(grads, want[1]))
