@@ -19,7 +19,7 @@ cudaError_t sm_count(int* n) {
 }
 
 // cudaFuncSetAttribute holds for the current device only; it is asked for once per kernel and device.
-cudaError_t allow_smem(const void* kernel, int bytes) {
+cudaError_t allow_smem(const void* kernel, int bytes) try {
   static std::mutex mu;
   static std::set<std::pair<const void*, int>> done;
   int device = 0;
@@ -30,6 +30,8 @@ cudaError_t allow_smem(const void* kernel, int bytes) {
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e == cudaSuccess) done.insert({kernel, device});
   return e;
+} catch (...) {  // the entries are C
+  return cudaErrorMemoryAllocation;
 }
 
 template <typename T, int DP>
@@ -69,15 +71,12 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
+  static const EncodeTiledFn fn = []() -> EncodeTiledFn {
     void* ptr = nullptr;
     cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  });
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q);
+    return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeTiledFn>(ptr) : nullptr;
+  }();
   return fn;
 }
 

@@ -12,7 +12,7 @@
 // few small values, so there P carries a factor 2^10 and dS the power of two that brings the largest
 // |do| of the rows concerned to [1/2, 1): both are taken out of the fp32 sums at the end.
 //
-// Rows whose results are not finite are computed again over what they attend alone, as in the forward pass.
+// Rows whose results are not finite are put right after a block's last unit, as in the forward pass.
 #pragma once
 
 #include "packed_fwd.cuh"
@@ -131,28 +131,41 @@ constexpr int dq_smem_bytes() {
   return (2 + kDqKStages + kDqVStages) * tile_bytes<DP>() + kDqRowFloats * 4 + 256;
 }
 
-// One half of the features of a row of dQ.
+// A warp puts right one half of the features of a row of dQ, in the tile at row0.
 template <int FMT, int DP>
-__device__ __noinline__ void exact_dq_row(const PackedBwdArgs& p, int row, int head, float bias2, float neg_delta, int half,
-                                          int lane) {
+__device__ __noinline__ void exact_dq_row(const PackedBwdArgs& p, int row0, int row, int head, int half, int lane) {
   using T = typename Type16<FMT>::T;
   const int kv = head / (p.heads / p.kv_heads), first = p.first_key[row];
-  const float c = p.scale * kPackedLog2e;
+  const int f0 = half ? DP / 2 : 0, f1 = min(f0 + DP / 2, p.dim);
+  const long at = (long(row) * p.heads + head) * p.dim, k_off = long(kv) * p.k_head;
   float q[DP / 32], g[DP / 32], dq[DP / 32] = {};
+  load_row<FMT, DP>(q, p.dq, at, p.dim, lane);
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < DP / 32; ++e) bad |= lane + 32 * e >= f0 && lane + 32 * e < f1 && !(fabsf(q[e]) < INFINITY);
+  if (!__any_sync(0xffffffffu, bad)) return;
+  // see exact_forward_row; here the keys are visited from the first one of the tile's first row on
+  if (first <= row0 && !some_not_finite<FMT, DP>(p.k, p.k_tok, k_off, row + 1, min(row0 + 2 * kTile, p.valid), p.dim, lane))
+    return;
+  const float c = p.scale * kPackedLog2e, bias2 = p.bias2[long(head) * p.pitch + row] - p_shift<FMT>();
+  const float neg_delta = p.neg_delta[long(head) * p.pitch + row];
   load_row<FMT, DP>(q, p.q, long(row) * p.q_tok + long(head) * p.q_head, p.dim, lane);
   load_row<FMT, DP>(g, p.d_o, long(row) * p.do_tok + long(head) * p.do_head, p.dim, lane);
-  for (int j = first; j <= row && first < row; ++j) {
-    float k[DP / 32], v[DP / 32];
-    load_row<FMT, DP>(k, p.k, long(j) * p.k_tok + long(kv) * p.k_head, p.dim, lane);
-    load_row<FMT, DP>(v, p.v, long(j) * p.v_tok + long(kv) * p.v_head, p.dim, lane);
-    const float ds = exp2f(warp_dot(q, k) * c + (bias2 - p_shift<FMT>())) * (warp_dot(g, v) + neg_delta);
+  for (int j0 = first; j0 <= row && first < row && !all_nan(dq, f0, f1, lane); j0 += 64) {
+#pragma unroll 4
+    for (int j = j0; j <= min(j0 + 63, row); ++j) {
+      float k[DP / 32], v[DP / 32];
+      load_row<FMT, DP>(k, p.k, long(j) * p.k_tok + k_off, p.dim, lane);
+      load_row<FMT, DP>(v, p.v, long(j) * p.v_tok + long(kv) * p.v_head, p.dim, lane);
+      const float ds = exp2f(warp_dot(q, k) * c + bias2) * (warp_dot(g, v) + neg_delta);
 #pragma unroll
-    for (int e = 0; e < DP / 32; ++e) dq[e] = fmaf(ds, k[e], dq[e]);
+      for (int e = 0; e < DP / 32; ++e) dq[e] = fmaf(ds, k[e], dq[e]);
+    }
   }
-  T* dst = static_cast<T*>(p.dq) + (long(row) * p.heads + head) * p.dim;
+  T* dst = static_cast<T*>(p.dq) + at;
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e)
-    if (lane + 32 * e < p.dim && (lane + 32 * e >= DP / 2) == (half != 0)) dst[lane + 32 * e] = from_float<T>(dq[e] * p.scale);
+    if (lane + 32 * e >= f0 && lane + 32 * e < f1) dst[lane + 32 * e] = from_float<T>(dq[e] * p.scale);
 }
 
 template <int FMT, int DP>
@@ -353,7 +366,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const uint32_t lane_base = uint32_t(quad * 32) << 16;
     const uint32_t ts = tmem_s + lane_base + 64 * half;
     const float c = p.scale * kPackedLog2e;
-    bool ok = true;
+    bool ok = true, bad = false;
     int j = 0, count = 0;
     for (int r = 0; unit >= 0 && ok; ++r) {
       const int after = nth_unit(r + 1, p.units);
@@ -447,18 +460,21 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (!ok) break;
         tc_fence_after();
         // each of the two threads of a row stores one half of the features
-        const bool bad = store_row<FMT, DP>(tmem_dq + lane_base, p.scale / factor, dst, p.dim, some, half);
-        for (uint32_t again = __ballot_sync(0xffffffffu, bad); again != 0; again &= again - 1) {
-          const int rr = __ffs(again) - 1;
-          exact_dq_row<FMT, DP>(p, warp_row0 + rr, head, __shfl_sync(0xffffffffu, bias2, rr),
-                                __shfl_sync(0xffffffffu, neg_delta, rr), half, lane);
-        }
+        bad |= store_row<FMT, DP>(tmem_dq + lane_base, p.scale / factor, dst, p.dim, some, half);
         tc_fence_before();
       }
       if (!some && row < p.rows && half == 0)
         for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
     }
     if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutEpilogue);
+    if (ok && __any_sync(0xffffffffu, bad)) {
+      __syncwarp();  // the lanes' rows are read by all
+      for (int r = 0; (unit = nth_unit(r, p.units)) >= 0; ++r) {
+        const int row0 = p.tiles[unit / p.heads].x, begin = row0 + quad * 32;
+        for (int row = begin; row < min(begin + 32, p.valid); ++row)
+          exact_dq_row<FMT, DP>(p, row0, row, unit % p.heads, half, lane);
+      }
+    }
   }
 
   tc_fence_before();
@@ -490,36 +506,51 @@ constexpr int dkv_smem_bytes() {
   return (2 + kDkvQStages + kDkvGStages) * tile_bytes<DP>() + kDkvGStages * kDkvRowBytes + 512;
 }
 
-// A row of dV (half 0) or of dK.
+// A warp puts right a row of dV (half 0) or of dK, of the tile of keys whose queries are [row0, last).
 template <int FMT, int DP>
-__device__ __noinline__ void exact_dkv_row(const PackedBwdArgs& p, int key, int kv, int half, int lane) {
+__device__ __noinline__ void exact_dkv_row(const PackedBwdArgs& p, int row0, int last, int key, int kv, int half, int lane) {
   using T = typename Type16<FMT>::T;
   const int group = p.heads / p.kv_heads, end = p.end_query[key], first = p.first_key[key];
+  T* dst = static_cast<T*>(half ? p.dk : p.dv) + (long(key) * p.kv_heads + kv) * p.dim;
+  float k[DP / 32], v[DP / 32], sum[DP / 32] = {};
+  load_row<FMT, DP>(k, dst, 0, p.dim, lane);
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < DP / 32; ++e) bad |= !(fabsf(k[e]) < INFINITY);
+  if (!__any_sync(0xffffffffu, bad)) return;
+  // A document that ends in the tile is short there; the others are left with few rows that do not attend them.
+  if (end > row0 + kTile) {
+    bad = false;
+    for (int head = kv * group; head < (kv + 1) * group && !bad; ++head) {
+      const void* x = half ? p.q : p.d_o;
+      const long tok = half ? p.q_tok : p.do_tok, off = long(head) * (half ? p.q_head : p.do_head);
+      bad = some_not_finite<FMT, DP>(x, tok, off, row0, key, p.dim, lane) ||
+            some_not_finite<FMT, DP>(x, tok, off, end, min(last, p.valid), p.dim, lane);
+    }
+    if (!bad) return;
+  }
   const float c = p.scale * kPackedLog2e;
-  float k[DP / 32], v[DP / 32], dk[DP / 32] = {}, dv[DP / 32] = {};
   load_row<FMT, DP>(k, p.k, long(key) * p.k_tok + long(kv) * p.k_head, p.dim, lane);
   load_row<FMT, DP>(v, p.v, long(key) * p.v_tok + long(kv) * p.v_head, p.dim, lane);
+  const int begin = half && key == first ? key + 1 : key;  // a document's first row has a single key, and no dS
   for (int head = kv * group; head < (kv + 1) * group; ++head) {
-    for (int row = key; row < end; ++row) {
-      float q[DP / 32], g[DP / 32];
-      load_row<FMT, DP>(q, p.q, long(row) * p.q_tok + long(head) * p.q_head, p.dim, lane);
-      load_row<FMT, DP>(g, p.d_o, long(row) * p.do_tok + long(head) * p.do_head, p.dim, lane);
-      const float w = exp2f(warp_dot(q, k) * c + (p.bias2[long(head) * p.pitch + row] - p_shift<FMT>()));
-      const float ds = row == first ? 0.f : w * (warp_dot(g, v) + p.neg_delta[long(head) * p.pitch + row]);
+    const long at = long(head) * p.pitch;
+    for (int i0 = begin; i0 < end && !all_nan(sum, 0, p.dim, lane); i0 += 64) {
+#pragma unroll 4
+      for (int row = i0; row < min(i0 + 64, end); ++row) {
+        float q[DP / 32], g[DP / 32];
+        load_row<FMT, DP>(q, p.q, long(row) * p.q_tok + long(head) * p.q_head, p.dim, lane);
+        load_row<FMT, DP>(g, p.d_o, long(row) * p.do_tok + long(head) * p.do_head, p.dim, lane);
+        float w = exp2f(warp_dot(q, k) * c + (p.bias2[at + row] - p_shift<FMT>()));
+        if (half) w *= warp_dot(g, v) + p.neg_delta[at + row];
 #pragma unroll
-      for (int e = 0; e < DP / 32; ++e) {
-        dv[e] = fmaf(w, g[e], dv[e]);
-        if (row != first) dk[e] = fmaf(ds, q[e], dk[e]);
+        for (int e = 0; e < DP / 32; ++e) sum[e] = fmaf(w, half ? q[e] : g[e], sum[e]);
       }
     }
   }
-  const long at = (long(key) * p.kv_heads + kv) * p.dim;
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e)
-    if (lane + 32 * e < p.dim) {
-      if (half) static_cast<T*>(p.dk)[at + lane + 32 * e] = from_float<T>(dk[e] * p.scale);
-      else static_cast<T*>(p.dv)[at + lane + 32 * e] = from_float<T>(dv[e]);
-    }
+    if (lane + 32 * e < p.dim) dst[lane + 32 * e] = from_float<T>(half ? sum[e] * p.scale : sum[e]);
 }
 
 template <int FMT, int DP>
@@ -746,7 +777,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const uint32_t ts = tmem_s + lane_base + 64 * half, tp = tmem_dp + lane_base + 64 * half;
     const float c = p.scale * kPackedLog2e;
     const float2 c2 = make_float2(c, c);
-    bool ok = true;
+    bool ok = true, bad = false;
     int j = 0, count = 0;
     for (int r = 0; unit >= 0 && ok; ++r) {
       const int after = nth_unit(r + 1, p.units);
@@ -861,15 +892,22 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (!ok) break;
         tc_fence_after();
         const float out = half ? p.scale / factor : (FMT == 0 ? 1.f / 1024.f : 1.f);
-        const bool bad = store_row<FMT, DP>((half ? tmem_dk : tmem_dv) + lane_base, out, dst, p.dim, in);
-        for (uint32_t again = __ballot_sync(0xffffffffu, bad); again != 0; again &= again - 1)
-          exact_dkv_row<FMT, DP>(p, warp_key0 + __ffs(again) - 1, kv_head, half, lane);
+        bad |= store_row<FMT, DP>((half ? tmem_dk : tmem_dv) + lane_base, out, dst, p.dim, in);
         tc_fence_before();
       }
       if (!in && key < p.rows)
         for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
     }
     if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutEpilogue);
+    if (ok && __any_sync(0xffffffffu, bad)) {
+      __syncwarp();  // the lanes' rows are read by all
+      for (int r = 0; (unit = nth_unit(r, p.units)) >= 0; ++r) {
+        const int4 e = p.tiles[unit / p.kv_heads];
+        const int begin = e.x + quad * 32;
+        for (int key = begin; key < min(begin + 32, p.valid); ++key)
+          exact_dkv_row<FMT, DP>(p, e.x, e.x + tiles_of(e) * kTile, key, unit % p.kv_heads, half, lane);
+      }
+    }
   }
 
   tc_fence_before();

@@ -16,8 +16,10 @@
 //
 // An infinity or NaN in a value row that some rows of a tile do not attend reaches them all the same, as
 // 0 * NaN of the second product.  It shows as a NaN of the result: a row whose result is not finite is
-// computed again, over its own keys alone.  (Looking through the tiles in shared memory instead held up
-// the pipeline: other reads wait long while the tensor core takes its operands from there.)
+// computed again over its own keys alone, unless the few value rows that it was multiplied with and does not
+// attend are all finite.  That comes after a block's last unit, when no other warp waits for this one with
+// a limit.  (Looking through the tiles in shared memory instead held up the pipeline: other reads wait
+// long while the tensor core takes its operands from there.)
 //
 // What bounds it: a tile of 128 x 128 scores takes 1024 cycles of the tensor core at 128 features and
 // 1024 of the exponential unit (twice that of the tensor core at 64), in a chain that the two tiles
@@ -105,20 +107,35 @@ __device__ __forceinline__ QueryUnit query_unit(const int4 (&e)[2], int head_pai
   return w;
 }
 
+// A warp puts right a row of the tile at row0.
 template <int FMT, int DP>
-__device__ __noinline__ void exact_forward_row(const PackedFwdArgs& p, int row, int head, float bias2, int lane) {
+__device__ __noinline__ void exact_forward_row(const PackedFwdArgs& p, int row0, int row, int head, int lane) {
   using T = typename Type16<FMT>::T;
-  const int kv = head / (p.heads / p.kv_heads);
-  const float c = p.scale * kPackedLog2e;
+  const int kv = head / (p.heads / p.kv_heads), first = p.first_key[row];
   float q[DP / 32], o[DP / 32] = {};
-  load_row<FMT, DP>(q, p.q, long(row) * p.q_tok + long(head) * p.q_head, p.dim, lane);
-  for (int j = p.first_key[row]; j <= row; ++j) {
-    float k[DP / 32], v[DP / 32];
-    load_row<FMT, DP>(k, p.k, long(j) * p.k_tok + long(kv) * p.k_head, p.dim, lane);
-    load_row<FMT, DP>(v, p.v, long(j) * p.v_tok + long(kv) * p.v_head, p.dim, lane);
-    const float w = exp2f(warp_dot(q, k) * c + (bias2 - p_shift<FMT>()));
+  const long v_off = long(kv) * p.v_head;
+  load_row<FMT, DP>(q, p.o, (long(row) * p.heads + head) * p.dim, p.dim, lane);
+  bool bad = false;
 #pragma unroll
-    for (int e = 0; e < DP / 32; ++e) o[e] = fmaf(w, v[e], o[e]);
+  for (int e = 0; e < DP / 32; ++e) bad |= !(fabsf(q[e]) < INFINITY);
+  if (!__any_sync(0xffffffffu, bad)) return;
+  // A document that begins in the tile is short there.  Another one begins less than a tile behind the first
+  // key that was visited, and the last one visited is less than two tiles behind row0.
+  if (first <= row0 && !some_not_finite<FMT, DP>(p.v, p.v_tok, v_off, max(first - kTile + 1, 0), first, p.dim, lane) &&
+      !some_not_finite<FMT, DP>(p.v, p.v_tok, v_off, row + 1, min(row0 + 2 * kTile, p.valid), p.dim, lane))
+    return;
+  const float c = p.scale * kPackedLog2e, bias2 = p.bias2[long(head) * p.pitch + row] - p_shift<FMT>();
+  load_row<FMT, DP>(q, p.q, long(row) * p.q_tok + long(head) * p.q_head, p.dim, lane);
+  for (int j0 = first; j0 <= row && !all_nan(o, 0, p.dim, lane); j0 += 64) {
+#pragma unroll 4
+    for (int j = j0; j <= min(j0 + 63, row); ++j) {
+      float k[DP / 32], v[DP / 32];
+      load_row<FMT, DP>(k, p.k, long(j) * p.k_tok + long(kv) * p.k_head, p.dim, lane);
+      load_row<FMT, DP>(v, p.v, long(j) * p.v_tok + v_off, p.dim, lane);
+      const float w = exp2f(warp_dot(q, k) * c + bias2);
+#pragma unroll
+      for (int e = 0; e < DP / 32; ++e) o[e] = fmaf(w, v[e], o[e]);
+    }
   }
   const long at = (long(row) * p.heads + head) * p.dim + lane;
 #pragma unroll
@@ -382,7 +399,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const uint32_t lane_base = uint32_t(quad * 32) << 16;
     const uint32_t ts = tmem_s + 128 * t + lane_base, to = tmem_o + 128 * t + lane_base;
     const float c = p.scale * kPackedLog2e;
-    bool ok = true;
+    bool ok = true, bad = false;
     int steps = 0, uses = 0, turns = 0;
     // The two tiles take turns at the exponentials, tile 0 first: left alone they fall into step, and then
     // nobody computes under the products.  A tile takes its turn at every key tile of the unit, needed
@@ -502,17 +519,23 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ++uses;
         if (!ok) break;
         tc_fence_after();
-        const bool bad = store_row<FMT, DP>(to, some ? 1.f / l : 0.f, dst, p.dim, some, -1, rest);
-        for (uint32_t again = __ballot_sync(0xffffffffu, bad); again != 0; again &= again - 1) {
-          const int rr = __ffs(again) - 1;
-          exact_forward_row<FMT, DP>(p, warp_row0 + rr, head, __shfl_sync(0xffffffffu, bias2, rr), lane);
-        }
+        bad |= store_row<FMT, DP>(to, some ? 1.f / l : 0.f, dst, p.dim, some, -1, rest);
         tc_fence_before();
       }
       if (!some && row < p.rows)
         for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
     }
     if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutEpilogue);
+    if (ok && __any_sync(0xffffffffu, bad)) {
+      __syncwarp();  // the lanes' rows are read by all
+      for (int r = 0; (unit = nth_unit(r, p.units)) >= 0; ++r) {
+        fetch_unit(p.tiles, p.head_pairs, p.heads, unit, entry);
+        const QueryUnit u = query_unit(entry, p.head_pairs, p.heads, p.kv_heads, unit);
+        const int row0 = t ? u.row0[1] : u.row0[0], begin = row0 + quad * 32;
+        for (int row = begin; row < min(begin + 32, p.valid); ++row)
+          exact_forward_row<FMT, DP>(p, row0, row, t ? u.head[1] : u.head[0], lane);
+      }
+    }
   }
 
   tc_fence_before();

@@ -141,6 +141,29 @@ __device__ __forceinline__ void load_row(float (&x)[DP / 32], const void* base, 
   for (int e = 0; e < DP / 32; ++e) x[e] = lane + 32 * e < dim ? to_float<T>(p[lane + 32 * e]) : 0.f;
 }
 
+// Whether a value of the rows [from, to) is infinite or NaN.
+template <int FMT, int DP>
+__device__ __forceinline__ bool some_not_finite(const void* base, long tok, long offset, int from, int to, int dim, int lane) {
+  bool bad = false;
+#pragma unroll 4
+  for (int j = from; j < to; ++j) {
+    float x[DP / 32];
+    load_row<FMT, DP>(x, base, long(j) * tok + offset, dim, lane);
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) bad |= !(fabsf(x[e]) < INFINITY);
+  }
+  return __any_sync(0xffffffffu, bad);
+}
+
+// Whether every value that counts is NaN, which no further sum changes.
+template <int N>
+__device__ __forceinline__ bool all_nan(const float (&x)[N], int from, int to, int lane) {
+  bool yes = true;
+#pragma unroll
+  for (int e = 0; e < N; ++e) yes &= lane + 32 * e < from || lane + 32 * e >= to || isnan(x[e]);
+  return __all_sync(0xffffffffu, yes);
+}
+
 template <int N>
 __device__ __forceinline__ float warp_dot(const float (&x)[N], const float (&y)[N]) {
   float s = 0.f;

@@ -158,6 +158,63 @@ def test_attention_keeps_documents_apart(native, d, poison, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hk", [(4, 2), (3, 3)])
+def test_attention_a_nan_reaches_what_depends_on_it(native, hq, hk, d, dtype):
+    """One NaN in v, then one in the output's gradient, in the middle of a long document."""
+    lens = [700, 40, 1500]
+    begin, at, rows = 740, 740 + 900, sum(lens)
+    q, k, v, do = (_rand((rows, h, d), dtype, 170 + i) for i, h in enumerate((hq, hk, hk, hq)))
+    want, tol = attention64(q, k, v, lens, do=do)
+    group, kv = hq // hk, hk - 1
+
+    def check(got, name, hit):
+        assert torch.equal(torch.isnan(got[name]), hit), name
+        assert_within(got[name][~hit], want[name][~hit], tol[name][~hit], name, floor=6e-8)
+
+    bad = v.clone()
+    bad[at, kv, 5] = float("nan")
+    hit = torch.zeros((rows, hq, d), dtype=torch.bool, device="cuda")
+    hit[at:, kv * group:, 5] = True
+    check(_attend(native, q, k, bad, lens), "o", hit)
+
+    bad = do.clone()
+    bad[at, hq - 1, 5] = float("nan")
+    got = _attend(native, q, k, v, lens, do=bad)
+    hit_v, hit_k = (torch.zeros((rows, hk, d), dtype=torch.bool, device="cuda") for _ in range(2))
+    hit_v[begin:at + 1, kv, 5] = True
+    hit_k[begin:at + 1, kv] = True
+    hit_q = torch.zeros_like(hit)
+    hit_q[at, hq - 1] = True
+    for name, h in (("dv", hit_v), ("dk", hit_k), ("dq", hit_q)):
+        check(got, name, h)
+
+
+def test_attention_nan_in_a_very_long_document(native):
+    """Putting rows right takes time where they are long; nobody waits for it with a limit."""
+    from bergson_b200.ops import attribution
+
+    n = 30000
+    q, k, v, do = (_rand((n, h, 64), torch.bfloat16, 180 + i) for i, h in enumerate((4, 1, 1, 4)))
+    do[-1] = float("nan")
+    got = _attend(native, q, k, v, [n], do=do)
+    assert torch.isnan(got["dv"]).all() and torch.isnan(got["dk"]).all()
+    assert torch.isfinite(got["dq"][:-1]).all() and torch.isnan(got["dq"][-1]).all()
+    do[-1] = do[0]
+    do[100] = float("nan")
+    got = _attend(native, q, k, v, [n], do=do)
+    assert torch.isnan(got["dv"][:101]).all() and torch.isfinite(got["dv"][101:]).all()
+    assert torch.isnan(got["dk"][:101]).all() and torch.isfinite(got["dk"][101:]).all()
+    v[-1] = float("nan")
+    got = _attend(native, q, k, v, [n])
+    assert torch.isfinite(got["o"][:-1]).all() and torch.isnan(got["o"][-1]).all()
+    q[0] = float("nan")
+    got = _attend(native, q, k, v, [n], do=do)
+    assert torch.isnan(got["o"][0]).all() and torch.isfinite(got["o"][1:-1]).all()
+    assert attribution.kernel_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_later_rows_do_not_reach_earlier_ones(native, dtype):
     n, at = 400, 207
     q, k, v = (_rand((n, 2, 64), dtype, 90 + i) for i in range(3))
