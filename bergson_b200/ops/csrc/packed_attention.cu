@@ -34,35 +34,35 @@ cudaError_t allow_smem(const void* kernel, int bytes) try {
   return cudaErrorMemoryAllocation;
 }
 
-template <typename T, int DP>
+template <int DP>
 cudaError_t simple_fwd(const BgnPackedAttention& a, void* o, float* bias2, cudaStream_t stream) {
   constexpr int smem = simple_smem<DP>(3);
-  auto kern = packed_fwd_simple_kernel<T, DP>;
+  auto kern = packed_fwd_simple_kernel<DP>;
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
   const unsigned grid = unsigned((a.rows + 127) / 128) * 2u * unsigned(a.heads);
-  kern<<<grid, kSimpleThreads, smem, stream>>>(a, static_cast<T*>(o), bias2);
+  kern<<<grid, kSimpleThreads, smem, stream>>>(a, static_cast<float*>(o), bias2);
   return cudaGetLastError();
 }
 
-template <typename T, int DP>
+template <int DP>
 cudaError_t simple_bwd(const BgnPackedAttention& a, const void* o, const float* bias2, const void* d_o, long do_tok,
                        long do_head, float* delta, void* dq, void* dk, void* dv, cudaStream_t stream) {
   constexpr int smem = simple_smem<DP>(4);
-  auto kq = packed_dq_simple_kernel<T, DP>;
-  auto kk = packed_dkv_simple_kernel<T, DP>;
+  auto kq = packed_dq_simple_kernel<DP>;
+  auto kk = packed_dkv_simple_kernel<DP>;
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kq), smem);
   if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(kk), smem);
   if (e != cudaSuccess) return e;
   const unsigned tiles = unsigned((a.rows + 127) / 128) * 2u;
-  kq<<<tiles * unsigned(a.heads), kSimpleThreads, smem, stream>>>(a, static_cast<const T*>(o), bias2,
-                                                                  static_cast<const T*>(d_o), do_tok, do_head, delta,
-                                                                  static_cast<T*>(dq));
+  kq<<<tiles * unsigned(a.heads), kSimpleThreads, smem, stream>>>(a, static_cast<const float*>(o), bias2,
+                                                                  static_cast<const float*>(d_o), do_tok, do_head, delta,
+                                                                  static_cast<float*>(dq));
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  kk<<<tiles * unsigned(a.kv_heads), kSimpleThreads, smem, stream>>>(a, bias2, static_cast<const T*>(d_o), do_tok,
-                                                                     do_head, delta, static_cast<T*>(dk),
-                                                                     static_cast<T*>(dv));
+  kk<<<tiles * unsigned(a.kv_heads), kSimpleThreads, smem, stream>>>(a, bias2, static_cast<const float*>(d_o), do_tok,
+                                                                     do_head, delta, static_cast<float*>(dk),
+                                                                     static_cast<float*>(dv));
   return cudaGetLastError();
 }
 
@@ -218,7 +218,7 @@ extern "C" int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, vo
   if (!sound(a)) return int(cudaErrorInvalidValue);
   const bool narrow = a->dim <= 64;
   if (a->type == 2) {
-    auto run = a->dim <= 32 ? simple_fwd<float, 32> : (narrow ? simple_fwd<float, 64> : simple_fwd<float, 128>);
+    auto run = a->dim <= 32 ? simple_fwd<32> : (narrow ? simple_fwd<64> : simple_fwd<128>);
     return int(run(*a, o, bias2, stream));
   }
   if (a->type == 1)
@@ -233,7 +233,7 @@ extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void*
   if (!sound(a)) return int(cudaErrorInvalidValue);
   const bool narrow = a->dim <= 64;
   if (a->type == 2) {
-    auto run = a->dim <= 32 ? simple_bwd<float, 32> : (narrow ? simple_bwd<float, 64> : simple_bwd<float, 128>);
+    auto run = a->dim <= 32 ? simple_bwd<32> : (narrow ? simple_bwd<64> : simple_bwd<128>);
     return int(run(*a, o, bias2, d_o, do_tok, do_head, delta, dq, dk, dv, stream));
   }
   auto run = a->type == 1 ? (narrow ? tensor_bwd<1, 64> : tensor_bwd<1, 128>)

@@ -1,4 +1,4 @@
-// Causal attention over packed documents on the FMA units: forward and backward for every type.
+// Causal attention over packed documents in fp32 on the FMA units: forward and backward.
 //
 // Token t attends the keys first_key[t] .. t.  Tiles are cut from the packed token axis without
 // regard to documents: a tile of 64 queries visits the keys from its first row's first key to its
@@ -11,6 +11,11 @@
 // The scaled score is rounded on its own in both directions, so that a row with one key has P = 1 exactly.
 // dQ and dK/dV are two kernels that recompute P from the stored log-sum-exp: sums stay in one block
 // and one order, so results do not depend on scheduling.
+//
+// Bound by the FMA units and the shared memory that feeds them (a thread's 4 x 4 scores take two 16-byte loads
+// to 16 operations): 8 documents of 1024 tokens, 12 heads of 64, forward 500 us (26 TFLOP/s), backward
+// 1510 us.  Small batches wait for one block's chain of tiles.  Fetching a tile into registers while the one
+// before it is at work took 540 and 1715 us: the registers leave room for one block on an SM instead of two.
 #pragma once
 
 #include "common.cuh"
@@ -25,18 +30,19 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // Tile of `kSimpleTile` tokens in shared memory as [feature][token]; rows at or past `limit` and
 // features at or past `dim` are zero.
-template <typename T, int DP>
-__device__ __forceinline__ void simple_load(float* dst, const T* src, long tok_stride, int t0, int limit, int dim) {
-  constexpr int V = 16 / int(sizeof(T));
+template <int DP>
+__device__ __forceinline__ void simple_load(float* dst, const float* src, long tok_stride, int t0, int limit, int dim) {
   // One packet per step; neighbouring threads take neighbouring tokens, so the transposed stores
   // fall into different banks.
-  for (int i = threadIdx.x; i < kSimpleTile * (DP / V); i += kSimpleThreads) {
-    const int tok = i % kSimpleTile, d = (i / kSimpleTile) * V;
-    union { uint4 u; T h[V]; } p;
-    p.u = make_uint4(0, 0, 0, 0);
-    if (t0 + tok < limit && d < dim) p.u = *reinterpret_cast<const uint4*>(src + long(t0 + tok) * tok_stride + d);
-#pragma unroll
-    for (int e = 0; e < V; ++e) dst[(d + e) * kSimplePitch + tok] = to_float<T>(p.h[e]);
+  for (int i = threadIdx.x; i < kSimpleTile * (DP / 4); i += kSimpleThreads) {
+    const int tok = i % kSimpleTile, d = (i / kSimpleTile) * 4;
+    float4 p = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (t0 + tok < limit && d < dim) p = *reinterpret_cast<const float4*>(src + long(t0 + tok) * tok_stride + d);
+    float* to = dst + d * kSimplePitch + tok;
+    to[0] = p.x;
+    to[kSimplePitch] = p.y;
+    to[2 * kSimplePitch] = p.z;
+    to[3 * kSimplePitch] = p.w;
   }
 }
 
@@ -102,8 +108,8 @@ __device__ __forceinline__ float half_warp_max(float v) {
   return v;
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPackedAttention a, T* o, float* bias2) {
+template <int DP>
+__global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPackedAttention a, float* o, float* bias2) {
   extern __shared__ float smem[];
   float* qs = smem;
   float* ks = qs + DP * kSimplePitch;
@@ -116,7 +122,7 @@ __global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPa
   if (q0 >= a.rows) return;
   const float c = a.scale * kLog2e;
 
-  simple_load<T, DP>(qs, static_cast<const T*>(a.q) + long(head) * a.q_head, a.q_tok, q0, a.valid, a.dim);
+  simple_load<DP>(qs, static_cast<const float*>(a.q) + long(head) * a.q_head, a.q_tok, q0, a.valid, a.dim);
   int first[4];
   float m[4], l[4], out[4][DP / 16];
 #pragma unroll
@@ -133,8 +139,8 @@ __global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPa
   for (int k0 = q1 > q0 ? a.first_key[q0] : q1; k0 < q1; k0 += kSimpleTile) {
     const bool masked = k0 + kSimpleTile - 1 > q0 || k0 < last_first;
     __syncthreads();
-    simple_load<T, DP>(ks, static_cast<const T*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
-    simple_load<T, DP>(vs, static_cast<const T*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
+    simple_load<DP>(ks, static_cast<const float*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
+    simple_load<DP>(vs, static_cast<const float*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
     __syncthreads();
     float s[4][4] = {};
     simple_scores<DP>(s, qs, ks, ty, tx);
@@ -173,17 +179,17 @@ __global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPa
     const bool some = row < a.valid && first[i] <= row;
     const float inv = some ? 1.f / l[i] : 0.f;
     if (tx == 0) bias2[long(head) * a.pitch + row] = some ? -(m[i] + log2f(l[i])) : -INFINITY;
-    T* dst = o + (long(row) * a.heads + head) * a.dim;
+    float* dst = o + (long(row) * a.heads + head) * a.dim;
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
-      if (tx + 16 * d < a.dim) dst[tx + 16 * d] = from_float<T>(some ? out[i][d] * inv : 0.f);
+      if (tx + 16 * d < a.dim) dst[tx + 16 * d] = some ? out[i][d] * inv : 0.f;
   }
 }
 
-template <typename T, int DP>
+template <int DP>
 __global__ void __launch_bounds__(kSimpleThreads)
-packed_dq_simple_kernel(BgnPackedAttention a, const T* o, const float* bias2, const T* d_o, long do_tok, long do_head,
-                        float* delta, T* dq) {
+packed_dq_simple_kernel(BgnPackedAttention a, const float* o, const float* bias2, const float* d_o, long do_tok, long do_head,
+                        float* delta, float* dq) {
   extern __shared__ float smem[];
   float* qs = smem;
   float* gs = qs + DP * kSimplePitch;
@@ -197,8 +203,8 @@ packed_dq_simple_kernel(BgnPackedAttention a, const T* o, const float* bias2, co
   if (q0 >= a.rows) return;
   const float c = a.scale * kLog2e;
 
-  simple_load<T, DP>(qs, static_cast<const T*>(a.q) + long(head) * a.q_head, a.q_tok, q0, a.valid, a.dim);
-  simple_load<T, DP>(gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
+  simple_load<DP>(qs, static_cast<const float*>(a.q) + long(head) * a.q_head, a.q_tok, q0, a.valid, a.dim);
+  simple_load<DP>(gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
   __syncthreads();
   int first[4];
   float bias[4], dl[4], out[4][DP / 16];
@@ -210,8 +216,8 @@ packed_dq_simple_kernel(BgnPackedAttention a, const T* o, const float* bias2, co
     bias[i] = in ? bias2[long(head) * a.pitch + row] : -INFINITY;
     float sum = 0.f;
     if (in) {
-      const T* orow = o + (long(row) * a.heads + head) * a.dim;
-      for (int d = tx; d < a.dim; d += 16) sum = fmaf(to_float<T>(orow[d]), gs[d * kSimplePitch + 4 * ty + i], sum);
+      const float* orow = o + (long(row) * a.heads + head) * a.dim;
+      for (int d = tx; d < a.dim; d += 16) sum = fmaf(orow[d], gs[d * kSimplePitch + 4 * ty + i], sum);
     }
     dl[i] = half_warp_sum(sum);
     if (tx == 0 && row < a.rows) delta[long(head) * a.pitch + row] = dl[i];
@@ -223,8 +229,8 @@ packed_dq_simple_kernel(BgnPackedAttention a, const T* o, const float* bias2, co
   for (int k0 = q1 > q0 ? a.first_key[q0] : q1; k0 < q1; k0 += kSimpleTile) {
     const bool masked = k0 + kSimpleTile - 1 > q0 || k0 < last_first;
     __syncthreads();
-    simple_load<T, DP>(ks, static_cast<const T*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
-    simple_load<T, DP>(vs, static_cast<const T*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
+    simple_load<DP>(ks, static_cast<const float*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
+    simple_load<DP>(vs, static_cast<const float*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
     __syncthreads();
     float s[4][4] = {}, dp[4][4] = {};
     simple_scores<DP>(s, qs, ks, ty, tx);
@@ -247,17 +253,17 @@ packed_dq_simple_kernel(BgnPackedAttention a, const T* o, const float* bias2, co
   for (int i = 0; i < 4; ++i) {
     const int row = q0 + 4 * ty + i;
     if (row >= a.rows) continue;
-    T* dst = dq + (long(row) * a.heads + head) * a.dim;
+    float* dst = dq + (long(row) * a.heads + head) * a.dim;
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
-      if (tx + 16 * d < a.dim) dst[tx + 16 * d] = from_float<T>(out[i][d] * a.scale);
+      if (tx + 16 * d < a.dim) dst[tx + 16 * d] = out[i][d] * a.scale;
   }
 }
 
-template <typename T, int DP>
+template <int DP>
 __global__ void __launch_bounds__(kSimpleThreads)
-packed_dkv_simple_kernel(BgnPackedAttention a, const float* bias2, const T* d_o, long do_tok, long do_head,
-                         const float* delta, T* dk, T* dv) {
+packed_dkv_simple_kernel(BgnPackedAttention a, const float* bias2, const float* d_o, long do_tok, long do_head,
+                         const float* delta, float* dk, float* dv) {
   extern __shared__ float smem[];
   float* ks = smem;
   float* vs = ks + DP * kSimplePitch;
@@ -271,8 +277,8 @@ packed_dkv_simple_kernel(BgnPackedAttention a, const float* bias2, const T* d_o,
   if (k0 >= a.rows) return;
   const float c = a.scale * kLog2e;
 
-  simple_load<T, DP>(ks, static_cast<const T*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
-  simple_load<T, DP>(vs, static_cast<const T*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
+  simple_load<DP>(ks, static_cast<const float*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
+  simple_load<DP>(vs, static_cast<const float*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
   int end[4], own_first[4];
   float out_k[4][DP / 16], out_v[4][DP / 16];
 #pragma unroll
@@ -290,8 +296,8 @@ packed_dkv_simple_kernel(BgnPackedAttention a, const float* bias2, const T* d_o,
     for (int q0 = k0; q0 < q_end; q0 += kSimpleTile) {
       const bool masked = q0 < k0 + kSimpleTile || q0 + kSimpleTile > first_end;
       __syncthreads();
-      simple_load<T, DP>(qs, static_cast<const T*>(a.q) + long(head) * a.q_head, a.q_tok, q0, a.valid, a.dim);
-      simple_load<T, DP>(gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
+      simple_load<DP>(qs, static_cast<const float*>(a.q) + long(head) * a.q_head, a.q_tok, q0, a.valid, a.dim);
+      simple_load<DP>(gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
       __syncthreads();
       float s[4][4] = {}, dp[4][4] = {};
       simple_scores<DP>(s, ks, qs, ty, tx);
@@ -334,8 +340,8 @@ packed_dkv_simple_kernel(BgnPackedAttention a, const float* bias2, const T* d_o,
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
       if (tx + 16 * d < a.dim) {
-        dk[at + tx + 16 * d] = from_float<T>(out_k[i][d] * a.scale);
-        dv[at + tx + 16 * d] = from_float<T>(out_v[i][d]);
+        dk[at + tx + 16 * d] = out_k[i][d] * a.scale;
+        dv[at + tx + 16 * d] = out_v[i][d];
       }
   }
 }
