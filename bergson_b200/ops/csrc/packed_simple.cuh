@@ -61,12 +61,13 @@ __device__ __forceinline__ void simple_scores(float (&acc)[4][4], const float* a
   }
 }
 
-// out[i][c] += sum_j p[4 ty + i][j] x[tx + 16 c][j].  In a tile with masked scores (exact zeros of p) a
-// zero takes no part at all: what stands in a masked row may be infinite or NaN.
+// out[i][c] += sum_j p[4 ty + i][j] x[tx + 16 c][j].  `careful`: a zero of p takes no part at all, for what
+// stands in a masked row may be infinite or NaN.  That is slow, and only done over again when a result has
+// turned out not to be finite.
 template <int DP>
 __device__ __forceinline__ void simple_product(float (&out)[4][DP / 16], const float* p, const float* x, int ty, int tx,
-                                               bool masked) {
-  if (!masked) {
+                                               bool careful) {
+  if (!careful) {
 #pragma unroll 4
     for (int j = 0; j < kSimpleTile; j += 4) {
       float4 a[4];
@@ -94,6 +95,16 @@ __device__ __forceinline__ void simple_product(float (&out)[4][DP / 16], const f
       }
     }
   }
+}
+
+template <int N>
+__device__ __forceinline__ bool some_not_finite(const float (&x)[4][N]) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int d = 0; d < N; ++d) bad |= !(fabsf(x[i][d]) < INFINITY);
+  return bad;
 }
 
 // Sum / maximum over the 16 threads that share a row group (half a warp).
@@ -129,15 +140,18 @@ __global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPa
   for (int i = 0; i < 4; ++i) {
     const int row = q0 + 4 * ty + i;
     first[i] = row < a.valid ? a.first_key[row] : 0x7fffffff;
+  }
+  const int q1 = min(q0 + kSimpleTile, a.valid);
+  bool careful = false;
+again:
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) out[i][d] = 0.f;
   }
-  const int q1 = min(q0 + kSimpleTile, a.valid);
-  const int last_first = q1 > q0 ? a.first_key[q1 - 1] : 0;
   for (int k0 = q1 > q0 ? a.first_key[q0] : q1; k0 < q1; k0 += kSimpleTile) {
-    const bool masked = k0 + kSimpleTile - 1 > q0 || k0 < last_first;
     __syncthreads();
     simple_load<DP>(ks, static_cast<const float*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
     simple_load<DP>(vs, static_cast<const float*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
@@ -170,7 +184,11 @@ __global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPa
       for (int d = 0; d < DP / 16; ++d) out[i][d] *= old;
     }
     __syncthreads();
-    simple_product<DP>(out, ps, vs, ty, tx, masked);
+    simple_product<DP>(out, ps, vs, ty, tx, careful);
+  }
+  if (!careful && __syncthreads_or(some_not_finite(out))) {
+    careful = true;
+    goto again;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -221,13 +239,15 @@ packed_dq_simple_kernel(BgnPackedAttention a, const float* o, const float* bias2
     }
     dl[i] = half_warp_sum(sum);
     if (tx == 0 && row < a.rows) delta[long(head) * a.pitch + row] = dl[i];
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) out[i][d] = 0.f;
   }
   const int q1 = min(q0 + kSimpleTile, a.valid);
-  const int last_first = q1 > q0 ? a.first_key[q1 - 1] : 0;
+  bool careful = false;
+again:
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) out[i][d] = 0.f;
   for (int k0 = q1 > q0 ? a.first_key[q0] : q1; k0 < q1; k0 += kSimpleTile) {
-    const bool masked = k0 + kSimpleTile - 1 > q0 || k0 < last_first;
     __syncthreads();
     simple_load<DP>(ks, static_cast<const float*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
     simple_load<DP>(vs, static_cast<const float*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
@@ -247,7 +267,11 @@ packed_dq_simple_kernel(BgnPackedAttention a, const float* o, const float* bias2
       }
     }
     __syncthreads();
-    simple_product<DP>(out, ds, ks, ty, tx, masked);
+    simple_product<DP>(out, ds, ks, ty, tx, careful);
+  }
+  if (!careful && __syncthreads_or(some_not_finite(out))) {
+    careful = true;
+    goto again;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -286,15 +310,17 @@ packed_dkv_simple_kernel(BgnPackedAttention a, const float* bias2, const float* 
     const int key = k0 + 4 * ty + i;
     end[i] = key < a.valid ? a.end_query[key] : 0;
     own_first[i] = key < a.valid ? a.first_key[key] : 0;
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) out_k[i][d] = out_v[i][d] = 0.f;
   }
   const int k1 = min(k0 + kSimpleTile, a.valid);
   const int q_end = k1 > k0 ? min(a.end_query[k1 - 1], a.valid) : 0;
-  const int first_end = k1 > k0 ? a.end_query[k0] : 0;
+  bool careful = false;
+again:
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) out_k[i][d] = out_v[i][d] = 0.f;
   for (int head = kv_head * group; head < (kv_head + 1) * group; ++head) {
     for (int q0 = k0; q0 < q_end; q0 += kSimpleTile) {
-      const bool masked = q0 < k0 + kSimpleTile || q0 + kSimpleTile > first_end;
       __syncthreads();
       simple_load<DP>(qs, static_cast<const float*>(a.q) + long(head) * a.q_head, a.q_tok, q0, a.valid, a.dim);
       simple_load<DP>(gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
@@ -322,15 +348,19 @@ packed_dkv_simple_kernel(BgnPackedAttention a, const float* bias2, const float* 
 #pragma unroll
         for (int j = 0; j < 4; ++j) ps[(4 * ty + i) * kSimplePitch + 4 * tx + j] = s[i][j];
       __syncthreads();
-      simple_product<DP>(out_v, ps, gs, ty, tx, masked);
+      simple_product<DP>(out_v, ps, gs, ty, tx, careful);
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) ps[(4 * ty + i) * kSimplePitch + 4 * tx + j] = dp[i][j];
       __syncthreads();
-      simple_product<DP>(out_k, ps, qs, ty, tx, masked);
+      simple_product<DP>(out_k, ps, qs, ty, tx, careful);
     }
+  }
+  if (!careful && __syncthreads_or(some_not_finite(out_k) || some_not_finite(out_v))) {
+    careful = true;
+    goto again;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
