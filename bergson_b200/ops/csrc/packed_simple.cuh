@@ -13,9 +13,9 @@
 // and one order, so results do not depend on scheduling.
 //
 // Bound by the FMA units and the shared memory that feeds them (a thread's 4 x 4 scores take two 16-byte loads
-// to 16 operations): 8 documents of 1024 tokens, 12 heads of 64, forward 500 us (26 TFLOP/s), backward
-// 1510 us.  Small batches wait for one block's chain of tiles.  Fetching a tile into registers while the one
-// before it is at work took 540 and 1715 us: the registers leave room for one block on an SM instead of two.
+// to 16 operations): 8 documents of 1024 tokens, 12 heads of 64, forward 480 us (27 TFLOP/s), backward
+// 1460 us.  Small batches wait for one block's chain of tiles.  Fetching a tile into registers while the one
+// before it is at work took 540 and 1715 us (then against 500 and 1510): the registers leave room for one block on an SM instead of two.
 #pragma once
 
 #include "common.cuh"
@@ -28,17 +28,27 @@ constexpr int kSimplePitch = kSimpleTile + 4;  // floats between the rows of a t
 constexpr int kSimpleThreads = 256;          // 16 x 16 threads, 4 x 4 scores each
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Tile of `kSimpleTile` tokens in shared memory as [feature][token]; rows at or past `limit` and
-// features at or past `dim` are zero.
-template <int DP>
-__device__ __forceinline__ void simple_load(float* dst, const float* src, long tok_stride, int t0, int limit, int dim) {
-  // One packet per step; neighbouring threads take neighbouring tokens, so the transposed stores
-  // fall into different banks.
-  for (int i = threadIdx.x; i < kSimpleTile * (DP / 4); i += kSimpleThreads) {
-    const int tok = i % kSimpleTile, d = (i / kSimpleTile) * 4;
-    float4 p = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (t0 + tok < limit && d < dim) p = *reinterpret_cast<const float4*>(src + long(t0 + tok) * tok_stride + d);
-    float* to = dst + d * kSimplePitch + tok;
+// Tiles of `kSimpleTile` tokens of two operands (or one) in shared memory, as [feature][token]; rows at or past
+// `limit` and features at or past `dim` are zero.  All loads are on their way before the first store.
+template <int DP, bool TWO = true>
+__device__ __forceinline__ void simple_load(float* dst_x, const float* x, long x_tok, float* dst_y, const float* y,
+                                            long y_tok, int t0, int limit, int dim) {
+  constexpr int kPackets = kSimpleTile * (DP / 4) / kSimpleThreads;
+  float4 held[2][kPackets];
+  // Neighbouring threads take neighbouring tokens, so that the transposed stores fall into different banks.
+#pragma unroll
+  for (int n = 0; n < (TWO ? 2 : 1) * kPackets; ++n) {
+    const int i = threadIdx.x + n % kPackets * kSimpleThreads, tok = i % kSimpleTile, d = (i / kSimpleTile) * 4;
+    const float* from = n < kPackets ? x + long(t0 + tok) * x_tok : y + long(t0 + tok) * y_tok;
+    float4& to = held[n / kPackets][n % kPackets];
+    to = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (t0 + tok < limit && d < dim) to = *reinterpret_cast<const float4*>(from + d);
+  }
+#pragma unroll
+  for (int n = 0; n < (TWO ? 2 : 1) * kPackets; ++n) {
+    const int i = threadIdx.x + n % kPackets * kSimpleThreads;
+    const float4 p = held[n / kPackets][n % kPackets];
+    float* to = (n < kPackets ? dst_x : dst_y) + (i / kSimpleTile) * 4 * kSimplePitch + i % kSimpleTile;
     to[0] = p.x;
     to[kSimplePitch] = p.y;
     to[2 * kSimplePitch] = p.z;
@@ -59,6 +69,10 @@ __device__ __forceinline__ void simple_scores(float (&acc)[4][4], const float* a
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[i], ys[j], acc[i][j]);
   }
+}
+
+__device__ __forceinline__ void store_scores(float* p, const float (&s)[4], int row, int tx) {
+  *reinterpret_cast<float4*>(p + row * kSimplePitch + 4 * tx) = make_float4(s[0], s[1], s[2], s[3]);
 }
 
 // out[i][c] += sum_j p[4 ty + i][j] x[tx + 16 c][j].  `careful`: a zero of p takes no part at all, for what
@@ -133,7 +147,8 @@ __global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPa
   if (q0 >= a.rows) return;
   const float c = a.scale * kLog2e;
 
-  simple_load<DP>(qs, static_cast<const float*>(a.q) + long(head) * a.q_head, a.q_tok, q0, a.valid, a.dim);
+  const float* q = static_cast<const float*>(a.q) + long(head) * a.q_head;
+  simple_load<DP, false>(qs, q, a.q_tok, nullptr, nullptr, 0, q0, a.valid, a.dim);
   int first[4];
   float m[4], l[4], out[4][DP / 16];
 #pragma unroll
@@ -141,6 +156,8 @@ __global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPa
     const int row = q0 + 4 * ty + i;
     first[i] = row < a.valid ? a.first_key[row] : 0x7fffffff;
   }
+  const float* k = static_cast<const float*>(a.k) + long(kv_head) * a.k_head;
+  const float* v = static_cast<const float*>(a.v) + long(kv_head) * a.v_head;
   const int q1 = min(q0 + kSimpleTile, a.valid);
   bool careful = false;
 again:
@@ -153,8 +170,7 @@ again:
   }
   for (int k0 = q1 > q0 ? a.first_key[q0] : q1; k0 < q1; k0 += kSimpleTile) {
     __syncthreads();
-    simple_load<DP>(ks, static_cast<const float*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
-    simple_load<DP>(vs, static_cast<const float*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
+    simple_load<DP>(ks, k, a.k_tok, vs, v, a.v_tok, k0, a.valid, a.dim);
     __syncthreads();
     float s[4][4] = {};
     simple_scores<DP>(s, qs, ks, ty, tx);
@@ -174,10 +190,10 @@ again:
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float p = exp2f(s[i][j] - base);
-        ps[(4 * ty + i) * kSimplePitch + 4 * tx + j] = p;
-        sum += p;
+        s[i][j] = exp2f(s[i][j] - base);
+        sum += s[i][j];
       }
+      store_scores(ps, s[i], 4 * ty + i, tx);
       l[i] = l[i] * old + half_warp_sum(sum);
       m[i] = mx;
 #pragma unroll
@@ -221,8 +237,8 @@ packed_dq_simple_kernel(BgnPackedAttention a, const float* o, const float* bias2
   if (q0 >= a.rows) return;
   const float c = a.scale * kLog2e;
 
-  simple_load<DP>(qs, static_cast<const float*>(a.q) + long(head) * a.q_head, a.q_tok, q0, a.valid, a.dim);
-  simple_load<DP>(gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
+  const float* q = static_cast<const float*>(a.q) + long(head) * a.q_head;
+  simple_load<DP>(qs, q, a.q_tok, gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
   __syncthreads();
   int first[4];
   float bias[4], dl[4], out[4][DP / 16];
@@ -240,6 +256,8 @@ packed_dq_simple_kernel(BgnPackedAttention a, const float* o, const float* bias2
     dl[i] = half_warp_sum(sum);
     if (tx == 0 && row < a.rows) delta[long(head) * a.pitch + row] = dl[i];
   }
+  const float* k = static_cast<const float*>(a.k) + long(kv_head) * a.k_head;
+  const float* v = static_cast<const float*>(a.v) + long(kv_head) * a.v_head;
   const int q1 = min(q0 + kSimpleTile, a.valid);
   bool careful = false;
 again:
@@ -249,8 +267,7 @@ again:
     for (int d = 0; d < DP / 16; ++d) out[i][d] = 0.f;
   for (int k0 = q1 > q0 ? a.first_key[q0] : q1; k0 < q1; k0 += kSimpleTile) {
     __syncthreads();
-    simple_load<DP>(ks, static_cast<const float*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
-    simple_load<DP>(vs, static_cast<const float*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
+    simple_load<DP>(ks, k, a.k_tok, vs, v, a.v_tok, k0, a.valid, a.dim);
     __syncthreads();
     float s[4][4] = {}, dp[4][4] = {};
     simple_scores<DP>(s, qs, ks, ty, tx);
@@ -263,8 +280,9 @@ again:
         const int key = k0 + 4 * tx + j;
         // A row with one key has P = 1 and no gradient through the softmax: exactly zero.
         const bool in = key >= first[i] && key <= row && first[i] < row;
-        ds[(4 * ty + i) * kSimplePitch + 4 * tx + j] = in ? exp2f(__fmul_rn(s[i][j], c) + bias[i]) * (dp[i][j] - dl[i]) : 0.f;
+        s[i][j] = in ? exp2f(__fmul_rn(s[i][j], c) + bias[i]) * (dp[i][j] - dl[i]) : 0.f;
       }
+      store_scores(ds, s[i], 4 * ty + i, tx);
     }
     __syncthreads();
     simple_product<DP>(out, ds, ks, ty, tx, careful);
@@ -301,8 +319,8 @@ packed_dkv_simple_kernel(BgnPackedAttention a, const float* bias2, const float* 
   if (k0 >= a.rows) return;
   const float c = a.scale * kLog2e;
 
-  simple_load<DP>(ks, static_cast<const float*>(a.k) + long(kv_head) * a.k_head, a.k_tok, k0, a.valid, a.dim);
-  simple_load<DP>(vs, static_cast<const float*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
+  simple_load<DP>(ks, static_cast<const float*>(a.k) + long(kv_head) * a.k_head, a.k_tok, vs,
+                  static_cast<const float*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
   int end[4], own_first[4];
   float out_k[4][DP / 16], out_v[4][DP / 16];
 #pragma unroll
@@ -322,8 +340,8 @@ again:
   for (int head = kv_head * group; head < (kv_head + 1) * group; ++head) {
     for (int q0 = k0; q0 < q_end; q0 += kSimpleTile) {
       __syncthreads();
-      simple_load<DP>(qs, static_cast<const float*>(a.q) + long(head) * a.q_head, a.q_tok, q0, a.valid, a.dim);
-      simple_load<DP>(gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
+      const float* q = static_cast<const float*>(a.q) + long(head) * a.q_head;
+      simple_load<DP>(qs, q, a.q_tok, gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
       __syncthreads();
       float s[4][4] = {}, dp[4][4] = {};
       simple_scores<DP>(s, ks, qs, ty, tx);
@@ -344,16 +362,12 @@ again:
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) ps[(4 * ty + i) * kSimplePitch + 4 * tx + j] = s[i][j];
+      for (int i = 0; i < 4; ++i) store_scores(ps, s[i], 4 * ty + i, tx);
       __syncthreads();
       simple_product<DP>(out_v, ps, gs, ty, tx, careful);
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) ps[(4 * ty + i) * kSimplePitch + 4 * tx + j] = dp[i][j];
+      for (int i = 0; i < 4; ++i) store_scores(ps, dp[i], 4 * ty + i, tx);
       __syncthreads();
       simple_product<DP>(out_k, ps, qs, ty, tx, careful);
     }
