@@ -34,36 +34,45 @@ cudaError_t allow_smem(const void* kernel, int bytes) try {
   return cudaErrorMemoryAllocation;
 }
 
-template <int DP>
+template <int DP, int R>
 cudaError_t simple_fwd(const BgnPackedAttention& a, void* o, float* bias2, cudaStream_t stream) {
   constexpr int smem = simple_smem<DP>(3);
-  auto kern = packed_fwd_simple_kernel<DP>;
+  auto kern = packed_fwd_simple_kernel<DP, R>;
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
   const unsigned grid = unsigned((a.rows + 127) / 128) * 2u * unsigned(a.heads);
-  kern<<<grid, kSimpleThreads, smem, stream>>>(a, static_cast<float*>(o), bias2);
+  kern<<<grid, simple_threads<R>(), smem, stream>>>(a, static_cast<float*>(o), bias2);
   return cudaGetLastError();
 }
 
-template <int DP>
+template <int DP, int R>
 cudaError_t simple_bwd(const BgnPackedAttention& a, const void* o, const float* bias2, const void* d_o, long do_tok,
                        long do_head, float* delta, void* dq, void* dk, void* dv, cudaStream_t stream) {
   constexpr int smem = simple_smem<DP>(4);
-  auto kq = packed_dq_simple_kernel<DP>;
-  auto kk = packed_dkv_simple_kernel<DP>;
+  auto kq = packed_dq_simple_kernel<DP, R>;
+  auto kk = packed_dkv_simple_kernel<DP, R>;
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kq), smem);
   if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(kk), smem);
   if (e != cudaSuccess) return e;
   const unsigned tiles = unsigned((a.rows + 127) / 128) * 2u;
-  kq<<<tiles * unsigned(a.heads), kSimpleThreads, smem, stream>>>(a, static_cast<const float*>(o), bias2,
+  kq<<<tiles * unsigned(a.heads), simple_threads<R>(), smem, stream>>>(a, static_cast<const float*>(o), bias2,
                                                                   static_cast<const float*>(d_o), do_tok, do_head, delta,
                                                                   static_cast<float*>(dq));
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  kk<<<tiles * unsigned(a.kv_heads), kSimpleThreads, smem, stream>>>(a, bias2, static_cast<const float*>(d_o), do_tok,
+  kk<<<tiles * unsigned(a.kv_heads), simple_threads<R>(), smem, stream>>>(a, bias2, static_cast<const float*>(d_o), do_tok,
                                                                      do_head, delta, static_cast<float*>(dk),
                                                                      static_cast<float*>(dv));
   return cudaGetLastError();
+}
+
+// fp32: eight rows to a thread take fewer loads from shared memory for the same operations than four, and half the
+// threads.  Up to 64 features that is faster in the forward pass (8 documents of 1024, 12 heads of 64: 435 against
+// 480 us; 7 of 2000 tokens together, 4 heads of 32: 30 against 34); in the backward pass where there are more than
+// two blocks to an SM (1363 against 1462 us; but 91 against 86 for the small batch).  At 128 features the registers do
+// not suffice (2 of 2048, 16 over 4 heads: forward 1706 against 1239 us).
+bool many_blocks(const BgnPackedAttention& a) {
+  return (a.rows + 127) / 128 * 2 * a.heads > 2 * 148;
 }
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -218,7 +227,7 @@ extern "C" int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, vo
   if (!sound(a)) return int(cudaErrorInvalidValue);
   const bool narrow = a->dim <= 64;
   if (a->type == 2) {
-    auto run = a->dim <= 32 ? simple_fwd<32> : (narrow ? simple_fwd<64> : simple_fwd<128>);
+    auto run = a->dim <= 32 ? simple_fwd<32, 8> : narrow ? simple_fwd<64, 8> : simple_fwd<128, 4>;
     return int(run(*a, o, bias2, stream));
   }
   if (a->type == 1)
@@ -233,7 +242,9 @@ extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void*
   if (!sound(a)) return int(cudaErrorInvalidValue);
   const bool narrow = a->dim <= 64;
   if (a->type == 2) {
-    auto run = a->dim <= 32 ? simple_bwd<32> : (narrow ? simple_bwd<64> : simple_bwd<128>);
+    auto run = simple_bwd<128, 4>;
+    if (narrow && many_blocks(*a)) run = a->dim <= 32 ? simple_bwd<32, 8> : simple_bwd<64, 8>;
+    else if (narrow) run = a->dim <= 32 ? simple_bwd<32, 4> : simple_bwd<64, 4>;
     return int(run(*a, o, bias2, d_o, do_tok, do_head, delta, dq, dk, dv, stream));
   }
   auto run = a->type == 1 ? (narrow ? tensor_bwd<1, 64> : tensor_bwd<1, 128>)

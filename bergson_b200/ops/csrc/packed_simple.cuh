@@ -12,10 +12,11 @@
 // dQ and dK/dV are two kernels that recompute P from the stored log-sum-exp: sums stay in one block
 // and one order, so results do not depend on scheduling.
 //
-// Bound by the FMA units and the shared memory that feeds them (a thread's 4 x 4 scores take two 16-byte loads
-// to 16 operations): 8 documents of 1024 tokens, 12 heads of 64, forward 480 us (27 TFLOP/s), backward
-// 1460 us.  Small batches wait for one block's chain of tiles.  Fetching a tile into registers while the one
-// before it is at work took 540 and 1715 us (then against 500 and 1510): the registers leave room for one block on an SM instead of two.
+// Bound by the FMA units and the shared memory that feeds them (a thread's 8 x 4 scores take three 16-byte loads
+// to 32 operations): 8 documents of 1024 tokens, 12 heads of 64, forward 435 us (30 TFLOP/s), backward
+// 1363 us.  Small batches wait for one block's chain of tiles; two rows to a thread did not shorten it.
+// Fetching a tile into registers while the one before it is at work was slower (540 and 1715 against 500 and
+// 1510 us, with four rows to a thread): the registers leave room for one block on an SM instead of two.
 #pragma once
 
 #include "common.cuh"
@@ -25,20 +26,25 @@ namespace bgn {
 
 constexpr int kSimpleTile = 64;              // queries and keys of a tile
 constexpr int kSimplePitch = kSimpleTile + 4;  // floats between the rows of a tile in shared memory
-constexpr int kSimpleThreads = 256;          // 16 x 16 threads, 4 x 4 scores each
+
+// R: rows of a tile that a thread has, 4 or 8; 16 threads share a row, with 4 scores each.
+template <int R>
+constexpr int simple_threads() {
+  return 16 * kSimpleTile / R;
+}
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Tiles of `kSimpleTile` tokens of two operands (or one) in shared memory, as [feature][token]; rows at or past
 // `limit` and features at or past `dim` are zero.  All loads are on their way before the first store.
-template <int DP, bool TWO = true>
+template <int DP, int R, bool TWO = true>
 __device__ __forceinline__ void simple_load(float* dst_x, const float* x, long x_tok, float* dst_y, const float* y,
                                             long y_tok, int t0, int limit, int dim) {
-  constexpr int kPackets = kSimpleTile * (DP / 4) / kSimpleThreads;
+  constexpr int kPackets = kSimpleTile * (DP / 4) / simple_threads<R>();
   float4 held[2][kPackets];
   // Neighbouring threads take neighbouring tokens, so that the transposed stores fall into different banks.
 #pragma unroll
   for (int n = 0; n < (TWO ? 2 : 1) * kPackets; ++n) {
-    const int i = threadIdx.x + n % kPackets * kSimpleThreads, tok = i % kSimpleTile, d = (i / kSimpleTile) * 4;
+    const int i = threadIdx.x + n % kPackets * simple_threads<R>(), tok = i % kSimpleTile, d = (i / kSimpleTile) * 4;
     const float* from = n < kPackets ? x + long(t0 + tok) * x_tok : y + long(t0 + tok) * y_tok;
     float4& to = held[n / kPackets][n % kPackets];
     to = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -46,7 +52,7 @@ __device__ __forceinline__ void simple_load(float* dst_x, const float* x, long x
   }
 #pragma unroll
   for (int n = 0; n < (TWO ? 2 : 1) * kPackets; ++n) {
-    const int i = threadIdx.x + n % kPackets * kSimpleThreads;
+    const int i = threadIdx.x + n % kPackets * simple_threads<R>();
     const float4 p = held[n / kPackets][n % kPackets];
     float* to = (n < kPackets ? dst_x : dst_y) + (i / kSimpleTile) * 4 * kSimplePitch + i % kSimpleTile;
     to[0] = p.x;
@@ -57,17 +63,18 @@ __device__ __forceinline__ void simple_load(float* dst_x, const float* x, long x
 }
 
 // acc[i][j] += sum_d a[d][4 ty + i] b[d][4 tx + j]
-template <int DP>
-__device__ __forceinline__ void simple_scores(float (&acc)[4][4], const float* a, const float* b, int ty, int tx) {
+template <int DP, int R>
+__device__ __forceinline__ void simple_scores(float (&acc)[R][4], const float* a, const float* b, int ty, int tx) {
 #pragma unroll 8
   for (int d = 0; d < DP; ++d) {
-    const float4 x = *reinterpret_cast<const float4*>(a + d * kSimplePitch + 4 * ty);
+    struct alignas(16) Rows { float v[R]; };
+    const Rows x = *reinterpret_cast<const Rows*>(a + d * kSimplePitch + R * ty);
     const float4 y = *reinterpret_cast<const float4*>(b + d * kSimplePitch + 4 * tx);
-    const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    const float ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[i], ys[j], acc[i][j]);
+      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(x.v[i], ys[j], acc[i][j]);
   }
 }
 
@@ -78,44 +85,44 @@ __device__ __forceinline__ void store_scores(float* p, const float (&s)[4], int 
 // out[i][c] += sum_j p[4 ty + i][j] x[tx + 16 c][j].  `careful`: a zero of p takes no part at all, for what
 // stands in a masked row may be infinite or NaN.  That is slow, and only done over again when a result has
 // turned out not to be finite.
-template <int DP>
-__device__ __forceinline__ void simple_product(float (&out)[4][DP / 16], const float* p, const float* x, int ty, int tx,
+template <int DP, int R>
+__device__ __forceinline__ void simple_product(float (&out)[R][DP / 16], const float* p, const float* x, int ty, int tx,
                                                bool careful) {
   if (!careful) {
 #pragma unroll 4
     for (int j = 0; j < kSimpleTile; j += 4) {
-      float4 a[4];
+      float4 a[R];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(p + (4 * ty + i) * kSimplePitch + j);
+      for (int i = 0; i < R; ++i) a[i] = *reinterpret_cast<const float4*>(p + (R * ty + i) * kSimplePitch + j);
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
         const float4 b = *reinterpret_cast<const float4*>(x + (tx + 16 * c) * kSimplePitch + j);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < R; ++i)
           out[i][c] = fmaf(a[i].x, b.x, fmaf(a[i].y, b.y, fmaf(a[i].z, b.z, fmaf(a[i].w, b.w, out[i][c]))));
       }
     }
   } else {
     for (int j = 0; j < kSimpleTile; ++j) {
-      float a[4];
+      float a[R];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = p[(4 * ty + i) * kSimplePitch + j];
+      for (int i = 0; i < R; ++i) a[i] = p[(R * ty + i) * kSimplePitch + j];
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
         const float b = x[(tx + 16 * c) * kSimplePitch + j];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < R; ++i)
           if (a[i] != 0.f) out[i][c] = fmaf(a[i], b, out[i][c]);
       }
     }
   }
 }
 
-template <int N>
-__device__ __forceinline__ bool some_not_finite(const float (&x)[4][N]) {
+template <int R, int N>
+__device__ __forceinline__ bool some_not_finite(const float (&x)[R][N]) {
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
     for (int d = 0; d < N; ++d) bad |= !(fabsf(x[i][d]) < INFINITY);
   return bad;
@@ -133,8 +140,8 @@ __device__ __forceinline__ float half_warp_max(float v) {
   return v;
 }
 
-template <int DP>
-__global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPackedAttention a, float* o, float* bias2) {
+template <int DP, int R>
+__global__ void __launch_bounds__(simple_threads<R>()) packed_fwd_simple_kernel(BgnPackedAttention a, float* o, float* bias2) {
   extern __shared__ float smem[];
   float* qs = smem;
   float* ks = qs + DP * kSimplePitch;
@@ -148,12 +155,12 @@ __global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPa
   const float c = a.scale * kLog2e;
 
   const float* q = static_cast<const float*>(a.q) + long(head) * a.q_head;
-  simple_load<DP, false>(qs, q, a.q_tok, nullptr, nullptr, 0, q0, a.valid, a.dim);
-  int first[4];
-  float m[4], l[4], out[4][DP / 16];
+  simple_load<DP, R, false>(qs, q, a.q_tok, nullptr, nullptr, 0, q0, a.valid, a.dim);
+  int first[R];
+  float m[R], l[R], out[R][DP / 16];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = q0 + 4 * ty + i;
+  for (int i = 0; i < R; ++i) {
+    const int row = q0 + R * ty + i;
     first[i] = row < a.valid ? a.first_key[row] : 0x7fffffff;
   }
   const float* k = static_cast<const float*>(a.k) + long(kv_head) * a.k_head;
@@ -162,7 +169,7 @@ __global__ void __launch_bounds__(kSimpleThreads) packed_fwd_simple_kernel(BgnPa
   bool careful = false;
 again:
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < R; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
@@ -170,13 +177,13 @@ again:
   }
   for (int k0 = q1 > q0 ? a.first_key[q0] : q1; k0 < q1; k0 += kSimpleTile) {
     __syncthreads();
-    simple_load<DP>(ks, k, a.k_tok, vs, v, a.v_tok, k0, a.valid, a.dim);
+    simple_load<DP, R>(ks, k, a.k_tok, vs, v, a.v_tok, k0, a.valid, a.dim);
     __syncthreads();
-    float s[4][4] = {};
-    simple_scores<DP>(s, qs, ks, ty, tx);
+    float s[R][4] = {};
+    simple_scores<DP, R>(s, qs, ks, ty, tx);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = q0 + 4 * ty + i;
+    for (int i = 0; i < R; ++i) {
+      const int row = q0 + R * ty + i;
       float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -193,22 +200,22 @@ again:
         s[i][j] = exp2f(s[i][j] - base);
         sum += s[i][j];
       }
-      store_scores(ps, s[i], 4 * ty + i, tx);
+      store_scores(ps, s[i], R * ty + i, tx);
       l[i] = l[i] * old + half_warp_sum(sum);
       m[i] = mx;
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) out[i][d] *= old;
     }
     __syncthreads();
-    simple_product<DP>(out, ps, vs, ty, tx, careful);
+    simple_product<DP, R>(out, ps, vs, ty, tx, careful);
   }
   if (!careful && __syncthreads_or(some_not_finite(out))) {
     careful = true;
     goto again;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = q0 + 4 * ty + i;
+  for (int i = 0; i < R; ++i) {
+    const int row = q0 + R * ty + i;
     if (row >= a.rows) continue;
     const bool some = row < a.valid && first[i] <= row;
     const float inv = some ? 1.f / l[i] : 0.f;
@@ -220,8 +227,8 @@ again:
   }
 }
 
-template <int DP>
-__global__ void __launch_bounds__(kSimpleThreads)
+template <int DP, int R>
+__global__ void __launch_bounds__(simple_threads<R>())
 packed_dq_simple_kernel(BgnPackedAttention a, const float* o, const float* bias2, const float* d_o, long do_tok, long do_head,
                         float* delta, float* dq) {
   extern __shared__ float smem[];
@@ -238,20 +245,20 @@ packed_dq_simple_kernel(BgnPackedAttention a, const float* o, const float* bias2
   const float c = a.scale * kLog2e;
 
   const float* q = static_cast<const float*>(a.q) + long(head) * a.q_head;
-  simple_load<DP>(qs, q, a.q_tok, gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
+  simple_load<DP, R>(qs, q, a.q_tok, gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
   __syncthreads();
-  int first[4];
-  float bias[4], dl[4], out[4][DP / 16];
+  int first[R];
+  float bias[R], dl[R], out[R][DP / 16];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = q0 + 4 * ty + i;
+  for (int i = 0; i < R; ++i) {
+    const int row = q0 + R * ty + i;
     const bool in = row < a.valid;
     first[i] = in ? a.first_key[row] : 0x7fffffff;
     bias[i] = in ? bias2[long(head) * a.pitch + row] : -INFINITY;
     float sum = 0.f;
     if (in) {
       const float* orow = o + (long(row) * a.heads + head) * a.dim;
-      for (int d = tx; d < a.dim; d += 16) sum = fmaf(orow[d], gs[d * kSimplePitch + 4 * ty + i], sum);
+      for (int d = tx; d < a.dim; d += 16) sum = fmaf(orow[d], gs[d * kSimplePitch + R * ty + i], sum);
     }
     dl[i] = half_warp_sum(sum);
     if (tx == 0 && row < a.rows) delta[long(head) * a.pitch + row] = dl[i];
@@ -262,19 +269,19 @@ packed_dq_simple_kernel(BgnPackedAttention a, const float* o, const float* bias2
   bool careful = false;
 again:
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) out[i][d] = 0.f;
   for (int k0 = q1 > q0 ? a.first_key[q0] : q1; k0 < q1; k0 += kSimpleTile) {
     __syncthreads();
-    simple_load<DP>(ks, k, a.k_tok, vs, v, a.v_tok, k0, a.valid, a.dim);
+    simple_load<DP, R>(ks, k, a.k_tok, vs, v, a.v_tok, k0, a.valid, a.dim);
     __syncthreads();
-    float s[4][4] = {}, dp[4][4] = {};
-    simple_scores<DP>(s, qs, ks, ty, tx);
-    simple_scores<DP>(dp, gs, vs, ty, tx);
+    float s[R][4] = {}, dp[R][4] = {};
+    simple_scores<DP, R>(s, qs, ks, ty, tx);
+    simple_scores<DP, R>(dp, gs, vs, ty, tx);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = q0 + 4 * ty + i;
+    for (int i = 0; i < R; ++i) {
+      const int row = q0 + R * ty + i;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int key = k0 + 4 * tx + j;
@@ -282,18 +289,18 @@ again:
         const bool in = key >= first[i] && key <= row && first[i] < row;
         s[i][j] = in ? exp2f(__fmul_rn(s[i][j], c) + bias[i]) * (dp[i][j] - dl[i]) : 0.f;
       }
-      store_scores(ds, s[i], 4 * ty + i, tx);
+      store_scores(ds, s[i], R * ty + i, tx);
     }
     __syncthreads();
-    simple_product<DP>(out, ds, ks, ty, tx, careful);
+    simple_product<DP, R>(out, ds, ks, ty, tx, careful);
   }
   if (!careful && __syncthreads_or(some_not_finite(out))) {
     careful = true;
     goto again;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = q0 + 4 * ty + i;
+  for (int i = 0; i < R; ++i) {
+    const int row = q0 + R * ty + i;
     if (row >= a.rows) continue;
     float* dst = dq + (long(row) * a.heads + head) * a.dim;
 #pragma unroll
@@ -302,8 +309,8 @@ again:
   }
 }
 
-template <int DP>
-__global__ void __launch_bounds__(kSimpleThreads)
+template <int DP, int R>
+__global__ void __launch_bounds__(simple_threads<R>())
 packed_dkv_simple_kernel(BgnPackedAttention a, const float* bias2, const float* d_o, long do_tok, long do_head,
                          const float* delta, float* dk, float* dv) {
   extern __shared__ float smem[];
@@ -319,13 +326,13 @@ packed_dkv_simple_kernel(BgnPackedAttention a, const float* bias2, const float* 
   if (k0 >= a.rows) return;
   const float c = a.scale * kLog2e;
 
-  simple_load<DP>(ks, static_cast<const float*>(a.k) + long(kv_head) * a.k_head, a.k_tok, vs,
+  simple_load<DP, R>(ks, static_cast<const float*>(a.k) + long(kv_head) * a.k_head, a.k_tok, vs,
                   static_cast<const float*>(a.v) + long(kv_head) * a.v_head, a.v_tok, k0, a.valid, a.dim);
-  int end[4], own_first[4];
-  float out_k[4][DP / 16], out_v[4][DP / 16];
+  int end[R], own_first[R];
+  float out_k[R][DP / 16], out_v[R][DP / 16];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int key = k0 + 4 * ty + i;
+  for (int i = 0; i < R; ++i) {
+    const int key = k0 + R * ty + i;
     end[i] = key < a.valid ? a.end_query[key] : 0;
     own_first[i] = key < a.valid ? a.first_key[key] : 0;
   }
@@ -334,18 +341,18 @@ packed_dkv_simple_kernel(BgnPackedAttention a, const float* bias2, const float* 
   bool careful = false;
 again:
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) out_k[i][d] = out_v[i][d] = 0.f;
   for (int head = kv_head * group; head < (kv_head + 1) * group; ++head) {
     for (int q0 = k0; q0 < q_end; q0 += kSimpleTile) {
       __syncthreads();
       const float* q = static_cast<const float*>(a.q) + long(head) * a.q_head;
-      simple_load<DP>(qs, q, a.q_tok, gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
+      simple_load<DP, R>(qs, q, a.q_tok, gs, d_o + long(head) * do_head, do_tok, q0, a.valid, a.dim);
       __syncthreads();
-      float s[4][4] = {}, dp[4][4] = {};
-      simple_scores<DP>(s, ks, qs, ty, tx);
-      simple_scores<DP>(dp, vs, gs, ty, tx);
+      float s[R][4] = {}, dp[R][4] = {};
+      simple_scores<DP, R>(s, ks, qs, ty, tx);
+      simple_scores<DP, R>(dp, vs, gs, ty, tx);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int row = q0 + 4 * tx + j;
@@ -353,8 +360,8 @@ again:
         const float bias = in_row ? bias2[long(head) * a.pitch + row] : -INFINITY;
         const float dl = in_row ? delta[long(head) * a.pitch + row] : 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = k0 + 4 * ty + i;
+        for (int i = 0; i < R; ++i) {
+          const int key = k0 + R * ty + i;
           const bool in = row >= key && row < end[i];
           const float p = in ? exp2f(__fmul_rn(s[i][j], c) + bias) : 0.f;
           s[i][j] = p;
@@ -362,14 +369,14 @@ again:
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) store_scores(ps, s[i], 4 * ty + i, tx);
+      for (int i = 0; i < R; ++i) store_scores(ps, s[i], R * ty + i, tx);
       __syncthreads();
-      simple_product<DP>(out_v, ps, gs, ty, tx, careful);
+      simple_product<DP, R>(out_v, ps, gs, ty, tx, careful);
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) store_scores(ps, dp[i], 4 * ty + i, tx);
+      for (int i = 0; i < R; ++i) store_scores(ps, dp[i], R * ty + i, tx);
       __syncthreads();
-      simple_product<DP>(out_k, ps, qs, ty, tx, careful);
+      simple_product<DP, R>(out_k, ps, qs, ty, tx, careful);
     }
   }
   if (!careful && __syncthreads_or(some_not_finite(out_k) || some_not_finite(out_v))) {
@@ -377,8 +384,8 @@ again:
     goto again;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int key = k0 + 4 * ty + i;
+  for (int i = 0; i < R; ++i) {
+    const int key = k0 + R * ty + i;
     if (key >= a.rows) continue;
     const long at = (long(key) * a.kv_heads + kv_head) * a.dim;
 #pragma unroll
