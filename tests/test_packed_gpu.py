@@ -157,6 +157,72 @@ def test_attention_keeps_documents_apart(native, d, poison, dtype):
         assert not torch.isfinite(got[name][begin:begin + lens[bad]]).all()
 
 
+def test_offsets_beyond_32_bits(native):
+    """More than 2^31 elements in q, o and the logits: the last rows are as they are alone."""
+    n, docs, hq, d = 128, 1100, 120, 128
+    rows = n * docs
+    assert rows * hq * d > 2**31
+    p, alone = ops.PackedSequences([n] * docs, device="cuda"), ops.PackedSequences([n], device="cuda")
+    q = torch.empty(rows, hq, d, device="cuda", dtype=torch.bfloat16).normal_()
+    k, v = (_rand((rows, 1, d), torch.bfloat16, 190 + i) for i in range(2))
+    cos, sin = ops.rotary_tables(n, d, 1e4, "cuda")
+
+    def run(packing, q, k, v):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        turned = ops.packed_rotary(*leaves[:2], cos, sin, d, packing)
+        o = ops.packed_causal_attention(*turned, leaves[2], packing)
+        return (o.detach(), *torch.autograd.grad(o, leaves, o.detach()))
+
+    got, want = run(p, q, k, v), run(alone, q[-n:], k[-n:], v[-n:])
+    for x, y in zip(got, want):
+        assert torch.equal(x[-n:], y)
+    _status_ok(native)
+    del got, q
+    T, V = 17000, 128256
+    assert T * V > 2**31
+    z = torch.empty(T, V, device="cuda", dtype=torch.bfloat16).normal_().requires_grad_()
+    ids, t = torch.randint(0, V, (T, 8), device="cuda"), _rand((T, 8), torch.float32, 195)
+    loss = ops.token_distillation(z, ids, t)
+    (g,) = torch.autograd.grad(loss.sum(), z)
+    end = slice(T - 600, T)
+    last = z.detach()[end].clone().requires_grad_()
+    one = ops.token_distillation(last, ids[end], t[end])
+    (g1,) = torch.autograd.grad(one.sum(), last)
+    assert torch.equal(loss[end], one) and torch.equal(g[end], g1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradients_of_some_operands_only(native, dtype):
+    lens = [150, 3, 70]
+    p = ops.PackedSequences(lens, device="cuda")
+    rows, d = sum(lens), 64
+    q, k, v, do = (_rand((rows, h, d), dtype, 200 + i) for i, h in enumerate((4, 2, 2, 4)))
+    want, tol = attention64(q, k, v, lens, do=do)
+    for i, name in enumerate(("dq", "dk", "dv")):
+        xs = [q, k, v]
+        leaf = xs[i] = xs[i].detach().requires_grad_()
+        (g,) = torch.autograd.grad(ops.packed_causal_attention(*xs, p), leaf, do)
+        assert_within(g, want[name], tol[name], name, floor=6e-8)
+    # one tensor in all three places gets the sum
+    x = _rand((rows, 2, d), dtype, 210)
+    apart, _ = attention64(x, x, x, lens, do=do[:, :2])
+    leaf = x.requires_grad_()
+    (g,) = torch.autograd.grad(ops.packed_causal_attention(leaf, leaf, leaf, p), leaf, do[:, :2])
+    _, tol = attention64(x.detach(), x.detach(), x.detach(), lens, do=do[:, :2])
+    u = torch.finfo(dtype).eps / 2  # the two additions of the three gradients round twice
+    parts = [apart[n] for n in ("dq", "dk", "dv")]
+    assert_within(g, sum(parts), sum(tol[n] for n in ("dq", "dk", "dv")) + 3 * u * sum(y.abs() for y in parts), floor=6e-8)
+    # only one of the rotated tensors is used
+    cos, sin = ops.rotary_tables(150, d, 1e4, "cuda")
+    a, b = q.detach().requires_grad_(), k.detach().requires_grad_()
+    turned, other = ops.packed_rotary(a, b, cos, sin, d, p)
+    ga, gb = torch.autograd.grad(turned, (a, b), do, retain_graph=True)
+    back, _ = ops.packed_rotary(do, k, cos, -sin, d, p)
+    assert torch.equal(ga, back) and gb.abs().max() == 0
+    with torch.inference_mode():
+        assert torch.equal(ops.packed_causal_attention(q, k, v, p), ops.packed_causal_attention(q, k, v, p))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("hq,hk", [(4, 2), (3, 3)])
