@@ -529,10 +529,10 @@ _DISTILL_MAX_TOP = 1024
 
 def token_distillation_ref(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor, temperature: float) -> Tensor:
     dtype = torch.float64 if logits.dtype == torch.float64 else torch.float32
-    z = logits.to(dtype) / temperature
     t = teacher_logits.to(dtype) / temperature
     used = (teacher_ids >= 0) & (teacher_ids < logits.shape[1]) & (t != float("-inf"))
     some = used.any(1, keepdim=True)
+    z = (logits.to(dtype) / temperature).masked_fill(~some, 0.0)  # whatever stands in rows without a loss
     t = torch.where(used, t, float("-inf"))
     log_p = torch.log_softmax(torch.where(some, t, torch.zeros_like(t)), dim=1)
     p = log_p.exp()

@@ -191,6 +191,18 @@ def test_reference_distillation_masked_student():
     assert torch.isfinite(loss).all() and torch.isfinite(g).all() and g[0, 1] == 0
 
 
+@pytest.mark.parametrize("value", [math.nan, -math.inf, math.inf])
+def test_reference_distillation_rows_without_entries(value):
+    """Such a row gives 0 and a zero gradient, whatever its logits are."""
+    z = torch.randn(3, 7)
+    z[1] = value
+    z.requires_grad_()
+    ids, t = torch.tensor([[1, 2], [-1, 7], [0, 6]]), torch.randn(3, 2)
+    loss = ops.token_distillation(z, ids, t)
+    (g,) = torch.autograd.grad(loss.sum(), z)
+    assert loss[1] == 0 and (g[1] == 0).all() and torch.isfinite(loss).all() and torch.isfinite(g).all()
+
+
 def test_distillation_refusals():
     z, ids, t = torch.randn(4, 9), torch.zeros(4, 2, dtype=torch.int64), torch.randn(4, 2)
     call = ops.token_distillation
