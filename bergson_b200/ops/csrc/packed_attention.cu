@@ -149,6 +149,23 @@ cudaError_t tensor_fwd(const BgnPackedAttention& a, void* o, void* o_rest, float
   return cudaGetLastError();
 }
 
+// Launches a kernel of the backward pass whose blocks may come before the one before it has ended.  For kernels
+// with one block to an SM only: small blocks (fp32) that come early crowd on the SMs that were free first (242 against 177 us).
+template <typename... Args>
+cudaError_t launch_next(void (*kernel)(Args...), int blocks, int smem, cudaStream_t stream, Args... args) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(blocks));
+  cfg.blockDim = dim3(kBwdThreads);
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <int FMT, int DP>
 cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const void* o_rest, const float* bias2, const void* d_o, long do_tok,
                        long do_head, float* delta, float* do_max, void* dq, void* dk, void* dv, int* status,
@@ -205,13 +222,11 @@ cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const void* o
   if (e != cudaSuccess) return e;
   p.tiles = reinterpret_cast<const int4*>(a.query_tiles);
   p.units = tiles * a.heads;
-  kq<<<unsigned(p.units < sms ? p.units : sms), kBwdThreads, dq_smem_bytes<DP>(), stream>>>(mq, mg, mk, mv, p, status);
-  e = cudaGetLastError();
+  e = launch_next(kq, p.units < sms ? p.units : sms, dq_smem_bytes<DP>(), stream, mq, mg, mk, mv, p, status);
   if (e != cudaSuccess) return e;
   p.tiles = reinterpret_cast<const int4*>(a.key_tiles);
   p.units = tiles * a.kv_heads;
-  kk<<<unsigned(p.units < sms ? p.units : sms), kBwdThreads, dkv_smem_bytes<DP>(), stream>>>(mq, mg, mk, mv, p, status);
-  return cudaGetLastError();
+  return launch_next(kk, p.units < sms ? p.units : sms, dkv_smem_bytes<DP>(), stream, mq, mg, mk, mv, p, status);
 }
 
 bool sound(const BgnPackedAttention* a) {

@@ -78,6 +78,7 @@ template <int FMT, int LANES>
 __global__ void __launch_bounds__(32 * LANES) packed_delta_kernel(const __grid_constant__ PackedBwdArgs p) {
   using T = typename Type16<FMT>::T;
   __shared__ float tops[LANES];
+  next_kernel_may_come();
   const int head = blockIdx.x % p.heads, row0 = blockIdx.x / p.heads * 32;
   const int lane = threadIdx.x % LANES, row = row0 + threadIdx.x / LANES, f = 8 * lane;
   float sum = 0.f, top = 0.f;
@@ -206,6 +207,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = p.heads / p.kv_heads;
 
+  next_kernel_may_come();
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 9);  // the MMA warp's commit and the softmax warps, which read the row values
@@ -235,6 +237,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  wait_for_last_kernel();
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_dq = tmem, tmem_s = tmem + 128, tmem_dp = tmem + 256;  // dp: two places
 
@@ -626,6 +629,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  wait_for_last_kernel();
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_dv = tmem, tmem_dk = tmem + 128, tmem_s = tmem + 256, tmem_dp = tmem + 384;
 

@@ -172,6 +172,12 @@ __device__ __forceinline__ float warp_dot(const float (&x)[N], const float (&y)[
   return warp_sum(s);
 }
 
+// The kernels of a backward pass follow one another closely: each lets the next one's blocks come as soon as there is
+// room on an SM, and they wait for the end of the kernel before them when they have set up what they need.
+// 8187 tokens in facts, 12 heads of 64: 68 us instead of 73; 1024 tokens, 32 over 8 heads of 128: 87 instead of 92.
+__device__ __forceinline__ void next_kernel_may_come() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Gives up after a wait that ran out: long enough for every copy in flight to land.
 __device__ __forceinline__ void drain_copies() {
   const long long start = clock64();
