@@ -168,7 +168,7 @@ cudaError_t launch_next(void (*kernel)(Args...), int blocks, int smem, cudaStrea
 
 template <int FMT, int DP>
 cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const void* o_rest, const float* bias2, const void* d_o, long do_tok,
-                       long do_head, float* delta, float* do_max, void* dq, void* dk, void* dv, int* status,
+                       long do_head, float* delta, float* do_sizes, void* dq, void* dk, void* dv, int* status,
                        cudaStream_t stream) {
   ensure_context_bound();
   CUtensorMap mq, mk, mv, mg;
@@ -203,7 +203,8 @@ cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const void* o
   p.do_head = do_head;
   p.bias2 = bias2;
   p.neg_delta = delta;
-  p.do_max = do_max;
+  p.row_do = do_sizes;
+  p.doc_do = do_sizes + long(a.heads) * a.pitch;
   p.dq = dq;
   p.dk = dk;
   p.dv = dv;
@@ -252,7 +253,7 @@ extern "C" int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, vo
 
 extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const void* o_rest,
                                         const float* bias2, const void* d_o,
-                                        long do_tok, long do_head, float* delta, float* do_max, void* dq, void* dk,
+                                        long do_tok, long do_head, float* delta, float* do_sizes, void* dq, void* dk,
                                         void* dv, int* status, cudaStream_t stream) {
   if (!sound(a)) return int(cudaErrorInvalidValue);
   const bool narrow = a->dim <= 64;
@@ -264,6 +265,6 @@ extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void*
   }
   auto run = a->type == 1 ? (narrow ? tensor_bwd<1, 64> : tensor_bwd<1, 128>)
                           : (narrow ? tensor_bwd<0, 64> : tensor_bwd<0, 128>);
-  if (o_rest == nullptr) return int(cudaErrorInvalidValue);
-  return int(run(*a, o, o_rest, bias2, d_o, do_tok, do_head, delta, do_max, dq, dk, dv, status, stream));
+  if (o_rest == nullptr || (a->type == 0 && do_sizes == nullptr)) return int(cudaErrorInvalidValue);
+  return int(run(*a, o, o_rest, bias2, d_o, do_tok, do_head, delta, do_sizes, dq, dk, dv, status, stream));
 }

@@ -9,8 +9,10 @@
 // a fp32 copy of dQ in memory.  Tiles are cut from the packed axis as in the forward pass.
 //
 // P and dS are rounded to the operands' type for the tensor core; everything else is fp32.  fp16 has
-// few small values, so there P carries a factor 2^10 and dS the power of two that brings the largest
-// |do| of the rows concerned to [1/2, 1): both are taken out of the fp32 sums at the end.
+// few small values, so there P carries a factor 2^10 and dS a power of two: for dQ the one that brings the largest
+// |do| of the row to [1/2, 1), for dK that of the rows of the key's own document from the key's 32 rows on.  Both are
+// taken out of the fp32 sums at the end.  A row, or a key, is a thread of the softmax warps, so each has a factor of
+// its own and no document sets the precision of another one.
 //
 // Rows whose results are not finite are put right after a block's last unit, as in the forward pass.
 #pragma once
@@ -33,7 +35,8 @@ struct PackedBwdArgs {
   long q_tok, q_head, k_tok, k_head, v_tok, v_head, do_tok, do_head;
   const float* bias2;
   float* neg_delta;
-  float* do_max;  // [heads, pitch / 32]: largest |do| of 32 rows (fp16)
+  float* row_do;  // fp16, [heads, pitch]: largest |do| of a row (0 if not finite)
+  float* doc_do;  // fp16, [heads, pitch]: the same of the 32 rows around it, as far as they are of its document
   void *dq, *dk, *dv;
 };
 
@@ -43,6 +46,20 @@ __device__ __forceinline__ float power_below_one(float top) {
   const int e = int((__float_as_uint(top) >> 23) & 0xff) - 126;  // top in [2^(e-1), 2^e)
   const int f = 127 - e;
   return __uint_as_float(uint32_t(f < 1 ? 1 : (f > 253 ? 253 : f)) << 23);
+}
+
+// Largest value of the lanes with the same `run`, which lie side by side.
+__device__ __forceinline__ float max_of_run(float x, int run) {
+  const int lane = threadIdx.x & 31;
+  float before = x, behind = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float b = __shfl_up_sync(0xffffffffu, before, o), f = __shfl_down_sync(0xffffffffu, behind, o);
+    const int rb = __shfl_up_sync(0xffffffffu, run, o), rf = __shfl_down_sync(0xffffffffu, run, o);
+    if (lane >= o && rb == run) before = fmaxf(before, b);
+    if (lane + o < 32 && rf == run) behind = fmaxf(behind, f);
+  }
+  return fmaxf(before, behind);
 }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -77,7 +94,7 @@ __device__ __forceinline__ float2 score_gradient(uint32_t p0, uint32_t p1, uint3
 template <int FMT, int LANES>
 __global__ void __launch_bounds__(32 * LANES) packed_delta_kernel(const __grid_constant__ PackedBwdArgs p) {
   using T = typename Type16<FMT>::T;
-  __shared__ float tops[LANES];
+  __shared__ float row_top[32];
   next_kernel_may_come();
   const int head = blockIdx.x % p.heads, row0 = blockIdx.x / p.heads * 32;
   const int lane = threadIdx.x % LANES, row = row0 + threadIdx.x / LANES, f = 8 * lane;
@@ -100,12 +117,15 @@ __global__ void __launch_bounds__(32 * LANES) packed_delta_kernel(const __grid_c
   const long at = long(head) * p.pitch + row;
   if (lane == 0) p.neg_delta[at] = sum;  // zero where there is no row
   if (FMT == 0) {
-    top = warp_max(top);
-    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) row_top[threadIdx.x / LANES] = top < INFINITY ? top : 0.f;
     __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < LANES; ++w) top = fmaxf(top, tops[w]);
-      p.do_max[at / 32] = top;
+    if (threadIdx.x < 32) {  // a row to a lane
+      const int own = row0 + threadIdx.x, doc = own < p.valid ? __ldg(p.first_key + own) : -1;
+      const long to = long(head) * p.pitch + own;
+      p.row_do[to] = row_top[threadIdx.x];
+      p.doc_do[to] = max_of_run(row_top[threadIdx.x], doc);
     }
   }
 }
@@ -390,7 +410,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (!ok) break;
         neg_delta = row_values[tile_row];
         bias2 = in ? row_values[kTile + tile_row] : -INFINITY;
-        if (FMT == 0) factor = power_below_one(p.do_max[(long(head) * p.pitch + warp_row0) / 32]);
+        if (FMT == 0) factor = power_below_one(p.row_do[long(head) * p.pitch + row]);
         __syncwarp();
         if (lane == 0) mbar_arrive(q_empty);
       }
@@ -797,15 +817,19 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const int end = in ? __ldg(p.end_query + key) : 0;
       const bool opens = in && __ldg(p.first_key + key) == key;  // its own row attends nothing else
       const int min_end = __reduce_min_sync(0xffffffffu, end), max_end = __reduce_max_sync(0xffffffffu, end);
-      // fp16: the largest |do| among the rows of all steps sets the factor of dS.
+      // fp16: the largest |do| of the document's rows sets the factor of dS.  Only the document of the warp's last
+      // key goes on behind these 32 rows, and every later group of 32 that it reaches begins with it.
       float factor = 1.f;
-      if (FMT == 0) {
-        float top = 0.f;
-        for (int i = lane; i < n * 4; i += 32) {
-          const int h = kv_head * group + i / (per_head * 4);
-          top = fmaxf(top, p.do_max[(long(h) * p.pitch + entry.x) / 32 + i % (per_head * 4)]);
+      if (FMT == 0 && n > 0) {
+        const int behind = warp_key0 + 32, last_end = __shfl_sync(0xffffffffu, end, 31);
+        float top = 0.f, rest = 0.f;
+        for (int h = kv_head * group; h < (kv_head + 1) * group; ++h) {
+          const float* doc_do = p.doc_do + long(h) * p.pitch;
+          top = fmaxf(top, doc_do[key]);
+          for (int r32 = behind + 32 * lane; r32 < last_end; r32 += 1024) rest = fmaxf(rest, doc_do[r32]);
         }
-        factor = power_below_one(warp_max(top));
+        rest = warp_max(rest);
+        factor = power_below_one(end > behind ? fmaxf(top, rest) : top);
       }
       const float ds_factor = FMT == 0 ? factor * (1.f / 1024.f) : 1.f;
       const float2 f2 = make_float2(ds_factor, ds_factor);
