@@ -136,13 +136,13 @@ std::vector<at::Tensor> packed_attention_bwd(at::Tensor d_o, at::Tensor q, at::T
   d_o = readable(d_o);
   const auto a = packed_args(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale);
   auto delta = at::empty_like(bias2);
-  auto do_sizes = at::empty({a.type == 0 ? 2 * bias2.numel() : 0}, bias2.options());
+  auto ds_bounds = at::empty({a.type == 0 ? (3 * q.size(1) + k.size(1)) * a.pitch : 0}, bias2.options());
   auto dq = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
   auto dk = at::empty({k.size(0), k.size(1), k.size(2)}, k.options());
   auto dv = at::empty_like(dk);
   const auto [tok, head] = strides_of(d_o);
   ran(bgn_packed_attention_bwd(&a, o.data_ptr(), rest.has_value() ? rest->data_ptr() : nullptr, bias2.data_ptr<float>(), d_o.data_ptr(), tok, head,
-                               delta.data_ptr<float>(), a.type == 0 ? do_sizes.data_ptr<float>() : nullptr, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                               delta.data_ptr<float>(), a.type == 0 ? ds_bounds.data_ptr<float>() : nullptr, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                bgn_status_word(q), current()),
       "packed_attention_bwd");
   return {dq, dk, dv};

@@ -34,9 +34,9 @@ typedef struct {
 int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, void* o_rest, float* bias2, int* status, cudaStream_t stream);
 
 // Gradients of the operands (contiguous) from the output's gradient d_o [rows, heads, dim] (strides in
-// elements), the forward's o, o_rest and bias2.  Scratch: delta [heads, pitch]; for fp16 do_sizes [2, heads, pitch].
+// elements), the forward's o, o_rest and bias2.  Scratch: delta [heads, pitch]; for fp16 ds_bounds [3 heads + kv_heads, pitch].
 int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const void* o_rest, const float* bias2,
-                             const void* d_o, long do_tok, long do_head, float* delta, float* do_sizes, void* dq, void* dk, void* dv, int* status,
+                             const void* d_o, long do_tok, long do_head, float* delta, float* ds_bounds, void* dq, void* dk, void* dv, int* status,
                              cudaStream_t stream);
 
 typedef struct {

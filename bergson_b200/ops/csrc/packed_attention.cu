@@ -168,7 +168,7 @@ cudaError_t launch_next(void (*kernel)(Args...), int blocks, int smem, cudaStrea
 
 template <int FMT, int DP>
 cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const void* o_rest, const float* bias2, const void* d_o, long do_tok,
-                       long do_head, float* delta, float* do_sizes, void* dq, void* dk, void* dv, int* status,
+                       long do_head, float* delta, float* ds_bounds, void* dq, void* dk, void* dv, int* status,
                        cudaStream_t stream) {
   ensure_context_bound();
   CUtensorMap mq, mk, mv, mg;
@@ -203,8 +203,13 @@ cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const void* o
   p.do_head = do_head;
   p.bias2 = bias2;
   p.neg_delta = delta;
-  p.row_do = do_sizes;
-  p.doc_do = do_sizes + long(a.heads) * a.pitch;
+  if (FMT == 0) {
+    const long heads = long(a.heads) * a.pitch;
+    p.row_do = ds_bounds;
+    p.doc_do = ds_bounds + heads;
+    p.doc_delta = ds_bounds + 2 * heads;
+    p.doc_v = ds_bounds + 3 * heads;
+  }
   p.dq = dq;
   p.dk = dk;
   p.dv = dv;
@@ -218,7 +223,7 @@ cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const void* o
   if (e != cudaSuccess) return e;
   const int tiles = (a.rows + kTile - 1) / kTile;
   constexpr int kLanes = DP / 8;
-  packed_delta_kernel<FMT, kLanes><<<unsigned(4 * tiles) * unsigned(a.heads), 32 * kLanes, 0, stream>>>(p);
+  packed_delta_kernel<FMT, kLanes><<<unsigned(4 * tiles) * unsigned(a.heads), delta_threads<FMT, kLanes>(), 0, stream>>>(p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   p.tiles = reinterpret_cast<const int4*>(a.query_tiles);
@@ -253,7 +258,7 @@ extern "C" int bgn_packed_attention_fwd(const BgnPackedAttention* a, void* o, vo
 
 extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void* o, const void* o_rest,
                                         const float* bias2, const void* d_o,
-                                        long do_tok, long do_head, float* delta, float* do_sizes, void* dq, void* dk,
+                                        long do_tok, long do_head, float* delta, float* ds_bounds, void* dq, void* dk,
                                         void* dv, int* status, cudaStream_t stream) {
   if (!sound(a)) return int(cudaErrorInvalidValue);
   const bool narrow = a->dim <= 64;
@@ -265,6 +270,6 @@ extern "C" int bgn_packed_attention_bwd(const BgnPackedAttention* a, const void*
   }
   auto run = a->type == 1 ? (narrow ? tensor_bwd<1, 64> : tensor_bwd<1, 128>)
                           : (narrow ? tensor_bwd<0, 64> : tensor_bwd<0, 128>);
-  if (o_rest == nullptr || (a->type == 0 && do_sizes == nullptr)) return int(cudaErrorInvalidValue);
-  return int(run(*a, o, o_rest, bias2, d_o, do_tok, do_head, delta, do_sizes, dq, dk, dv, status, stream));
+  if (o_rest == nullptr || (a->type == 0 && ds_bounds == nullptr)) return int(cudaErrorInvalidValue);
+  return int(run(*a, o, o_rest, bias2, d_o, do_tok, do_head, delta, ds_bounds, dq, dk, dv, status, stream));
 }

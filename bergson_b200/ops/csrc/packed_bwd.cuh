@@ -9,10 +9,12 @@
 // a fp32 copy of dQ in memory.  Tiles are cut from the packed axis as in the forward pass.
 //
 // P and dS are rounded to the operands' type for the tensor core; everything else is fp32.  fp16 has
-// few small values, so there P carries a factor 2^10 and dS a power of two: for dQ the one that brings the largest
-// |do| of the row to [1/2, 1), for dK that of the rows of the key's own document from the key's 32 rows on.  Both are
-// taken out of the fp32 sums at the end.  A row, or a key, is a thread of the softmax warps, so each has a factor of
-// its own and no document sets the precision of another one.
+// few small values and ends at 65504, so there P carries a factor 2^10 and dS the power of two that brings B, a bound of
+// |do.v - delta|, to [2^14, 2^15): dS cannot overflow and uses what the type has below that.
+//   dQ, row t:  B = sum|do_t| max|v_j| + |delta_t|,  over the row's own keys (to the end of its 32 rows)
+//   dK, key j:  B = max sum|do_t| max|v| + max|delta_t|,  over the document's rows t from the key's 32 rows on, v of those 32
+// Both factors are taken out of the fp32 sums at the end.  A row, or a key, is a thread of the softmax warps, so each
+// has its own factor and no document sets the precision of another one.
 //
 // Rows whose results are not finite are put right after a block's last unit, as in the forward pass.
 #pragma once
@@ -35,32 +37,50 @@ struct PackedBwdArgs {
   long q_tok, q_head, k_tok, k_head, v_tok, v_head, do_tok, do_head;
   const float* bias2;
   float* neg_delta;
-  float* row_do;  // fp16, [heads, pitch]: largest |do| of a row (0 if not finite)
-  float* doc_do;  // fp16, [heads, pitch]: the same of the 32 rows around it, as far as they are of its document
+  // fp16, what bounds dS; what is not finite counts as zero.  "doc": the largest value of the row's group of 32 rows
+  // (from a multiple of 32 on), as far as they are of its document.
+  float* row_do;     // [heads, pitch]: sum |do|
+  float* doc_do;     // [heads, pitch]: the same, doc
+  float* doc_delta;  // [heads, pitch]: |delta|, doc
+  float* doc_v;      // [kv_heads, pitch]: |v|, doc
   void *dq, *dk, *dv;
 };
 
-// The power of two that brings `top` to [1/2, 1); 1 where there is nothing to scale.
-__device__ __forceinline__ float power_below_one(float top) {
-  if (!(top > 0.f) || !(top < INFINITY)) return 1.f;
-  const int e = int((__float_as_uint(top) >> 23) & 0xff) - 126;  // top in [2^(e-1), 2^e)
-  const int f = 127 - e;
-  return __uint_as_float(uint32_t(f < 1 ? 1 : (f > 253 ? 253 : f)) << 23);
+// The power of two that brings `bound` to [2^14, 2^15); 1 where there is nothing to scale.
+__device__ __forceinline__ float power_for(float bound) {
+  if (!(bound > 0.f) || !(bound < INFINITY)) return 1.f;
+  const int f = 268 - int(__float_as_uint(bound) >> 23);  // biased: bound in [2^(e-127), 2^(e-126)), factor 2^(141-e)
+  return __uint_as_float(uint32_t(f < 253 ? f : 253) << 23);
 }
 
-// Largest value of the lanes with the same `run`, which lie side by side.
-__device__ __forceinline__ float max_of_run(float x, int run) {
+// Each value becomes the largest of the lanes with the same `run`, which lie side by side.
+template <int N>
+__device__ __forceinline__ void max_of_run(float (&x)[N], int run) {
+  if (__all_sync(0xffffffffu, run == __shfl_sync(0xffffffffu, run, 0))) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) x[n] = warp_max(x[n]);
+    return;
+  }
   const int lane = threadIdx.x & 31;
-  float before = x, behind = x;
+  float behind[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) behind[n] = x[n];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const float b = __shfl_up_sync(0xffffffffu, before, o), f = __shfl_down_sync(0xffffffffu, behind, o);
-    const int rb = __shfl_up_sync(0xffffffffu, run, o), rf = __shfl_down_sync(0xffffffffu, run, o);
-    if (lane >= o && rb == run) before = fmaxf(before, b);
-    if (lane + o < 32 && rf == run) behind = fmaxf(behind, f);
+    const bool up = __shfl_up_sync(0xffffffffu, run, o) == run && lane >= o;
+    const bool down = __shfl_down_sync(0xffffffffu, run, o) == run && lane + o < 32;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const float b = __shfl_up_sync(0xffffffffu, x[n], o), f = __shfl_down_sync(0xffffffffu, behind[n], o);
+      if (up) x[n] = fmaxf(x[n], b);
+      if (down) behind[n] = fmaxf(behind[n], f);
+    }
   }
-  return fmaxf(before, behind);
+#pragma unroll
+  for (int n = 0; n < N; ++n) x[n] = fmaxf(x[n], behind[n]);
 }
+
+__device__ __forceinline__ float finite_or_zero(float x) { return fabsf(x) < INFINITY ? x : 0.f; }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -89,43 +109,79 @@ __device__ __forceinline__ float2 score_gradient(uint32_t p0, uint32_t p1, uint3
 //
 // delta = do . o, with what rounding took from o: dS is a difference against delta, and for rows with few
 // keys that rounding would be its largest error.  A block has 32 rows of a head, LANES lanes to a row.
-// HBM bounds it: o, its rest and do are read once (16384 tokens of 32 heads of 128: 61 us, 6600 GB/s).
+// HBM bounds it: o, its rest and do are read once (16384 tokens of 32 heads of 128: 61 us, 6600 GB/s).  For fp16 it also
+// reads v, for what bounds dS.
+
+// fp16: four rows to a thread and so small blocks, of which others read while one joins its rows' bounds (76 us at the
+// same size over 8 key heads, 90 with a row to a thread); bf16 has nothing to join.
+template <int FMT, int LANES>
+constexpr int delta_threads() {
+  return 32 * LANES / (FMT == 0 ? 4 : 1);
+}
 
 template <int FMT, int LANES>
-__global__ void __launch_bounds__(32 * LANES) packed_delta_kernel(const __grid_constant__ PackedBwdArgs p) {
+__global__ void __launch_bounds__(delta_threads<FMT, LANES>()) packed_delta_kernel(const __grid_constant__ PackedBwdArgs p) {
   using T = typename Type16<FMT>::T;
-  __shared__ float row_top[32];
+  constexpr int kStep = delta_threads<FMT, LANES>() / LANES, kRows = 32 / kStep;
+  __shared__ float of_row[3][32];  // sum |do|, |delta|, largest |v|
   next_kernel_may_come();
-  const int head = blockIdx.x % p.heads, row0 = blockIdx.x / p.heads * 32;
-  const int lane = threadIdx.x % LANES, row = row0 + threadIdx.x / LANES, f = 8 * lane;
-  float sum = 0.f, top = 0.f;
-  if (row < p.valid && f < p.dim) {
-    const long from = (long(row) * p.heads + head) * p.dim + f;
-    union { uint4 u; T h[8]; } o, rest, g;
-    o.u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.o) + from));
-    rest.u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.o_rest) + from));
-    g.u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.d_o) + long(row) * p.do_tok + long(head) * p.do_head + f));
+  const int head = blockIdx.x % p.heads, row0 = blockIdx.x / p.heads * 32, group = p.heads / p.kv_heads;
+  const int lane = threadIdx.x % LANES, row1 = threadIdx.x / LANES, f = 8 * lane;
+  const bool with_v = FMT == 0 && head % group == 0;  // one head of a group looks at v
+  union Packet { uint4 u; T h[8]; };
+  Packet o[kRows], rest[kRows], g[kRows], v[kRows];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = to_float<T>(g.h[e]);
-      sum = fmaf(-to_float<T>(o.h[e]) - to_float<T>(rest.h[e]), x, sum);
-      top = fmaxf(top, fabsf(x));
+  for (int n = 0; n < kRows; ++n) {
+    const int row = row0 + row1 + n * kStep;
+    o[n].u = rest[n].u = g[n].u = v[n].u = make_uint4(0, 0, 0, 0);
+    if (row < p.valid && f < p.dim) {
+      const long from = (long(row) * p.heads + head) * p.dim + f;
+      o[n].u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.o) + from));
+      rest[n].u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.o_rest) + from));
+      g[n].u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.d_o) + long(row) * p.do_tok + long(head) * p.do_head + f));
+      if (with_v)
+        v[n].u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.v) + long(row) * p.v_tok + long(head / group) * p.v_head + f));
     }
   }
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const long at = long(head) * p.pitch + row;
-  if (lane == 0) p.neg_delta[at] = sum;  // zero where there is no row
-  if (FMT == 0) {
+  for (int n = 0; n < kRows; ++n) {
+    float sum = 0.f, size = 0.f, top_v = 0.f;
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) row_top[threadIdx.x / LANES] = top < INFINITY ? top : 0.f;
+    for (int e = 0; e < 8; ++e) {
+      const float x = to_float<T>(g[n].h[e]);
+      sum = fmaf(-to_float<T>(o[n].h[e]) - to_float<T>(rest[n].h[e]), x, sum);
+      if (FMT == 0) size += fabsf(x);
+    }
+    if (with_v)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top_v = fmaxf(top_v, fabsf(finite_or_zero(to_float<T>(v[n].h[e]))));
+#pragma unroll
+    for (int x = LANES / 2; x > 0; x >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      if (FMT == 0) size += __shfl_xor_sync(0xffffffffu, size, x);
+      if (with_v) top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, x));
+    }
+    const int r = row1 + n * kStep;
+    if (lane == 0) {
+      p.neg_delta[long(head) * p.pitch + row0 + r] = sum;  // zero where there is no row
+      if (FMT == 0) {
+        of_row[0][r] = finite_or_zero(size);
+        of_row[1][r] = fabsf(finite_or_zero(sum));
+        of_row[2][r] = top_v;
+      }
+    }
+  }
+  if (FMT == 0) {
     __syncthreads();
     if (threadIdx.x < 32) {  // a row to a lane
-      const int own = row0 + threadIdx.x, doc = own < p.valid ? __ldg(p.first_key + own) : -1;
+      const int own = row0 + threadIdx.x;
       const long to = long(head) * p.pitch + own;
-      p.row_do[to] = row_top[threadIdx.x];
-      p.doc_do[to] = max_of_run(row_top[threadIdx.x], doc);
+      float x[3] = {of_row[0][threadIdx.x], of_row[1][threadIdx.x], of_row[2][threadIdx.x]};
+      p.row_do[to] = x[0];
+      max_of_run(x, own < p.valid ? __ldg(p.first_key + own) : -1);
+      p.doc_do[to] = x[0];
+      p.doc_delta[to] = x[1];
+      if (with_v) p.doc_v[long(head / group) * p.pitch + own] = x[2];
     }
   }
 }
@@ -394,6 +450,19 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const float c = p.scale * kPackedLog2e;
     bool ok = true, bad = false;
     int j = 0, count = 0;
+    // fp16: what bounds dS of a unit.  Only the document of the warp's first row began before its 32 rows, and the groups
+    // of 32 that it comes through end with it.
+    float row_do = 0.f, own_v = 0.f, before_v = 0.f;
+    const auto fetch_bounds = [&](const int4& e, int u) {
+      if (FMT != 0 || u < 0 || steps_of(e) == 0) return;
+      const int row32 = e.x + quad * 32, begin = row32 < p.valid ? __ldg(p.first_key + row32) : row32;
+      const float* doc_v = p.doc_v + long(u % p.heads / group) * p.pitch;
+      row_do = p.row_do[long(u % p.heads) * p.pitch + row32 + lane];
+      own_v = doc_v[row32 + lane];
+      before_v = 0.f;
+      for (int r32 = (begin & ~31) + 32 * lane; r32 < row32; r32 += 1024) before_v = fmaxf(before_v, doc_v[r32 + 31]);
+    };
+    fetch_bounds(entry, unit);
     for (int r = 0; unit >= 0 && ok; ++r) {
       const int after = nth_unit(r + 1, p.units);
       const int4 next = after >= 0 ? __ldg(p.tiles + after / p.heads) : entry;
@@ -410,7 +479,10 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (!ok) break;
         neg_delta = row_values[tile_row];
         bias2 = in ? row_values[kTile + tile_row] : -INFINITY;
-        if (FMT == 0) factor = power_below_one(p.row_do[long(head) * p.pitch + row]);
+        if (FMT == 0) {
+          const float before = warp_max(before_v);
+          factor = power_for(row_do * (first < warp_row0 ? fmaxf(own_v, before) : own_v) + fabsf(neg_delta));
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(q_empty);
       }
@@ -479,6 +551,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const bool some = in && first <= row;
       unit = after;
       entry = next;
+      fetch_bounds(entry, unit);  // under what is left of this unit
       T* dst = static_cast<T*>(p.dq) + at;
       if (n > 0) {
         ok = warp_wait(dq_full, count & 1);
@@ -817,19 +890,34 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const int end = in ? __ldg(p.end_query + key) : 0;
       const bool opens = in && __ldg(p.first_key + key) == key;  // its own row attends nothing else
       const int min_end = __reduce_min_sync(0xffffffffu, end), max_end = __reduce_max_sync(0xffffffffu, end);
-      // fp16: the largest |do| of the document's rows sets the factor of dS.  Only the document of the warp's last
-      // key goes on behind these 32 rows, and every later group of 32 that it reaches begins with it.
+      // fp16: what bounds dS.  Only the document of the warp's last key goes on behind its 32 rows, and every later
+      // group of 32 that it reaches begins with it.  (Asked for under the end of the unit before, as in dQ: 37 instead
+      // of 41 us for 211 facts of 12 heads of 64, but 56 instead of 51 for 16 over 2 heads.)
       float factor = 1.f;
       if (FMT == 0 && n > 0) {
-        const int behind = warp_key0 + 32, last_end = __shfl_sync(0xffffffffu, end, 31);
-        float top = 0.f, rest = 0.f;
-        for (int h = kv_head * group; h < (kv_head + 1) * group; ++h) {
-          const float* doc_do = p.doc_do + long(h) * p.pitch;
-          top = fmaxf(top, doc_do[key]);
-          for (int r32 = behind + 32 * lane; r32 < last_end; r32 += 1024) rest = fmaxf(rest, doc_do[r32]);
+        const int behind = warp_key0 + 32, later = max(__shfl_sync(0xffffffffu, end, 31) - behind + 31, 0) >> 5;
+        const long head0 = long(kv_head) * group * p.pitch;
+        float size = 0.f, delta = 0.f, later_size = 0.f, later_delta = 0.f;
+#pragma unroll 4
+        for (int h = 0; h < group; ++h) {
+          size = fmaxf(size, p.doc_do[head0 + long(h) * p.pitch + key]);
+          delta = fmaxf(delta, p.doc_delta[head0 + long(h) * p.pitch + key]);
         }
-        rest = warp_max(rest);
-        factor = power_below_one(end > behind ? fmaxf(top, rest) : top);
+#pragma unroll 4
+        for (int x = lane; x < later * group; x += 32) {
+          const long from = head0 + long(x / later) * p.pitch + behind + 32 * (x % later);
+          later_size = fmaxf(later_size, p.doc_do[from]);
+          later_delta = fmaxf(later_delta, p.doc_delta[from]);
+        }
+        if (later > 0) {
+          later_size = warp_max(later_size);
+          later_delta = warp_max(later_delta);
+          if (end > behind) {
+            size = fmaxf(size, later_size);
+            delta = fmaxf(delta, later_delta);
+          }
+        }
+        factor = power_for(size * p.doc_v[long(kv_head) * p.pitch + key] + delta);
       }
       const float ds_factor = FMT == 0 ? factor * (1.f / 1024.f) : 1.f;
       const float2 f2 = make_float2(ds_factor, ds_factor);

@@ -7,6 +7,7 @@ import torch
 
 from bergson_b200 import ops
 
+from .packed_bounds import attention_bounds64
 from .packed_reference import assert_within, attention64
 from .test_packed_gpu import DTYPES, _attend, _rand, native  # noqa: F401
 
@@ -49,3 +50,36 @@ def test_a_poisoned_document_leaves_small_fp16_gradients(native, poison, small):
     do = (do.float() * 2.0**-16).half()
     do[300:390] = poison
     _check_documents(_attend(native, q, k, v, lens, do=do), q, k, v, lens, do, which=(0, 2))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens", [[500], [130, 600, 11]])
+def test_large_values_along_the_gradient_do_not_overflow(native, lens, dtype):
+    """v of 3000 along do: score gradients above fp16's largest value, results far below it."""
+    d, scale = 128, 1.0 / 512
+    rows = sum(lens)
+    g = torch.Generator(device="cuda").manual_seed(720)
+    q, k = (_rand((rows, 2, d), dtype, 721 + i, std=24.0) for i in range(2))
+    along = torch.randint(0, 2, (d,), generator=g, device="cuda") * 2.0 - 1
+    sign = torch.randint(0, 2, (rows, 2, 1), generator=g, device="cuda") * 2.0 - 1
+    v = (sign * along * 3000).to(dtype)
+    do = (along * 0.99).expand(rows, 2, d).to(dtype)
+    want, tol = attention_bounds64(q, k, v, lens, do, scale)  # the step of dS as it is for values of this size
+    P = torch.softmax((q[:lens[0], 0].double() @ k[:lens[0], 0].double().T * scale)
+                      .masked_fill(torch.ones(lens[0], lens[0], dtype=torch.bool, device="cuda").triu(1), -math.inf), 1)
+    dP = do[:lens[0], 0].double() @ v[:lens[0], 0].double().T
+    assert (P * (dP - (P * dP).sum(1, keepdim=True))).abs().max() > 65504
+    assert max(want[n].abs().max() for n in want) < 65504  # the largest fp16
+    got = _attend(native, q, k, v, lens, 0, scale, do)
+    for name in got:
+        assert_within(got[name], want[name], tol[name], name, floor=6e-8)
+
+
+def test_fp16_outliers_in_a_neighbours_values(native):
+    """Values of 60000, an infinity or a NaN in another document's v: this one's gradients keep their precision."""
+    lens = [200, 100, 230]
+    q, k, v, do = (_rand((530, 2, 64), torch.float16, 730 + i) for i in range(4))
+    do = (do.float() * 2.0**-10).half()
+    for x in (60000.0, float("inf"), float("nan")):
+        v[200:300] = x
+        _check_documents(_attend(native, q, k, v, lens, do=do), q, k, v, lens, do, which=(0, 2))
