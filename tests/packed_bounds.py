@@ -64,3 +64,11 @@ def attention_bounds64(q, k, v, lens, do, scale=None, exact_weights=False):
             out[name][own] = x
             tol[name][own] = ex + u * x.abs()
     return out, tol
+
+
+def far_values(dtype):
+    """Documents of few rows, scores of zero, values of some 100: o is far larger than the differences that make dS."""
+    g = torch.Generator().manual_seed(790)
+    lens = [2, 3, 5, 4, 6, 2, 7]
+    k, v, do = (torch.randn(sum(lens), 2, 64, generator=g) for _ in range(3))
+    return torch.zeros_like(k).to(dtype), k.to(dtype), (v + 100).to(dtype), do.to(dtype), lens

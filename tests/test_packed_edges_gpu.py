@@ -7,7 +7,7 @@ import torch
 
 from bergson_b200 import ops
 
-from .packed_bounds import attention_bounds64
+from .packed_bounds import attention_bounds64, far_values
 from .packed_reference import assert_within, attention64
 from .test_packed_gpu import DTYPES, _attend, _rand, native  # noqa: F401
 
@@ -83,3 +83,28 @@ def test_fp16_outliers_in_a_neighbours_values(native):
     for x in (60000.0, float("inf"), float("nan")):
         v[200:300] = x
         _check_documents(_attend(native, q, k, v, lens, do=do), q, k, v, lens, do, which=(0, 2))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,hq,hk,d", [([2, 3, 1, 5, 4, 2], 4, 2, 64), ([130, 3, 200], 2, 2, 128), ([33, 95, 31, 1, 64, 300], 6, 2, 40),
+                                          ([1100], 4, 1, 64)])
+def test_attention_within_the_documents_own_bounds(native, lens, hq, hk, d, dtype):
+    """With what rounding took from o kept for delta, and scales of dS from a document's own rows."""
+    q, k, v, do = (_rand((sum(lens), h, d), dtype, 740 + i) for i, h in enumerate((hq, hk, hk, hq)))
+    sizes = 2.0 ** torch.randint(-8, 5, (len(lens),), generator=torch.Generator().manual_seed(1))
+    do = (do.float() * sizes.repeat_interleave(torch.tensor(lens)).cuda()[:, None, None]).to(dtype)
+    got = _attend(native, q, k, v, lens, do=do)
+    want, tol = attention_bounds64(q, k, v, lens, do)
+    for name in got:
+        assert_within(got[name], want[name], tol[name], name, floor=6e-8)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_delta_is_taken_from_more_than_the_rounded_output(native, dtype):
+    """Scores of zero and values far from zero: rounding o alone would be off by many times the bound."""
+    q, k, v, do, lens = far_values(dtype)
+    q, k, v, do = (x.cuda() for x in (q, k, v, do))
+    got = _attend(native, q, k, v, lens, do=do)
+    want, tol = attention_bounds64(q, k, v, lens, do, exact_weights=True)
+    for name in got:
+        assert_within(got[name], want[name], tol[name], name, floor=6e-8)
