@@ -82,12 +82,12 @@ __device__ __forceinline__ void store_scores(float* p, const float (&s)[4], int 
   *reinterpret_cast<float4*>(p + row * kSimplePitch + 4 * tx) = make_float4(s[0], s[1], s[2], s[3]);
 }
 
-// out[i][c] += sum_j p[4 ty + i][j] x[tx + 16 c][j].  `careful`: a zero of p takes no part at all, for what
-// stands in a masked row may be infinite or NaN.  That is slow, and only done over again when a result has
-// turned out not to be finite.
-template <int DP, int R>
+// out[i][c] += sum_j p[4 ty + i][j] x[tx + 16 c][j].  `careful`: only the columns inside(i) = [x, y] of a row take part,
+// for what stands in a masked one may be infinite or NaN (a zero of p inside makes NaN of that, as it must).  That is
+// slow, and only done over again when a result has turned out not to be finite.
+template <int DP, int R, typename Range>
 __device__ __forceinline__ void simple_product(float (&out)[R][DP / 16], const float* p, const float* x, int ty, int tx,
-                                               bool careful) {
+                                               bool careful, Range inside) {
   if (!careful) {
 #pragma unroll 4
     for (int j = 0; j < kSimpleTile; j += 4) {
@@ -112,7 +112,7 @@ __device__ __forceinline__ void simple_product(float (&out)[R][DP / 16], const f
         const float b = x[(tx + 16 * c) * kSimplePitch + j];
 #pragma unroll
         for (int i = 0; i < R; ++i)
-          if (a[i] != 0.f) out[i][c] = fmaf(a[i], b, out[i][c]);
+          if (j >= inside(i).x && j <= inside(i).y) out[i][c] = fmaf(a[i], b, out[i][c]);
       }
     }
   }
@@ -207,7 +207,7 @@ again:
       for (int d = 0; d < DP / 16; ++d) out[i][d] *= old;
     }
     __syncthreads();
-    simple_product<DP, R>(out, ps, vs, ty, tx, careful);
+    simple_product<DP, R>(out, ps, vs, ty, tx, careful, [&](int i) { return make_int2(first[i] - k0, q0 + R * ty + i - k0); });
   }
   if (!careful && __syncthreads_or(some_not_finite(out))) {
     careful = true;
@@ -292,7 +292,10 @@ again:
       store_scores(ds, s[i], R * ty + i, tx);
     }
     __syncthreads();
-    simple_product<DP, R>(out, ds, ks, ty, tx, careful);
+    simple_product<DP, R>(out, ds, ks, ty, tx, careful, [&](int i) {
+      const int row = q0 + R * ty + i;
+      return make_int2(first[i] < row ? first[i] - k0 : 0x7fffffff, row - k0);
+    });
   }
   if (!careful && __syncthreads_or(some_not_finite(out))) {
     careful = true;
@@ -371,12 +374,15 @@ again:
 #pragma unroll
       for (int i = 0; i < R; ++i) store_scores(ps, s[i], R * ty + i, tx);
       __syncthreads();
-      simple_product<DP, R>(out_v, ps, gs, ty, tx, careful);
+      simple_product<DP, R>(out_v, ps, gs, ty, tx, careful,
+                            [&](int i) { return make_int2(k0 + R * ty + i - q0, end[i] - 1 - q0); });
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < R; ++i) store_scores(ps, dp[i], R * ty + i, tx);
       __syncthreads();
-      simple_product<DP, R>(out_k, ps, qs, ty, tx, careful);
+      simple_product<DP, R>(out_k, ps, qs, ty, tx, careful, [&](int i) {
+        return make_int2(max(k0 + R * ty + i, own_first[i] + 1) - q0, end[i] - 1 - q0);
+      });
     }
   }
   if (!careful && __syncthreads_or(some_not_finite(out_k) || some_not_finite(out_v))) {

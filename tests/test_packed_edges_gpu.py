@@ -108,3 +108,52 @@ def test_delta_is_taken_from_more_than_the_rounded_output(native, dtype):
     want, tol = attention_bounds64(q, k, v, lens, do, exact_weights=True)
     for name in got:
         assert_within(got[name], want[name], tol[name], name, floor=6e-8)
+
+
+def _sharp(dtype, n=300, at=150, d=64, begin=0):
+    """Scores that rise by far from key to key: the weight of key `at` is zero in every later row but the next few."""
+    q, k, v, do = (_rand((n, 2, d), dtype, 750 + i) for i in range(4))
+    q[..., 0] = 16.0
+    k[..., 0] = torch.linspace(0, 3000, n, device="cuda")[:, None].to(dtype)
+    return q, k, v, do
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_attention_zero_weights_hide_nothing(native, value, dtype):
+    """An attended key's weight may underflow to zero; what is not finite reaches the row all the same, as in the
+    definition, where zero times it is NaN."""
+    n, at, lens = 300, 150, [300]
+    q, k, v, do = _sharp(dtype, n, at)
+    P = torch.softmax((q[..., 0, :].double() @ k[..., 0, :].double().T / 8).masked_fill(
+        torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1), -math.inf), 1)
+    assert P[at + 20:, at].max() < 1e-60  # zero in 32 bits
+    bad = v.clone()
+    bad[at, 1, 5] = value
+    got = _attend(native, q, k, bad, lens)["o"]
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[at:, 1, 5] = True
+    assert torch.equal(~torch.isfinite(got), hit) and torch.isnan(got[at + 20:, 1, 5]).all()
+    bad = do.clone()
+    bad[at, 1, 5] = value
+    got = _attend(native, q, k, v, lens, do=bad)
+    hit = torch.zeros_like(got["dv"], dtype=torch.bool)
+    hit[:at + 1, 1, 5] = True
+    assert torch.equal(~torch.isfinite(got["dv"]), hit) and torch.isnan(got["dv"][:at - 20, 1, 5]).all()
+    hit[:at + 1, 1] = True
+    assert torch.equal(~torch.isfinite(got["dk"]), hit) and torch.isfinite(got["dq"][:at]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_keys_at_minus_infinity(native, dtype):
+    """A key of -inf along a positive query has no weight: o is finite, dq = 0 * -inf is NaN in that feature."""
+    n, at = 300, 150
+    q, k, v, do = (_rand((n, 2, 64), dtype, 760 + i) for i in range(4))
+    q[..., 3] = 1.0
+    k[at, 1, 3] = float("-inf")
+    got = _attend(native, q, k, v, [n], do=do)
+    assert torch.isfinite(got["o"][at + 1:]).all()
+    hit = torch.zeros_like(got["dq"], dtype=torch.bool)
+    hit[at + 1:, 1, 3] = True
+    assert torch.equal(torch.isnan(got["dq"][at + 1:]), hit[at + 1:])
+    assert torch.isfinite(got["dq"][:at]).all() and torch.isfinite(got["dv"]).all()
