@@ -100,30 +100,38 @@ struct DistillStream {
   }
 };
 
-// A packet's values in fp32, and the largest of them (NaN does not count).
+// The larger value; NaN if there is one.
+__device__ __forceinline__ float max_or_nan(float x, float y) {
+  float z;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+
+// A packet's values in fp32, and the largest of them; NaN if one is: a packet of nothing but -inf adds nothing to the
+// sum and is left out, one with a NaN among them must not be.
 template <typename T>
 __device__ __forceinline__ float unpack_max(const DistillPacket<T>& p, float2 (&f)[DistillPacket<T>::N / 2]);
 template <>
 __device__ __forceinline__ float unpack_max<float>(const DistillPacket<float>& p, float2 (&f)[2]) {
   f[0] = make_float2(p.v[0], p.v[1]);
   f[1] = make_float2(p.v[2], p.v[3]);
-  return fmaxf(fmaxf(p.v[0], p.v[1]), fmaxf(p.v[2], p.v[3]));
+  return max_or_nan(max_or_nan(p.v[0], p.v[1]), max_or_nan(p.v[2], p.v[3]));
 }
 template <>
 __device__ __forceinline__ float unpack_max<__nv_bfloat16>(const DistillPacket<__nv_bfloat16>& p, float2 (&f)[4]) {
   const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(p.v);
 #pragma unroll
   for (int e = 0; e < 4; ++e) f[e] = __bfloat1622float2(h[e]);
-  const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-  return fmaxf(__low2float(m), __high2float(m));
+  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+  return max_or_nan(__low2float(m), __high2float(m));
 }
 template <>
 __device__ __forceinline__ float unpack_max<__half>(const DistillPacket<__half>& p, float2 (&f)[4]) {
   const __half2* h = reinterpret_cast<const __half2*>(p.v);
 #pragma unroll
   for (int e = 0; e < 4; ++e) f[e] = __half22float2(h[e]);
-  const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-  return fmaxf(__low2float(m), __high2float(m));
+  const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+  return max_or_nan(__low2float(m), __high2float(m));
 }
 
 // A cluster of blocks shares one row: block r of it sweeps the r-th part of the columns, the first

@@ -157,3 +157,21 @@ def test_attention_keys_at_minus_infinity(native, dtype):
     hit[at + 1:, 1, 3] = True
     assert torch.equal(torch.isnan(got["dq"][at + 1:]), hit[at + 1:])
     assert torch.isfinite(got["dq"][:at]).all() and torch.isfinite(got["dv"]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,V", [(3, 777), (700, 1003), (2, 50257)])
+def test_distillation_nan_among_masked_logits(native, T, V, dtype):
+    """A NaN whose neighbours are all -inf, in every place of a packet: the row's loss and gradient are NaN."""
+    ids, t = torch.randint(400, 600, (T, 4), device="cuda"), _rand((T, 4), torch.float32, 771)
+    for at in (*range(96, 112), V - 1, 0):
+        z = _rand((T, V), dtype, 770)
+        z[1, :300] = -math.inf
+        z[1, 700:] = -math.inf
+        z[1, at] = float("nan")
+        leaf = z.requires_grad_()
+        loss = ops.token_distillation(leaf, ids, t)
+        (g,) = torch.autograd.grad(loss.sum(), leaf)
+        others = [0] + list(range(2, T))
+        assert torch.isnan(loss[1]) and torch.isnan(g[1]).all(), at
+        assert torch.isfinite(loss[others]).all() and torch.isfinite(g[others]).all()
