@@ -537,8 +537,8 @@ def token_distillation_ref(logits: Tensor, teacher_ids: Tensor, teacher_logits: 
     log_p = torch.log_softmax(torch.where(some, t, torch.zeros_like(t)), dim=1)
     p = log_p.exp()
     log_q = torch.log_softmax(z, dim=1).gather(1, torch.where(used, teacher_ids, 0).long())
-    # Where an entry has no probability its term is zero whatever the student gives it.
-    term = torch.where(used & (p > 0), p * (log_p - log_q), torch.zeros_like(p))
+    # Where an entry has no probability its term is zero whatever the student gives it (NaN is not zero).
+    term = torch.where(used & (p != 0), p * (log_p - log_q), torch.zeros_like(p))
     return term.sum(1) * temperature**2
 
 

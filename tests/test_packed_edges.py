@@ -1,0 +1,21 @@
+"""Packed documents and distillation on torch operations, where values and calls are out of the ordinary."""
+
+import math
+
+import pytest
+import torch
+
+from bergson_b200 import ops
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_distillation_of_teacher_logits_that_are_not_finite(value):
+    """Such an entry has no distribution: NaN, unless the entry is not one."""
+    z = torch.randn(4, 9, requires_grad=True)
+    ids, t = torch.tensor([[1, 2], [3, 4], [5, -1], [0, 6]]), torch.randn(4, 2)
+    t[1, 0] = value
+    t[2, 1] = value
+    loss = ops.token_distillation(z, ids, t, 1.5)
+    (g,) = torch.autograd.grad(loss.sum(), z)
+    assert torch.isnan(loss[1]) and torch.isnan(g[1, [3, 4]]).all()
+    assert torch.isfinite(loss[[0, 2, 3]]).all() and torch.isfinite(g[[0, 2, 3]]).all()

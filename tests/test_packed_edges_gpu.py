@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from bergson_b200 import ops
+from bergson_b200.ops.functional import token_distillation_ref
 
 from .packed_bounds import attention_bounds64, far_values
 from .packed_reference import assert_within, attention64
@@ -175,3 +176,22 @@ def test_distillation_nan_among_masked_logits(native, T, V, dtype):
         others = [0] + list(range(2, T))
         assert torch.isnan(loss[1]) and torch.isnan(g[1]).all(), at
         assert torch.isfinite(loss[others]).all() and torch.isfinite(g[others]).all()
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("T", [4, 700])
+def test_distillation_of_teacher_logits_that_are_not_finite(native, T, value):
+    """NaN as on torch operations, unless the entry is not one; other rows are as they were."""
+    z, t = _rand((T, 1003), torch.bfloat16, 772), _rand((T, 5), torch.float32, 773)
+    ids = torch.randint(0, 1003, (T, 5), device="cuda")
+    ids[2, 1] = -1
+    t[1, 0] = t[2, 1] = value
+    leaf = z.requires_grad_()
+    loss = ops.token_distillation(leaf, ids, t, 1.5)
+    (g,) = torch.autograd.grad(loss.sum(), leaf)
+    want = token_distillation_ref(z.detach().double(), ids, t.double(), 1.5)
+    assert torch.equal(torch.isnan(loss), torch.isnan(want)) and torch.isnan(loss[1])
+    assert torch.isnan(g[1, ids[1]]).all()
+    others = [i for i in range(T) if i != 1]
+    torch.testing.assert_close(loss[others].double(), want[others], rtol=1e-5, atol=1e-5)
+    assert torch.isfinite(g[others]).all()
