@@ -252,6 +252,13 @@ at::Tensor distill_bwd(at::Tensor logits, at::Tensor ids, at::Tensor teacher, at
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// The kernels have no forward-mode derivatives; a tangent that came along would be lost without a word.
+void refuse_tangents(std::initializer_list<const at::Tensor*> inputs, const char* what) {
+  for (const auto* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "bergson_b200: ", what,
+                                " on the kernels has no forward-mode derivative");
+}
+
 bool tracked(std::initializer_list<const at::Tensor*> inputs, const char* what) {
   if (!at::GradMode::is_enabled()) return false;
   bool any = false;
@@ -309,6 +316,7 @@ struct PackedAttentionFn : torch::autograd::Function<PackedAttentionFn> {
 at::Tensor packed_attention(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor first_key, at::Tensor end_query,
                             at::Tensor query_tiles, at::Tensor query_pairs, at::Tensor key_tiles, int64_t valid,
                             double scale) {
+  refuse_tangents({&q, &k, &v}, "packed_causal_attention");
   if (tracked({&q, &k, &v}, "packed_causal_attention"))
     return PackedAttentionFn::apply(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale);
   return packed_attention_fwd(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale, false)[0];
@@ -336,6 +344,7 @@ struct PackedRotaryFn : torch::autograd::Function<PackedRotaryFn> {
 
 std::tuple<at::Tensor, at::Tensor> packed_rotary(at::Tensor q, at::Tensor k, at::Tensor cos, at::Tensor sin,
                                                  at::Tensor position, int64_t rot) {
+  refuse_tangents({&q, &k, &cos, &sin}, "packed_rotary");
   auto out = tracked({&q, &k}, "packed_rotary") ? PackedRotaryFn::apply(q, k, cos, sin, position, rot)
                                : packed_rotary_turn(q, k, cos, sin, position, rot, false);
   return {out[0], out[1]};
@@ -362,6 +371,7 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
 };
 
 at::Tensor distill(at::Tensor logits, at::Tensor ids, at::Tensor teacher, double temperature) {
+  refuse_tangents({&logits, &teacher}, "token_distillation");
   ids = ids.contiguous();
   teacher = teacher.contiguous();
   if (tracked({&logits}, "token_distillation")) return DistillFn::apply(logits, ids, teacher, temperature);

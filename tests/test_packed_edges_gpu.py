@@ -195,3 +195,31 @@ def test_distillation_of_teacher_logits_that_are_not_finite(native, T, value):
     others = [i for i in range(T) if i != 1]
     torch.testing.assert_close(loss[others].double(), want[others], rtol=1e-5, atol=1e-5)
     assert torch.isfinite(g[others]).all()
+
+
+@pytest.mark.parametrize("place", [0, 1, 2])
+def test_forward_mode_derivatives_are_refused(native, place):
+    """The kernels have no tangents: a dual tensor is refused and not computed without its tangent."""
+    import torch.autograd.forward_ad as fw
+
+    p = ops.PackedSequences([20], device="cuda")
+    q, k, v = (_rand((20, 2, 64), torch.float32, 780 + i) for i in range(3))
+    cos, sin = ops.rotary_tables(20, 64, 1e4, "cuda")
+    z, ids, t = _rand((20, 90), torch.float32, 783), torch.randint(0, 90, (20, 3), device="cuda"), _rand((20, 3), torch.float32, 784)
+    with fw.dual_level():
+        def dual(*xs):
+            return [fw.make_dual(x, torch.ones_like(x)) if i == place else x for i, x in enumerate(xs)]
+
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            ops.packed_causal_attention(*dual(q, k, v), p)
+        with pytest.raises((RuntimeError, NotImplementedError)), torch.no_grad():
+            ops.packed_causal_attention(*dual(q, k, v), p)
+        x = [*dual(q, k), cos, sin] if place < 2 else [q, k, fw.make_dual(cos, torch.ones_like(cos)), sin]
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            ops.packed_rotary(*x, 64, p)
+        if place < 2:
+            a, b = dual(z, t)
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                ops.token_distillation(a, ids, b)
+            with ops.composable():
+                assert fw.unpack_dual(ops.token_distillation(a, ids, t)).tangent is not None or place == 1
