@@ -7,6 +7,9 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
 
+#include <cstring>
+#include <mutex>
+
 #include "bindings.h"
 #include "kernels_distill.h"
 #include "kernels_packed.h"
@@ -51,6 +54,45 @@ void check_packed(const at::Tensor& q, const at::Tensor& k) {
   TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 3 && q.size(0) == k.size(0) && q.size(2) == k.size(2) &&
                   q.scalar_type() == k.scalar_type() && k.device() == q.device(),
               "bergson_b200: q [T, H, D] and k [T, H_kv, D] of one dtype and device expected");
+}
+
+// One word a device in the host's memory, which kernels that give up on a wait set: a call can look at it without
+// asking the device.
+int* gave_up_word(int device) {
+  constexpr int kMost = 64;
+  static std::mutex mu;
+  static int* words = nullptr;
+  TORCH_CHECK(device >= 0 && device < kMost, "bergson_b200: device ", device);
+  std::lock_guard<std::mutex> lock(mu);
+  if (words == nullptr) {
+    c10::cuda::CUDAStreamCaptureModeGuard relaxed{cudaStreamCaptureModeRelaxed};  // the first call may be captured
+    void* host = nullptr;
+    C10_CUDA_CHECK(cudaHostAlloc(&host, kMost * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
+    std::memset(host, 0, kMost * sizeof(int));
+    words = static_cast<int*>(host);
+  }
+  return words + device;
+}
+
+// Raises if an attention kernel on the device gave up since the status word was last cleared.
+int* check_waits(const at::Tensor& like) {
+  int* word = gave_up_word(like.get_device());
+  volatile int* seen = word;
+  if (*seen == 0) return word;
+  int status = -1;
+  if (at::cuda::currentStreamCaptureStatus() == at::cuda::CaptureStatus::None) {
+    status = kernel_status(like.get_device()).item<int>();
+    if (status == 0) {  // cleared by whoever looked into it
+      *seen = 0;
+      return word;
+    }
+  }
+  TORCH_CHECK(false, "bergson_b200: a kernel of packed_causal_attention gave up on a bounded wait (status ", status,
+              "); its results are incomplete.  ops.native.kernel_status(device).zero_() clears this.");
+}
+
+at::Tensor packed_gave_up(int64_t device) {
+  return at::from_blob(gave_up_word(int(device)), {1}, at::TensorOptions().dtype(at::kInt));
 }
 
 void check_index(const at::Tensor& x, int64_t n, const at::Tensor& like) {
@@ -106,7 +148,8 @@ std::vector<at::Tensor> packed_attention_fwd(at::Tensor q, at::Tensor k, at::Ten
   q = readable(q);
   k = readable(k);
   v = readable(v);
-  const auto a = packed_args(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale);
+  auto a = packed_args(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale);
+  a.gave_up = check_waits(q);
   auto o = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
   auto bias2 = at::empty({q.size(1), a.pitch}, q.options().dtype(at::kFloat));
   at::Tensor rest;
@@ -134,7 +177,8 @@ std::vector<at::Tensor> packed_attention_bwd(at::Tensor d_o, at::Tensor q, at::T
                                     rest->is_contiguous() && rest->device() == o.device()),
               "bergson_b200: the output's rest does not fit the output");
   d_o = readable(d_o);
-  const auto a = packed_args(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale);
+  auto a = packed_args(q, k, v, first_key, end_query, query_tiles, query_pairs, key_tiles, valid, scale);
+  a.gave_up = check_waits(q);
   auto delta = at::empty_like(bias2);
   auto ds_bounds = at::empty({a.type == 0 ? (3 * q.size(1) + k.size(1)) * a.pitch : 0}, bias2.options());
   auto dq = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
@@ -384,4 +428,5 @@ void bgn_register_packed(pybind11::module& m) {
   m.def("packed_attention", &packed_attention);
   m.def("packed_rotary", &packed_rotary);
   m.def("distill", &distill);
+  m.def("packed_gave_up", &packed_gave_up);
 }

@@ -25,6 +25,7 @@ typedef struct {
   int heads, kv_heads, dim;
   int type;                // 0 = fp16, 1 = bf16, 2 = fp32
   float scale;             // > 0
+  int* gave_up;            // a word of the host's, set to 1 where a kernel gives up on a wait (besides its status)
 } BgnPackedAttention;
 
 // o [rows, heads, dim] contiguous and bias2 [heads, pitch]: minus the base-2 logarithm of the softmax

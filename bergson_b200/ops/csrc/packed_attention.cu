@@ -138,6 +138,7 @@ cudaError_t tensor_fwd(const BgnPackedAttention& a, void* o, void* o_rest, float
   p.o = o;
   p.o_rest = o_rest;
   p.bias2 = bias2;
+  p.gave_up = a.gave_up;
   constexpr int smem = fwd_smem_bytes<DP>();
   auto kern = packed_fwd_kernel<FMT, DP>;
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem);
@@ -213,6 +214,7 @@ cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const void* o
   p.dq = dq;
   p.dk = dk;
   p.dv = dv;
+  p.gave_up = a.gave_up;
   auto kq = packed_dq_kernel<FMT, DP>;
   auto kk = packed_dkv_kernel<FMT, DP>;
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kq), dq_smem_bytes<DP>());
@@ -238,7 +240,7 @@ cudaError_t tensor_bwd(const BgnPackedAttention& a, const void* o, const void* o
 bool sound(const BgnPackedAttention* a) {
   return a->rows > 0 && a->pitch >= a->rows && a->pitch % kTile == 0 && a->valid >= 0 && a->valid <= a->rows && a->heads > 0 && a->kv_heads > 0 &&
          a->heads % a->kv_heads == 0 && a->dim >= 8 && a->dim <= 128 && a->dim % 8 == 0 && a->type >= 0 && a->type <= 2 &&
-         a->scale > 0.f;
+         a->scale > 0.f && a->gave_up != nullptr;
 }
 
 }  // namespace

@@ -44,6 +44,7 @@ struct PackedBwdArgs {
   float* doc_delta;  // [heads, pitch]: |delta|, doc
   float* doc_v;      // [kv_heads, pitch]: |v|, doc
   void *dq, *dk, *dv;
+  int* gave_up;
 };
 
 // The power of two that brings `bound` to [2^14, 2^15); 1 where there is nothing to scale.
@@ -258,7 +259,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // Nearly all of the shared memory is in use at 128 features: there is no room for moving up to a boundary.
   if ((smem_u32(smem_raw) & 1023u) != 0) {
-    if (threadIdx.x == 0) atomicCAS(status, kStatusOk, kStatusTimeoutProducer);
+    if (threadIdx.x == 0) record_give_up(status, p.gave_up, kStatusTimeoutProducer);
     return;
   }
   uint8_t* q_tile = smem_raw;
@@ -363,7 +364,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         entry = next;
       }
       if (!ok) {
-        atomicCAS(status, kStatusOk, kStatusTimeoutProducer);
+        record_give_up(status, p.gave_up, kStatusTimeoutProducer);
         drain_copies();
       }
     }
@@ -440,7 +441,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       unit = after;
       entry = next;
     }
-    if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutMma);
+    if (!ok && lane == 0) record_give_up(status, p.gave_up, kStatusTimeoutMma);
   } else {
     using T = typename Type16<FMT>::T;
     const int half = warp >> 2, quad = warp & 3;
@@ -565,7 +566,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (!some && row < p.rows && half == 0)
         for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
     }
-    if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutEpilogue);
+    if (!ok && lane == 0) record_give_up(status, p.gave_up, kStatusTimeoutEpilogue);
     if (ok && __any_sync(0xffffffffu, bad)) {
       __syncwarp();  // the lanes' rows are read by all
       for (int r = 0; (unit = nth_unit(r, p.units)) >= 0; ++r) {
@@ -664,7 +665,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // All of the shared memory is in use at 128 features: there is no room for moving up to a boundary.
   if ((smem_u32(smem_raw) & 1023u) != 0) {
-    if (threadIdx.x == 0) atomicCAS(status, kStatusOk, kStatusTimeoutProducer);
+    if (threadIdx.x == 0) record_give_up(status, p.gave_up, kStatusTimeoutProducer);
     return;
   }
   uint8_t* k_tile = smem_raw;
@@ -780,7 +781,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         entry = next;
       }
       if (!ok) {
-        atomicCAS(status, kStatusOk, kStatusTimeoutProducer);
+        record_give_up(status, p.gave_up, kStatusTimeoutProducer);
         drain_copies();
       }
     }
@@ -871,7 +872,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       unit = after;
       entry = next;
     }
-    if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutMma);
+    if (!ok && lane == 0) record_give_up(status, p.gave_up, kStatusTimeoutMma);
   } else {
     using T = typename Type16<FMT>::T;
     const int half = warp >> 2, quad = warp & 3;
@@ -1019,7 +1020,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (!in && key < p.rows)
         for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
     }
-    if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutEpilogue);
+    if (!ok && lane == 0) record_give_up(status, p.gave_up, kStatusTimeoutEpilogue);
     if (ok && __any_sync(0xffffffffu, bad)) {
       __syncwarp();  // the lanes' rows are read by all
       for (int r = 0; (unit = nth_unit(r, p.units)) >= 0; ++r) {

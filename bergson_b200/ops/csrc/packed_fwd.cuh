@@ -63,6 +63,7 @@ struct PackedFwdArgs {
   void* o;
   void* o_rest;  // what rounding took from o, for the backward pass (may be null)
   float* bias2;
+  int* gave_up;
 };
 
 // The r-th unit of a block, -1 behind the last: units come most work first, so the blocks take them in
@@ -354,7 +355,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           entry[1] = next[1];
         }
         if (!ok) {
-          atomicCAS(status, kStatusOk, kStatusTimeoutProducer);
+          record_give_up(status, p.gave_up, kStatusTimeoutProducer);
           drain_copies();
         }
       }
@@ -392,7 +393,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         entry[0] = next[0];
         entry[1] = next[1];
       }
-      if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutMma);
+      if (!ok && lane == 0) record_give_up(status, p.gave_up, kStatusTimeoutMma);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -527,7 +528,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (!some && row < p.rows)
         for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
     }
-    if (!ok && lane == 0) atomicCAS(status, kStatusOk, kStatusTimeoutEpilogue);
+    if (!ok && lane == 0) record_give_up(status, p.gave_up, kStatusTimeoutEpilogue);
     if (ok && __any_sync(0xffffffffu, bad)) {
       __syncwarp();  // the lanes' rows are read by all
       for (int r = 0; (unit = nth_unit(r, p.units)) >= 0; ++r) {

@@ -178,6 +178,13 @@ __device__ __forceinline__ float warp_dot(const float (&x)[N], const float (&y)[
 __device__ __forceinline__ void next_kernel_may_come() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_last_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Records a wait that ran out: in the status word, then where the host sees it without asking the device.
+__device__ __forceinline__ void record_give_up(int* status, int* gave_up, int code) {
+  atomicCAS(status, kStatusOk, code);
+  __threadfence_system();
+  *reinterpret_cast<volatile int*>(gave_up) = 1;
+}
+
 // Gives up after a wait that ran out: long enough for every copy in flight to land.
 __device__ __forceinline__ void drain_copies() {
   const long long start = clock64();

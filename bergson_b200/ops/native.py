@@ -78,7 +78,7 @@ def ext():
 _launches = 0
 # Number of kernel launches behind one call of each extension function (helpers such as the
 # reduction of per-block partial sums are torch ops and are not counted).
-_KERNELS_PER_CALL = {"kernel_status": 0}
+_KERNELS_PER_CALL = {"kernel_status": 0, "packed_gave_up": 0}
 
 
 def launch_count() -> int:

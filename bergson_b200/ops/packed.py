@@ -161,6 +161,9 @@ def packed_causal_attention(q: Tensor, k: Tensor, v: Tensor, packing: PackedSequ
     get zero gradients.  ``scale`` (default ``1 / sqrt(D)``) must be positive.  The kernels take bf16, fp16 and fp32 with D a
     multiple of 8 up to 128; views of a fused projection are read in place.  Other dtypes and head sizes
     run document by document on torch operations.
+
+    A kernel that gives up on one of its bounded waits leaves its results incomplete; the next call on that device
+    raises (``ops.attribution.kernel_status`` tells at once, by waiting for the device).
     """
     _check("packed_causal_attention", packing, q, k, v)
     if k.shape != v.shape:

@@ -223,3 +223,24 @@ def test_forward_mode_derivatives_are_refused(native, place):
                 ops.token_distillation(a, ids, b)
             with ops.composable():
                 assert fw.unpack_dual(ops.token_distillation(a, ids, t)).tangent is not None or place == 1
+
+
+def test_a_wait_that_ran_out_is_raised_by_the_next_call(native):
+    """The words that a kernel which gives up sets, set here by the host: calls raise until the status is cleared."""
+    p = ops.PackedSequences([20], device="cuda")
+    q, k, v = (_rand((20, 2, 64), torch.bfloat16, 790 + i).requires_grad_() for i in range(3))
+    o = ops.packed_causal_attention(q, k, v, p)
+    want, word = o.detach().clone(), native.packed_gave_up(0)
+    assert word.item() == 0
+    try:
+        native.kernel_status(0).fill_(2)
+        word.fill_(1)
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match="gave up"):
+                ops.packed_causal_attention(q, k, v, p)
+        with pytest.raises(RuntimeError, match="gave up"):
+            torch.autograd.grad(o.sum(), q, retain_graph=True)
+    finally:
+        native.kernel_status(0).zero_()
+    assert torch.equal(ops.packed_causal_attention(q, k, v, p), want) and word.item() == 0
+    assert torch.isfinite(torch.autograd.grad(o.sum(), q)[0]).all()
