@@ -412,12 +412,15 @@ def _causal_bias(S: int, dtype: torch.dtype, device) -> Tensor:
     if bias is None:
         if len(_CAUSAL_BIAS) > 16:
             _CAUSAL_BIAS.clear()
-        bias = torch.full((S, S), float("-inf"), dtype=dtype, device=device).triu_(1)
-        _CAUSAL_BIAS[key] = bias
+        bias = _CAUSAL_BIAS[key] = new_causal_bias(S, dtype, device)
     return bias
 
 
-def causal_attention_ref(q: Tensor, k: Tensor, v: Tensor, scale: float) -> Tensor:
+def new_causal_bias(S: int, dtype: torch.dtype, device) -> Tensor:
+    return torch.full((S, S), float("-inf"), dtype=dtype, device=device).triu_(1)
+
+
+def causal_attention_ref(q: Tensor, k: Tensor, v: Tensor, scale: float, bias: Tensor | None = None) -> Tensor:
     # Explicit softmax(QK^T)V: differentiable to any order on every backend.  Three passes
     # over the [B, H, S, S] scores instead of six: the scale goes onto q, the causal mask
     # is the additive input of the batched product, and the softmax reads and writes the
@@ -428,7 +431,8 @@ def causal_attention_ref(q: Tensor, k: Tensor, v: Tensor, scale: float) -> Tenso
         rep = Hq // Hkv
         k = k.repeat_interleave(rep, dim=1)
         v = v.repeat_interleave(rep, dim=1)
-    bias = _causal_bias(S, q.dtype, q.device)
+    if bias is None:
+        bias = _causal_bias(S, q.dtype, q.device)
     att = torch.baddbmm(bias, (q * scale).reshape(B * Hq, S, D), k.reshape(B * Hq, S, D).transpose(1, 2))
     att = _softmax_last(att)
     return torch.bmm(att, v.reshape(B * Hq, S, D)).view(B, Hq, S, D)

@@ -18,7 +18,7 @@ import torch
 from torch import Tensor
 
 from . import native
-from .functional import causal_attention_ref, rotary_pairs, use_fused
+from .functional import causal_attention_ref, new_causal_bias, rotary_pairs, use_fused
 
 _TILE = 128  # rows of the kernels' tiles
 _KERNEL_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -142,9 +142,10 @@ def _check(name: str, packing: PackedSequences, q: Tensor, *others: Tensor) -> N
 def packed_causal_attention_ref(q: Tensor, k: Tensor, v: Tensor, packing: PackedSequences, scale: float) -> Tensor:
     """Document by document with differentiable torch operations."""
     parts = []
+    bias = new_causal_bias(packing.max_length, q.dtype, q.device)  # the longest document's; every other one is a corner of it
     for begin, end in packing.spans():
         one = [x[begin:end].transpose(0, 1)[None] for x in (q, k, v)]
-        parts.append(causal_attention_ref(*one, scale)[0].transpose(0, 1))
+        parts.append(causal_attention_ref(*one, scale, bias[: end - begin, : end - begin])[0].transpose(0, 1))
     if packing.rows > packing.num_tokens or not parts:
         behind = q[packing.num_tokens :]  # zeros that stay in the graph, whatever stands there
         parts.append(behind.masked_fill(torch.ones((), dtype=torch.bool, device=q.device), 0.0))

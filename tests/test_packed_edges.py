@@ -19,3 +19,13 @@ def test_distillation_of_teacher_logits_that_are_not_finite(value):
     (g,) = torch.autograd.grad(loss.sum(), z)
     assert torch.isnan(loss[1]) and torch.isnan(g[1, [3, 4]]).all()
     assert torch.isfinite(loss[[0, 2, 3]]).all() and torch.isfinite(g[[0, 2, 3]]).all()
+
+
+def test_documents_of_many_lengths_leave_no_masks_behind():
+    from bergson_b200.ops import functional
+
+    before = dict(functional._CAUSAL_BIAS)
+    lens = list(range(1, 40))
+    q = torch.randn(sum(lens), 1, 8)
+    ops.packed_causal_attention(q, q, q, ops.PackedSequences(lens))
+    assert functional._CAUSAL_BIAS.keys() == before.keys()
