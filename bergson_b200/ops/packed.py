@@ -147,7 +147,8 @@ def packed_causal_attention_ref(q: Tensor, k: Tensor, v: Tensor, packing: Packed
         one = [x[begin:end].transpose(0, 1)[None] for x in (q, k, v)]
         parts.append(causal_attention_ref(*one, scale, bias[: end - begin, : end - begin])[0].transpose(0, 1))
     if packing.rows > packing.num_tokens or not parts:
-        behind = q[packing.num_tokens :]  # zeros that stay in the graph, whatever stands there
+        # zeros that stay in the graph, whatever stands there
+        behind = q[packing.num_tokens :] if parts else q + (k.sum() + v.sum())
         parts.append(behind.masked_fill(torch.ones((), dtype=torch.bool, device=q.device), 0.0))
     return torch.cat(parts)
 
@@ -176,7 +177,7 @@ def packed_causal_attention(q: Tensor, k: Tensor, v: Tensor, packing: PackedSequ
         raise ValueError(f"packed_causal_attention: scale must be positive, got {scale}")
     if q.dtype in _KERNEL_DTYPES and q.shape[2] % 8 == 0 and q.shape[2] <= 128 and use_fused(q):
         if q.numel() == 0:
-            return q * 1.0  # no rows or no heads: nothing to launch
+            return q + (k.sum() + v.sum())  # no rows or no heads: nothing to launch, and a place in the graph
         return native.packed_attention(q, k, v, *packing.tables(), packing.num_tokens, scale)
     return packed_causal_attention_ref(q, k, v, packing, scale)
 

@@ -29,3 +29,24 @@ def test_documents_of_many_lengths_leave_no_masks_behind():
     q = torch.randn(sum(lens), 1, 8)
     ops.packed_causal_attention(q, q, q, ops.PackedSequences(lens))
     assert functional._CAUSAL_BIAS.keys() == before.keys()
+
+
+def check_empty_batches(device, dtype):
+    """No rows, or rows of no document: every operand has a gradient, of zeros."""
+    for rows in (0, 5):
+        for lens in ([], [0, 0]):
+            q, k, v = (torch.randn(rows, h, 64, device=device, dtype=dtype, requires_grad=True) for h in (4, 2, 2))
+            with torch.no_grad():
+                for x in (q, k, v):
+                    x[1:] = math.nan
+            p = ops.PackedSequences(lens, device=device, total=rows)
+            for only in (q, k, v):
+                xs = [x if x is only else x.detach() for x in (q, k, v)]
+                o = ops.packed_causal_attention(*xs, p)
+                assert o.shape == q.shape and o.dtype == dtype and (o == 0).all() and o.requires_grad
+            grads = torch.autograd.grad(ops.packed_causal_attention(q, k, v, p).sum(), (q, k, v))
+            assert all(g.shape == x.shape and (g == 0).all() for g, x in zip(grads, (q, k, v)))
+
+
+def test_empty_batches():
+    check_empty_batches("cpu", torch.float64)

@@ -10,6 +10,7 @@ from bergson_b200.ops.functional import token_distillation_ref
 
 from .packed_bounds import attention_bounds64, far_values
 from .packed_reference import assert_within, attention64
+from .test_packed_edges import check_empty_batches
 from .test_packed_gpu import DTYPES, _attend, _rand, native  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -244,3 +245,8 @@ def test_a_wait_that_ran_out_is_raised_by_the_next_call(native):
         native.kernel_status(0).zero_()
     assert torch.equal(ops.packed_causal_attention(q, k, v, p), want) and word.item() == 0
     assert torch.isfinite(torch.autograd.grad(o.sum(), q)[0]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_empty_batches_have_gradients_for_all_operands(native, dtype):
+    check_empty_batches("cuda", dtype)
