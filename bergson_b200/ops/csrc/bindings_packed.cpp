@@ -2,6 +2,7 @@
 // allocation of outputs, current-stream lookup.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
@@ -95,6 +96,12 @@ at::Tensor packed_gave_up(int64_t device) {
   return at::from_blob(gave_up_word(int(device)), {1}, at::TensorOptions().dtype(at::kInt));
 }
 
+// The plan's table was allocated on the stream that was current then and may be dropped while kernels of another one
+// still read it.
+void keep_plan(const at::Tensor& part) {
+  c10::cuda::CUDACachingAllocator::recordStream(part.storage().data_ptr(), at::cuda::getCurrentCUDAStream());
+}
+
 void check_index(const at::Tensor& x, int64_t n, const at::Tensor& like) {
   TORCH_CHECK(x.scalar_type() == at::kInt && x.is_contiguous() && x.device() == like.device() && x.numel() == n,
               "bergson_b200: the packing does not fit the tensors");
@@ -137,6 +144,7 @@ BgnPackedAttention packed_args(const at::Tensor& q, const at::Tensor& k, const a
   a.dim = int(q.size(2));
   a.type = type_of(q);
   a.scale = float(scale);
+  keep_plan(first_key);  // one storage holds all of the plan
   return a;
 }
 
@@ -197,6 +205,7 @@ std::vector<at::Tensor> packed_rotary_turn(at::Tensor q, at::Tensor k, at::Tenso
   c10::cuda::CUDAGuard guard(q.device());
   check_packed(q, k);
   check_index(position, q.size(0), q);
+  keep_plan(position);
   TORCH_CHECK(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat && cos.is_contiguous() &&
                   sin.is_contiguous() && cos.sizes() == sin.sizes() && cos.dim() == 2 && cos.size(1) == rot / 2 &&
                   cos.device() == q.device() && sin.device() == q.device(),

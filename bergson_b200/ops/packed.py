@@ -30,8 +30,8 @@ class PackedSequences:
     ``lengths``: the documents' lengths in their order (0 allowed), on the host.  ``total``: rows of the
     batch's tensors (default: the sum of the lengths); the rows behind the last document belong to
     nobody: attention gives zeros there.  The plan's tensors are on ``device`` when the constructor
-    returns, so any stream may use them; a captured graph replays the lengths it was captured with, and
-    a plan is made before a capture begins.
+    returns, so any stream may use them, and the plan may be dropped while it does.  A plan is made before a
+    capture begins; the captured graph replays its lengths, so it is kept as long as the graph is.
     """
 
     def __init__(self, lengths: Sequence[int] | np.ndarray | Tensor, device="cpu", total: int | None = None):

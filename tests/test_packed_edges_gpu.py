@@ -250,3 +250,27 @@ def test_a_wait_that_ran_out_is_raised_by_the_next_call(native):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_empty_batches_have_gradients_for_all_operands(native, dtype):
     check_empty_batches("cuda", dtype)
+
+
+def test_a_dropped_plan_stays_until_other_streams_have_read_it(native):
+    """A plan made on one stream, used on another and dropped at once: its memory is not given away before."""
+    side, lens = torch.cuda.Stream(), [100] * 300
+    q, k, v = (_rand((30000, 1, 64), torch.bfloat16, 800 + i) for i in range(3))
+    cos, sin = ops.rotary_tables(100, 64, 1e4, "cuda")
+    torch.cuda.synchronize()
+    for call in (lambda p: ops.packed_causal_attention(q, k, v, p), lambda p: ops.packed_rotary(q, k, cos, sin, 64, p)):
+        with torch.no_grad():
+            call(ops.PackedSequences(lens, device="cuda"))  # the kernels' code is loaded
+        torch.cuda.synchronize()
+        p = ops.PackedSequences(lens, device="cuda")
+        storage = p.first_key.untyped_storage()
+        at, size = storage.data_ptr(), storage.nbytes()
+        with torch.cuda.stream(side), torch.no_grad():
+            torch.cuda._sleep(100_000_000)  # some 50 ms
+            out = call(p)
+        del p, storage
+        assert not side.query()
+        others = [torch.empty(size, device="cuda", dtype=torch.uint8) for _ in range(8)]
+        assert all(not at <= x.data_ptr() < at + size for x in others)
+        torch.cuda.synchronize()
+        del out, others
