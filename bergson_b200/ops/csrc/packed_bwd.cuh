@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(delta_threads<FMT, LANES>()) packed_delta_kern
 // Delta comes from a kernel of its own: read here, by softmax warps or by others, o and do took as long as
 // two to four key tiles, as loads through the first-level cache wait for the tensor core's operands.
 //
-// Bound by the tensor core (three products of 1024 cycles a tile at 128 features) and the softmax warps in turn:
+// Bound by the tensor core (three products of 512 cycles a tile at 128 features) and the softmax warps in turn:
 // 32 over 8 heads of 128 in bf16, one document of 8192 tokens 0.63 ms (1320 TFLOP/s of its three products).
 
 constexpr int kDqKStages = 3;  // a key tile stays until dQ of its step, which comes after S and dP of the next
@@ -607,6 +607,10 @@ template <int DP>
 constexpr int dkv_smem_bytes() {
   return (2 + kDkvQStages + kDkvGStages) * tile_bytes<DP>() + kDkvGStages * kDkvRowBytes + 512;
 }
+
+// A block of dK, dV that came early holds its TMEM until all of dQ has ended.  A block of dQ that had to wait for it on
+// the same SM would wait for good, so there is no room for both (228 KB to an SM, 1 KB of them kept for each block).
+static_assert(dq_smem_bytes<64>() + dkv_smem_bytes<64>() + 2 * 1024 > 228 * 1024, "dQ and dK, dV must not share an SM");
 
 // A warp puts right a row of dV (half 0) or of dK, of the tile of keys whose queries are [row0, last).
 template <int FMT, int DP>
