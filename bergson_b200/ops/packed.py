@@ -87,10 +87,11 @@ class PackedSequences:
         key = key[np.argsort(-(key[:, 1] - key[:, 0]), kind="stable")]
         parts = [query, pairs, key, first_key, end_query, position, np.concatenate([[0], ends])]
         flat = np.concatenate([x.reshape(-1) for x in parts]).astype(np.int32)
-        table = torch.from_numpy(flat).to(device)
+        with torch.inference_mode(False):  # a graph may save the tables, wherever the plan was made
+            table = torch.from_numpy(flat).to(device)
+            (self.query_tiles, self.query_pairs, self.key_tiles, self.first_key, self.end_query, self.position,
+             self.cu_seqlens) = table.split([x.size for x in parts])
         self.device = table.device
-        (self.query_tiles, self.query_pairs, self.key_tiles, self.first_key, self.end_query, self.position,
-         self.cu_seqlens) = table.split([x.size for x in parts])
         self._tables = (self.first_key, self.end_query, self.query_tiles, self.query_pairs, self.key_tiles)
 
     def __repr__(self) -> str:

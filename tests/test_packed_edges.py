@@ -50,3 +50,15 @@ def check_empty_batches(device, dtype):
 
 def test_empty_batches():
     check_empty_batches("cpu", torch.float64)
+
+
+def test_a_plan_made_in_inference_mode_serves_training():
+    with torch.inference_mode():
+        p = ops.PackedSequences([3, 2])
+    x = torch.randn(5, 2, 8, requires_grad=True)
+    cos, sin = ops.rotary_tables(3, 8, 1e4, "cpu")
+    q, k = ops.packed_rotary(x, x, cos, sin, 8, p)
+    (g,) = torch.autograd.grad(ops.packed_causal_attention(q, k, x, p).sum(), x)
+    assert torch.isfinite(g).all()
+    emb = torch.nn.Embedding(3, 4)
+    emb(p.position).sum().backward()
